@@ -208,7 +208,7 @@ def _own_w4(s):
 
 def _own_clip(s):
     from disagmoe_amd.ops import grads
-    norm = grads.clip_grad_norm_(s["grads"], s["max_norm"])
+    norm = grads.clip_by_global_norm_(s["grads"], s["max_norm"])
     return {"norm": norm, "grads": s["flat"]}
 
 
