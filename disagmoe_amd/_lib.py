@@ -3,7 +3,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_int, c_int64, c_size_t, c_void_p, POINTER
+from ctypes import c_char_p, c_double, c_int, c_int64, c_size_t, c_void_p, POINTER
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libdmoe_hip.so")
@@ -57,6 +57,8 @@ SIGNATURES = {
                              c_int64, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
     "dmoe_gmm_fp8_swiglu": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int,
                                     c_int64, c_int64, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "dmoe_grad_norm": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "dmoe_clip_grads": (c_int, [c_void_p, c_int64, c_double, c_void_p, c_void_p, c_size_t, c_void_p]),
 }
 
 #: exported for the library's own tests and benchmarks, not declared in include/dmoe.h (csrc/tuning.h)
@@ -65,6 +67,7 @@ TEST_HOOKS = {
     "dmoe_gmm_plan": (c_int, [c_void_p, c_int, c_int64, c_int, c_int64, c_int64, c_int, c_int, c_int, c_size_t, c_void_p]),
 }
 GMM_STATE_BYTES = 33024
+GRAD_WORKSPACE_BYTES = 8192
 
 
 

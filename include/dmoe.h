@@ -307,6 +307,26 @@ int dmoe_gmm_fp8_swiglu(const void *a, const float *a_scale, const void *b, cons
                         int64_t I, void *state, void *workspace, size_t workspace_bytes,
                         const int64_t *host_batch_sizes, void *stream);
 
+/* ---- gradients: no counterpart in the reference -----------------------------
+ * Global norm of many gradients and clipping to a largest norm:
+ *     norm = sqrt(sum over every element of every tensor of g^2)        (64-bit sums in a fixed order)
+ *     coef = min(1, max_norm / (norm + 1e-6)),  g <- g * coef           (fp32 product, one rounding)
+ * `grads` is an array of n descriptions in HOST memory, read during the call only (a recorded launch holds its own
+ * copy): any number of tensors, each of DMOE_FP32, DMOE_BF16 or DMOE_FP16, of any length, aligned to its elements, dense.
+ * `norm` [1] fp32 on the device.  A norm below the limit writes no gradient; an infinite norm scales by zero (infinite
+ * gradients become NaN), a NaN norm makes every gradient NaN.  dmoe_clip_grads refuses tensors that share memory.
+ * `workspace`: DMOE_GRAD_WORKSPACE_BYTES, 8-byte aligned, any contents; calls that may overlap need their own. */
+typedef struct dmoe_grad {
+    void *data;
+    int64_t numel;
+    int dtype;
+} dmoe_grad;
+#define DMOE_GRAD_WORKSPACE_BYTES 8192
+int dmoe_grad_norm(const dmoe_grad *grads, int64_t n, float *norm, void *workspace, size_t workspace_bytes,
+                   void *stream);
+int dmoe_clip_grads(const dmoe_grad *grads, int64_t n, double max_norm, float *norm, void *workspace,
+                    size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
