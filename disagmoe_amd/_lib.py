@@ -57,6 +57,13 @@ SIGNATURES = {
                              c_int64, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
     "dmoe_gmm_fp8_swiglu": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int,
                                     c_int64, c_int64, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "dmoe_gmm_swiglu_keep": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int64, c_int64, c_int,
+                                     c_int, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "dmoe_gmm_swiglu_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                                         c_int, c_int64, c_int64, c_int, c_int, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "dmoe_gmm_wgrad": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int64, c_int64, c_int, c_void_p, c_void_p,
+                               c_size_t, c_void_p, c_void_p]),
+    "dmoe_zero_rows_behind": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int64, c_int, c_void_p]),
     "dmoe_grad_norm": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]),
     "dmoe_clip_grads": (c_int, [c_void_p, c_int64, c_double, c_void_p, c_void_p, c_size_t, c_void_p]),
 }

@@ -676,6 +676,55 @@ extern "C" int dmoe_gmm_swiglu(const void *a, const void *b, void *h, const int6
                    : launch_by_rows<false, true, false>(args, (hipStream_t)stream);
 }
 
+extern "C" int dmoe_gmm_swiglu_keep(const void *a, const void *b, void *h, void *u, const int64_t *batch_sizes, int64_t rows, int E,
+                                    int64_t K, int64_t I, int trans_b, int dtype, void *state, void *workspace,
+                                    size_t workspace_bytes, const int64_t *host_batch_sizes, void *stream) {
+    DMOE_REQUIRE(dtype == DMOE_BF16, DMOE_ERR_DTYPE, "dmoe_gmm_swiglu_keep: dtype %d (bf16 only)", dtype);
+    int rc = check_gmm("dmoe_gmm_swiglu_keep", a, b, h, batch_sizes, rows, E, K, I, 8);
+    if (rc != DMOE_OK) return rc;
+    DMOE_REQUIRE(rows == 0 || u != nullptr, DMOE_ERR_ARG, "dmoe_gmm_swiglu_keep: null pointer");
+    rc = dmoe_gmm(a, b, u, batch_sizes, rows, E, K, 2 * I, trans_b, dtype, state, workspace, workspace_bytes, host_batch_sizes, stream);
+    if (rc != DMOE_OK || rows == 0) return rc;
+    return launch_swiglu_forward(u, h, batch_sizes, rows, E, I, (hipStream_t)stream);
+}
+
+extern "C" int dmoe_gmm_wgrad(const void *a, const void *dc, void *db, const int64_t *batch_sizes, int64_t rows, int E,
+                              int64_t K, int64_t N, int dtype, void *state, void *workspace, size_t workspace_bytes,
+                              const int64_t *host_batch_sizes, void *stream) {
+    const HostSizes known(host_batch_sizes);
+    DMOE_REQUIRE(dtype == DMOE_BF16, DMOE_ERR_DTYPE, "dmoe_gmm_wgrad: dtype %d (bf16 only)", dtype);
+    int rc = check_shape("dmoe_gmm_wgrad", rows, E, K, N, 8);
+    if (rc != DMOE_OK) return rc;
+    DMOE_REQUIRE(batch_sizes != nullptr && db != nullptr && (rows == 0 || (a != nullptr && dc != nullptr)), DMOE_ERR_ARG,
+                 "dmoe_gmm_wgrad: null pointer");
+    DMOE_REQUIRE(db != a && db != dc, DMOE_ERR_ARG, "dmoe_gmm_wgrad: the result overlaps an input");
+    GmmArgs args{(const char *)a, (const char *)dc, (char *)db, batch_sizes, nullptr, nullptr, rows, E, (int)K, (int)N, (int)N};
+    rc = bind_state(args, state, workspace, workspace_bytes, (hipStream_t)stream);
+    if (rc != DMOE_OK) return rc;
+    return launch_wgrad(args, (hipStream_t)stream);
+}
+
+extern "C" int dmoe_gmm_swiglu_backward(const void *dh, const void *u, const void *a, const void *b, void *du, void *da, void *db,
+                                        const int64_t *batch_sizes, int64_t rows, int E, int64_t K, int64_t I, int trans_b,
+                                        int dtype, void *state, void *workspace, size_t workspace_bytes,
+                                        const int64_t *host_batch_sizes, void *stream) {
+    DMOE_REQUIRE(dtype == DMOE_BF16, DMOE_ERR_DTYPE, "dmoe_gmm_swiglu_backward: dtype %d (bf16 only)", dtype);
+    int rc = check_shape("dmoe_gmm_swiglu_backward", rows, E, K, I, 8);
+    if (rc != DMOE_OK) return rc;
+    DMOE_REQUIRE(batch_sizes != nullptr && (da == nullptr || b != nullptr), DMOE_ERR_ARG, "dmoe_gmm_swiglu_backward: null pointer");
+    DMOE_REQUIRE(rows == 0 || (dh != nullptr && u != nullptr && du != nullptr && (db == nullptr || a != nullptr)), DMOE_ERR_ARG,
+                 "dmoe_gmm_swiglu_backward: null pointer");
+    if (rows > 0) {
+        DMOE_REQUIRE(du != u && du != dh && da != dh && da != a, DMOE_ERR_ARG, "dmoe_gmm_swiglu_backward: a result overlaps an input");
+        rc = launch_swiglu_backward(dh, u, du, batch_sizes, rows, E, I, da, K, (hipStream_t)stream);
+        if (rc == DMOE_OK && da != nullptr)
+            rc = dmoe_gmm(du, b, da, batch_sizes, rows, E, 2 * I, K, !trans_b, dtype, state, workspace, workspace_bytes, host_batch_sizes, stream);
+    }
+    if (rc != DMOE_OK || db == nullptr) return rc;
+    return trans_b ? dmoe_gmm_wgrad(du, a, db, batch_sizes, rows, E, 2 * I, K, dtype, state, workspace, workspace_bytes, host_batch_sizes, stream)
+                   : dmoe_gmm_wgrad(a, du, db, batch_sizes, rows, E, K, 2 * I, dtype, state, workspace, workspace_bytes, host_batch_sizes, stream);
+}
+
 extern "C" int dmoe_gmm_swiglu_rows(const void *x, const int32_t *row_token, int64_t T, const void *b, void *h,
                                     const int64_t *batch_sizes, int64_t rows, int E, int64_t K, int64_t I, int dtype,
                                     void *state, void *workspace, size_t workspace_bytes,

@@ -366,5 +366,9 @@ int launch_tile256_fp8(const GmmArgs &args, bool swiglu, hipStream_t stream);
 int launch_wave128(const GmmArgs &args, bool swiglu, hipStream_t stream);
 int launch_wave128_fp8(const GmmArgs &args, bool swiglu, hipStream_t stream);
 int launch_tile256_rows(const GmmArgs &args, hipStream_t stream);
+int launch_wgrad(const GmmArgs &args, hipStream_t stream);
+int launch_swiglu_backward(const void *dh, const void *u, void *du, const int64_t *batch_sizes, int64_t rows, int E, int64_t I,
+                           void *da, int64_t K, hipStream_t stream);
+int launch_swiglu_forward(const void *u, void *h, const int64_t *batch_sizes, int64_t rows, int E, int64_t I, hipStream_t stream);
 
 }  // namespace dmoe

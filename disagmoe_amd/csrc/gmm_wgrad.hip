@@ -1,0 +1,256 @@
+// Weight gradient of a grouped product: db[e] = a[rows of e]^T @ dc[rows of e], bf16 in and out, fp32 sums.
+//
+// Bound by the matrix cores (2 rows K N flop) where experts have many rows, by the E K N results that are written where
+// they have few.  A work item is a 256 x 256 tile of one expert's result; its contraction runs over the expert's rows, so
+// both operands arrive with the contraction as their slow dimension.  Their images in LDS are therefore the same: [32 rows]
+// [256 columns], 512 bytes a row, copied there directly (32 KiB a stage, 4 stages, issued 3 stages ahead) and read with
+// ds_read_b64_tr_b16, which transposes 4 rows x 16 columns inside 16 lanes, so that two reads are a 32-deep operand of
+// v_mfma_f32_16x16x32_bf16.  The order of phases is that of gmm_tile256_kernel: the two wavefronts of a SIMD alternate
+// between a stage's operand reads and copies and its 32 MFMAs, handed over by workgroup barriers.
+//
+// An expert's last stage may reach past its rows.  What lies there belongs to the next expert, or to nobody: the copies
+// are aimed at the last row instead (so nothing outside the operands is read), and the lanes that copied write zeros over
+// them once they have landed, in both operands, because a zero in one does not silence an infinity in the other.
+#include "gmm_direct.h"
+
+namespace dmoe {
+
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void gmm_wgrad_kernel(const GmmArgs p) {
+    constexpr int BT = 256, NW = 8, WN = 4;
+    constexpr int TM = 128, TN = 64;
+    constexpr int FM = TM / 16, FN = TN / 16;            // 8 x 4 accumulators of 16 x 16
+    constexpr int CP = 2;                                // copies of 1 KiB per operand, wavefront and stage
+    constexpr int kLoads = 2 * CP;
+    constexpr int kBlock = NW * 1024;
+    constexpr int kImage = BT * kDK * 2;                 // 16 KiB per operand and stage
+    constexpr int kStage = 2 * kImage;
+    constexpr int kStages = 4;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    __shared__ int s_tile_start[kMaxGroups + 1];
+    __shared__ int s_row_start[kMaxGroups + 1];
+    __shared__ long long s_item;
+
+    const int tid = threadIdx.x;
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+    const int E = p.E;
+
+    build_work_list<BT>(p, s_tile_start, s_row_start);
+    __syncthreads();
+
+    const int kt_n = (p.K + BT - 1) / BT, nt_n = (p.N + BT - 1) / BT;
+    const long long per_expert = (long long)kt_n * nt_n;
+    const long long total = per_expert * E;
+    const int G = gridDim.x;
+    const uint32_t pitch_a = (uint32_t)p.K * 2, pitch_d = (uint32_t)p.N * 2;
+    const uint32_t smem_addr = lds_addr(smem);
+    const int streams = (G % kXcds == 0) ? kXcds : 1;
+
+    auto kn_swizzle = [](int k) { return ((k & 3) << 2) ^ (((k >> 3) & 1) << 1); };
+    const int kn_r = 2 * wave + (lane >> 5);               // row of the stage this lane copies; copy i adds 16
+    const int kn_chunk = (lane & 31) ^ kn_swizzle(kn_r);   // which 16 bytes of it
+
+    // operand reads: the 16 lanes of a group address 4 rows x 16 columns (see gmm_tile256.h)
+    const int l16 = lane & 15, g16 = lane >> 4;
+    auto read_off = [&](int slot0) {
+        const int col = slot0 + 4 * (l16 & 3);
+        const int r = g16 * 8 + (l16 >> 2);
+        return r * 512 + (((col >> 3) ^ kn_swizzle(r)) * 16) + (col & 7) * 2;
+    };
+    int fa_off[FM], fb_off[FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i) fa_off[i] = read_off(wm * TM + i * 16);
+#pragma unroll
+    for (int j = 0; j < FN; ++j) fb_off[j] = kImage + read_off(wn * TN + j * 16);
+
+    // ---- state of the item whose copies are being issued ----
+    int e = 0, k0 = 0, n0 = 0, rows_e = 0, S = 0, pre = 0;
+    uint64_t a_base = 0, d_base = 0;
+    uint32_t a_col = 0, d_col = 0;                         // byte offset of this lane's 16 bytes in a row
+    auto open_item = [&](long long q) {
+        const long long L = item_order(q, G, total);
+        e = (int)(L / per_expert);
+        const int idx = (int)(L - e * per_expert);
+        // bands of 4 k-tiles, their n-tiles one after the other, a band's k-tiles innermost: what shares an operand slice
+        // runs side by side on one XCD
+        constexpr int kBand = 4;
+        const int band = idx / (kBand * nt_n);
+        const int width = kt_n - band * kBand < kBand ? kt_n - band * kBand : kBand;
+        const int in = idx - band * kBand * nt_n;
+        n0 = (in / width) * BT;
+        k0 = (band * kBand + in % width) * BT;
+        const int row0 = __builtin_amdgcn_readfirstlane(s_row_start[e]);
+        rows_e = __builtin_amdgcn_readfirstlane(s_row_start[e + 1]) - row0;
+        S = (rows_e + kDK - 1) / kDK;
+        pre = S < kStages ? S : kStages;
+        a_base = to_scalar((uint64_t)(uintptr_t)p.a + (uint64_t)row0 * pitch_a);
+        d_base = to_scalar((uint64_t)(uintptr_t)p.b + (uint64_t)row0 * pitch_d);
+        const int ca = k0 + kn_chunk * 8, cd = n0 + kn_chunk * 8;
+        a_col = (uint32_t)(ca < p.K ? ca : 0) * 2;         // columns past the end read the first one (never stored)
+        d_col = (uint32_t)(cd < p.N ? cd : 0) * 2;
+    };
+    auto issue_copies = [&](int s) {
+        const uint32_t lds = smem_addr + (s % kStages) * kStage + wave * 1024;
+        const uint64_t ab = to_scalar(a_base + (uint64_t)s * kDK * pitch_a), db = to_scalar(d_base + (uint64_t)s * kDK * pitch_d);
+        const int last = rows_e - 1 - s * kDK;             // rows behind it are aimed at it
+        static_for<0, CP>([&](auto c_tag) {
+            constexpr int c = decltype(c_tag)::value;
+            const int r = kn_r + 16 * c;
+            const uint32_t rr = (uint32_t)(r < last ? r : last);
+            copy_g2lds_16<c * kBlock>(rr * pitch_a + a_col, ab, lds);
+            copy_g2lds_16<kImage + c * kBlock>(rr * pitch_d + d_col, db, lds);
+        });
+    };
+    auto issue_prologue = [&]() {
+        for (int s = 0; s < pre; ++s) issue_copies(s);
+    };
+    auto wait_ahead = [&](int n) {
+        if (n >= 3) DMOE_WAIT_VMCNT(3 * kLoads);
+        else if (n == 2) DMOE_WAIT_VMCNT(2 * kLoads);
+        else if (n == 1) DMOE_WAIT_VMCNT(kLoads);
+        else DMOE_WAIT_VMCNT(0);
+    };
+
+    unsigned int draw = 0;
+    const bool drawer = tid == 0;
+    if (drawer) draw = sched_draw(p.sched, streams);
+    long long q = blockIdx.x;
+    if (q < total) {
+        open_item(q);
+        issue_prologue();
+    }
+
+    while (q < total) {
+        const int cur_e = e, cur_k0 = k0, cur_n0 = n0, cur_S = S, cur_rows = rows_e;
+        f32x4 acc[FM][FN];
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+        // zeros over the rows of stage s behind the expert's last (this lane's own copies, which have landed)
+        auto clear_behind = [&](int s) {
+            const int valid = cur_rows - s * kDK;
+            __builtin_amdgcn_sched_barrier(0);             // behind the wait
+            char *mine = smem + (s % kStages) * kStage + wave * 1024 + lane * 16;
+#pragma unroll
+            for (int c = 0; c < CP; ++c) {
+                if (kn_r + 16 * c < valid) continue;
+                *(u32x4 *)(mine + c * kBlock) = u32x4{0, 0, 0, 0};
+                *(u32x4 *)(mine + kImage + c * kBlock) = u32x4{0, 0, 0, 0};
+            }
+        };
+        const bool ragged = (cur_rows & (kDK - 1)) != 0;
+        bf16x8 fa[FM], fb[FN];
+        auto read_operand = [&](bf16x8 &f, const char *src) {
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3))) *)DMOE_LDS_PTR(src));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3))) *)DMOE_LDS_PTR(src + 4 * 512));
+            const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            __builtin_memcpy(&f, &v, 16);
+        };
+        // `ahead`: stages behind s + 1 whose copies may still be in flight when s + 1 has to be there
+        auto stage = [&](int s, auto refill_tag, int ahead, bool next) {
+            constexpr bool kRefill = decltype(refill_tag)::value;
+            auto landed = [&]() {
+                if constexpr (kRefill) DMOE_WAIT_VMCNT((kStages - 2) * kLoads);
+                else {
+                    wait_ahead(ahead);
+                    if (ragged && s + 1 == cur_S - 1) clear_behind(s + 1);
+                }
+            };
+            const char *t = smem + (s % kStages) * kStage;
+#pragma unroll
+            for (int i = 0; i < FM; ++i) read_operand(fa[i], t + fa_off[i]);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) read_operand(fb[j], t + fb_off[j]);
+            if constexpr (kRefill) issue_copies(s + kStages - 1);
+            if (next && wm == 1) landed();
+            __builtin_amdgcn_sched_barrier(0);
+            __syncthreads();
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(1);
+            static_for<0, FM>([&](auto i_tag) {
+                constexpr int i = decltype(i_tag)::value;
+#pragma unroll
+                for (int jj = 0; jj < FN; ++jj) {
+                    const int j = (i & 1) ? FN - 1 - jj : jj;
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j], fa[i], acc[i][j], 0, 0, 0);
+                }
+            });
+            __builtin_amdgcn_s_setprio(0);
+            if (next && wm == 0) landed();
+            __builtin_amdgcn_sched_barrier(0);
+            __syncthreads();
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        if (cur_S > 0) {
+            wait_ahead(pre - 1);
+            if (ragged && cur_S == 1) clear_behind(0);
+            __syncthreads();
+            if (wm == 1) __syncthreads();                  // the half that runs a phase behind
+            int s = 0;
+            stage(0, std::false_type{}, (cur_S - 2 < kStages - 2 ? cur_S - 2 : kStages - 2), cur_S > 1);
+            for (s = 1; s + kStages - 1 < cur_S; ++s) stage(s, std::true_type{}, 0, true);
+            for (; s < cur_S; ++s) {
+                const int left = cur_S - 1 - s;
+                stage(s, std::false_type{}, left - 1 < kStages - 2 ? left - 1 : kStages - 2, left > 0);
+            }
+            if (wm == 0) __syncthreads();
+        }
+
+        // ---- epilogue: lane l holds, of fragment (i, j), row i * 16 + l % 16 (of K) and the 4 columns j * 16 + (l / 16) * 4 ..;
+        // 32 rows at a time through 4 KiB of LDS that belong to the wavefront, out by whole 128-byte lines ----
+        char *stg = smem + (cur_S % kStages) * kStage + wave * 4096;
+        const int col0 = cur_n0 + wn * TN;
+        uint16_t *out = (uint16_t *)p.c + ((long long)cur_e * p.K + cur_k0) * p.N;
+#pragma unroll
+        for (int i2 = 0; i2 < FM / 2; ++i2) {
+#pragma unroll
+            for (int ii = 0; ii < 2; ++ii) {
+                const int i = i2 * 2 + ii, row = ii * 16 + l16;
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+                    uint2 pk;
+                    pk.x = pack_bf16x2(acc[i][j][0], acc[i][j][1]);
+                    pk.y = pack_bf16x2(acc[i][j][2], acc[i][j][3]);
+                    const int cb = j * 32 + g16 * 8;
+                    *(uint2 *)(stg + row * 128 + (((cb >> 4) ^ ((row >> 1) & 7)) << 4) + (cb & 8)) = pk;
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int row = t * 8 + lane / 8, c = lane % 8;
+                const u32x4 val = *(const u32x4 *)(stg + row * 128 + ((c ^ ((row >> 1) & 7)) << 4));
+                const int krow = wm * TM + i2 * 32 + row, gcol = col0 + c * 8;
+                if (cur_k0 + krow >= p.K || gcol >= p.N) continue;
+                *(u32x4 *)(out + (long long)krow * p.N + gcol) = val;
+            }
+        }
+
+        if (drawer) s_item = sched_item(draw, streams);
+        __syncthreads();   // also: the last stage has been read by everyone and the staged rows have been read back
+        q = (long long)to_scalar((uint64_t)s_item);
+        if (q < total) {
+            if (drawer) draw = sched_draw(p.sched, streams);
+            open_item(q);
+            issue_prologue();
+        }
+    }
+    sched_finish(p.sched, drawer, draw, streams, total);
+}
+
+int launch_wgrad(const GmmArgs &args, hipStream_t stream) {
+    constexpr int lds = 4 * 2 * 256 * kDK * 2;
+    static unsigned long long configured = 0;   // devices on which the kernel's LDS size has been raised
+    DMOE_HIP(raise_dynamic_lds((const void *)gmm_wgrad_kernel, lds, &configured));
+    const long long tiles = (long long)args.E * ((args.K + 255) / 256) * ((args.N + 255) / 256);
+    const long long cus = device_cus();
+    const long long grid = ((tiles < cus ? tiles : cus) + kXcds - 1) / kXcds * kXcds;
+    hipLaunchKernelGGL(gmm_wgrad_kernel, dim3((unsigned)grid), dim3(512), lds, stream, args);
+    DMOE_LAUNCH_CHECK("gmm_wgrad_kernel");
+    return DMOE_OK;
+}
+
+}  // namespace dmoe

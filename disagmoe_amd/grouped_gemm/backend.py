@@ -235,6 +235,83 @@ def gmm_swiglu_rows(x: torch.Tensor, row_token: torch.Tensor, b: torch.Tensor, b
     return c
 
 
+# ---- gradients: no counterpart in the reference ------------------------------
+
+def gmm_swiglu_keep(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor, trans_b: bool = False,
+                    workspace: Optional[torch.Tensor] = None, arguments_ptr: Optional[int] = None,
+                    host_batch_sizes: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """:func:`gmm_swiglu` for a step whose gradient will be asked for: ``(h [rows, I], u [rows, 2I])``
+    with ``u = gmm(a, b)`` in bf16.  Rows of ``h`` past ``sum(batch_sizes)`` are zero."""
+    device = _check_operands(a, b, torch.bfloat16)
+    rows, K = a.shape
+    E = b.shape[0]
+    N2 = b.shape[1] if trans_b else b.shape[2]
+    assert (b.shape[2] if trans_b else b.shape[1]) == K, "contraction length mismatch"
+    assert N2 % 2 == 0 and batch_sizes.numel() == E
+    h = torch.empty((rows, N2 // 2), dtype=a.dtype, device=device)
+    u = torch.empty((rows, N2), dtype=a.dtype, device=device)
+    bs = _sizes_on_device(batch_sizes, device)
+    with torch.cuda.device(device):
+        _lib.call("dmoe_gmm_swiglu_keep", a.data_ptr(), b.data_ptr(), h.data_ptr(), u.data_ptr(), bs.data_ptr(), rows, E, K, N2 // 2,
+                  1 if trans_b else 0, _lib.BF16, *_state_args(device, workspace, arguments_ptr, _stream(device),
+                               _host_sizes(batch_sizes, host_batch_sizes)))
+    return h, u
+
+
+def gmm_swiglu_backward(dh: torch.Tensor, u: torch.Tensor, a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor,
+                        trans_b: bool = False, need_da: bool = True, need_db: bool = True, workspace: Optional[torch.Tensor] = None,
+                        arguments_ptr: Optional[int] = None, host_batch_sizes: Optional[torch.Tensor] = None):
+    """The gradients ``(da, db)`` of :func:`gmm_swiglu_keep`'s operands for a gradient ``dh [rows, I]``
+    of its ``h`` and the ``u`` it returned; ``None`` for one that is not needed.  Rows of ``da`` past
+    ``sum(batch_sizes)`` are zero."""
+    device = _check_operands(a, b, torch.bfloat16)
+    rows, K = a.shape
+    E, inter = b.shape[0], dh.shape[1]
+    assert b.shape == ((E, 2 * inter, K) if trans_b else (E, K, 2 * inter)) and batch_sizes.numel() == E
+    assert dh.shape == (rows, inter) and u.shape == (rows, 2 * inter), "dh is [rows, I], u is [rows, 2I]"
+    assert dh.dtype == torch.bfloat16 and u.dtype == torch.bfloat16 and dh.device == device and u.device == device
+    assert dh.is_contiguous() and u.is_contiguous()
+    du = torch.empty_like(u)
+    da = torch.empty_like(a) if need_da else None
+    db = torch.empty_like(b) if need_db else None
+    bs = _sizes_on_device(batch_sizes, device)
+    with torch.cuda.device(device):
+        _lib.call("dmoe_gmm_swiglu_backward", dh.data_ptr(), u.data_ptr(), a.data_ptr(), b.data_ptr(), du.data_ptr(),
+                  da.data_ptr() if need_da else None, db.data_ptr() if need_db else None, bs.data_ptr(), rows, E, K, inter,
+                  1 if trans_b else 0, _lib.BF16, *_state_args(device, workspace, arguments_ptr, _stream(device),
+                               _host_sizes(batch_sizes, host_batch_sizes)))
+    return da, db
+
+
+def gmm_wgrad(a: torch.Tensor, dc: torch.Tensor, batch_sizes: torch.Tensor, workspace: Optional[torch.Tensor] = None,
+              arguments_ptr: Optional[int] = None, host_batch_sizes: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The gradient of ``b [E, K, N]`` for ``c = gmm(a, b)`` and a gradient ``dc`` of ``c``:
+    ``a[o_e:o_e+n_e].T @ dc[o_e:o_e+n_e]`` for every expert, zeros for one without rows.  For
+    ``b [E, N, K]`` (``trans_b``) the two operands change places."""
+    if not a.is_cuda:
+        raise RuntimeError("gmm_wgrad needs device tensors; disagmoe_amd has no CPU fallback")
+    assert a.dim() == 2 and dc.dim() == 2 and a.shape[0] == dc.shape[0], "a is [rows, K], dc is [rows, N]"
+    assert a.dtype == torch.bfloat16 and dc.dtype == torch.bfloat16 and a.device == dc.device
+    assert a.is_contiguous() and dc.is_contiguous()
+    E, (rows, K), N, device = batch_sizes.numel(), a.shape, dc.shape[1], a.device
+    db = torch.empty((E, K, N), dtype=a.dtype, device=device)
+    bs = _sizes_on_device(batch_sizes, device)
+    with torch.cuda.device(device):
+        _lib.call("dmoe_gmm_wgrad", a.data_ptr(), dc.data_ptr(), db.data_ptr(), bs.data_ptr(), rows, E, K, N, _lib.BF16,
+                  *_state_args(device, workspace, arguments_ptr, _stream(device), _host_sizes(batch_sizes, host_batch_sizes)))
+    return db
+
+
+def zero_rows_behind(c: torch.Tensor, batch_sizes: torch.Tensor) -> torch.Tensor:
+    """Zeros in the rows of ``c [rows, d]`` past ``sum(batch_sizes)``, which the products leave as they are."""
+    assert c.is_cuda and c.dim() == 2 and c.is_contiguous() and c.dtype in (torch.bfloat16, torch.float16)
+    bs = _sizes_on_device(batch_sizes, c.device)
+    with torch.cuda.device(c.device):
+        _lib.call("dmoe_zero_rows_behind", c.data_ptr(), bs.data_ptr(), c.shape[0], bs.numel(), c.shape[1],
+                  _lib.BF16 if c.dtype == torch.bfloat16 else _lib.FP16, _stream(c.device))
+    return c
+
+
 def takes_rows(T: int, rows: int, num_experts: int, K: int, inter: int) -> bool:
     """Whether :func:`gmm_swiglu_rows` is the form to use for a gate-up projection of these
     shapes.  It always runs the 256-row tile kernel, so it needs the library to choose that

@@ -1,0 +1,85 @@
+"""The grouped products under autograd: :func:`gmm` and the gated block :func:`gmm_swiglu`
+with the operands of ``backend`` and gradients of both ``a`` and ``b``.
+
+Gradients are bf16 like the operands, each sum taken in fp32 and rounded once.  Rows past
+``sum(batch_sizes)`` belong to no expert: they come out as zeros and their gradient is zero;
+an expert without rows has a zero gradient.  ``workspace`` and ``arguments_ptr``
+(``backend.get_arguments``) serve the forward and the backward launches, which follow each other
+on the stream the forward ran on; a step that is captured into a graph has to bring them, as
+``backend.gmm`` does.  The gradients themselves are not differentiable.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import backend
+
+
+def _on_device(batch_sizes: torch.Tensor, host_batch_sizes: Optional[torch.Tensor], device: torch.device):
+    """(sizes on the device, sizes on the host or None), for the forward and the backward launches alike."""
+    return backend._sizes_on_device(batch_sizes, device), backend._host_sizes(batch_sizes, host_batch_sizes)
+
+
+class _Gmm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, a, b, sizes, host, trans_b, state):
+        ctx.save_for_backward(a, b, sizes)
+        ctx.host, ctx.trans_b, ctx.state = host, trans_b, state
+        return backend.zero_rows_behind(backend.gmm(a, b, sizes, trans_b=trans_b, host_batch_sizes=host, **state), sizes)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dc):
+        a, b, sizes = ctx.saved_tensors
+        more = dict(ctx.state, host_batch_sizes=ctx.host)
+        dc = dc.contiguous()
+        da = db = None
+        if ctx.needs_input_grad[0]:
+            da = backend.zero_rows_behind(backend.gmm(dc, b, sizes, trans_b=not ctx.trans_b, **more), sizes)
+        if ctx.needs_input_grad[1]:
+            db = backend.gmm_wgrad(dc, a, sizes, **more) if ctx.trans_b else backend.gmm_wgrad(a, dc, sizes, **more)
+        return da, db, None, None, None, None
+
+
+class _GmmSwiglu(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, a, b, sizes, host, trans_b, state):
+        h, u = backend.gmm_swiglu_keep(a, b, sizes, trans_b=trans_b, host_batch_sizes=host, **state)
+        ctx.save_for_backward(a, b, sizes, u)
+        ctx.host, ctx.trans_b, ctx.state = host, trans_b, state
+        return h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh):
+        a, b, sizes, u = ctx.saved_tensors
+        da, db = backend.gmm_swiglu_backward(dh.contiguous(), u, a, b, sizes, trans_b=ctx.trans_b, need_da=ctx.needs_input_grad[0],
+                                             need_db=ctx.needs_input_grad[1], host_batch_sizes=ctx.host, **ctx.state)
+        return da, db, None, None, None, None
+
+
+def gmm(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor, trans_b: bool = False,
+        workspace: Optional[torch.Tensor] = None, arguments_ptr: Optional[int] = None,
+        host_batch_sizes: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Differentiable ``backend.gmm``: ``c[o_e:o_e+n_e] = a[o_e:o_e+n_e] @ b[e]`` (``b[e].T`` with
+    ``trans_b``), bf16 in and out."""
+    backend._check_operands(a, b, torch.bfloat16)
+    sizes, host = _on_device(batch_sizes, host_batch_sizes, a.device)
+    return _Gmm.apply(a, b, sizes, host, trans_b, dict(workspace=workspace, arguments_ptr=arguments_ptr))
+
+
+def gmm_swiglu(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor, trans_b: bool = False,
+               workspace: Optional[torch.Tensor] = None, arguments_ptr: Optional[int] = None,
+               host_batch_sizes: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Differentiable ``backend.gmm_swiglu``: ``silu(u[:, :I]) * u[:, I:]`` for ``u = gmm(a, b)``,
+    ``b [E, K, 2I]`` (``[E, 2I, K]`` with ``trans_b``).  Keeps ``u`` in bf16 (4 bytes per element of
+    the result) for the backward pass; without a gradient to come it is ``backend.gmm_swiglu``."""
+    backend._check_operands(a, b, torch.bfloat16)
+    sizes, host = _on_device(batch_sizes, host_batch_sizes, a.device)
+    if not (torch.is_grad_enabled() and (a.requires_grad or b.requires_grad)):
+        return backend.zero_rows_behind(backend.gmm_swiglu(a, b, sizes, trans_b=trans_b, workspace=workspace,
+                                                           arguments_ptr=arguments_ptr, host_batch_sizes=host), sizes)
+    return _GmmSwiglu.apply(a, b, sizes, host, trans_b, dict(workspace=workspace, arguments_ptr=arguments_ptr))

@@ -9,6 +9,7 @@ from typing import Optional
 import torch
 
 from ..grouped_gemm import backend as gg
+from ..grouped_gemm import ops as gops
 
 MAX_BATCH_SIZE = 256  # disagmoe/utils/constants.py:20-22
 
@@ -121,6 +122,17 @@ class MoEExperts(_GemmState, torch.nn.Module):
         ws = dict(self._gemm_state(), host_batch_sizes=host_batch_sizes)
         h = gg.gmm_swiglu_rows(x, row_token, self.w13_weight, batch_sizes, **ws)
         return gg.gmm(h, self.w2_weight, batch_sizes, **ws)
+
+    def forward_train(self, bs: int, hiddens: torch.Tensor, batch_sizes: torch.Tensor,
+                      host_batch_sizes: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """:meth:`forward` under autograd (no counterpart in the reference, whose weights take no gradient):
+        gradients of ``hiddens`` and, after ``requires_grad_()``, of ``w13_weight`` and ``w2_weight``.  Rows past
+        ``sum(batch_sizes)`` are zero and have a zero gradient.  The backward pass runs on the stream of the
+        forward pass, with this layer's state block: as the forward passes of one layer, steps of one layer must
+        not overlap in time."""
+        ws = dict(self._gemm_state(), host_batch_sizes=host_batch_sizes)
+        h = gops.gmm_swiglu(hiddens, self.w13_weight, batch_sizes, **ws)
+        return gops.gmm(h, self.w2_weight, batch_sizes, **ws)
 
     def takes_rows(self, T: int, rows: int) -> bool:
         """Whether :meth:`forward_rows` is the faster form for a batch of these sizes."""

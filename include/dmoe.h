@@ -280,6 +280,35 @@ int dmoe_gmm_swiglu_rows(const void *x, const int32_t *row_token, int64_t T, con
                          void *state, void *workspace, size_t workspace_bytes,
                          const int64_t *host_batch_sizes, void *stream);
 
+/* ---- gradients of the grouped products: no counterpart in the reference --------
+ * dmoe_gmm_wgrad: the gradient of b for c = a @ b[e] and a gradient dc of c,
+ *     db[e] = a[o_e:o_e+n_e, :]^T @ dc[o_e:o_e+n_e, :]       a [rows, K], dc [rows, N], db [E, K, N]
+ *   (for b in the [E, N, K] layout: dmoe_gmm_wgrad(dc, a) gives it so).  fp32 sums, one rounding; zeros for an expert
+ *   without rows; every element of db is written.  K % 8 == 0 and N % 8 == 0.  The gradient of a is dmoe_gmm(dc, b) with
+ *   the other trans_b.  state, workspace and host_batch_sizes as for dmoe_gmm.
+ *
+ * The gated block h = silu(g) p, [g | p] = u = a @ b[e], as one differentiable step:
+ *   dmoe_gmm_swiglu_keep is dmoe_gmm_swiglu that also leaves u [rows, 2I] in bf16.
+ *   dmoe_gmm_swiglu_backward takes that u and a gradient dh [rows, I] of h; with s = sigmoid(g)
+ *     du[r, n] = dh p s (1 + g (1 - s)),  du[r, I + n] = dh g s          (fp32, one rounding)
+ *   goes to du [rows, 2I] (the caller's, any contents), and from it, where they are not NULL,
+ *     da [rows, K] = du @ b[e]^T  and  db[e] = a^T @ du  (b's layout).
+ *   The rows of h and of da behind the sum(batch_sizes) in use are set to zero: they belong to no expert.
+ *
+ * dmoe_zero_rows_behind does that to c [rows, d] (bf16 or fp16), for the products that leave such rows as they are. */
+int dmoe_gmm_wgrad(const void *a, const void *dc, void *db, const int64_t *batch_sizes, int64_t rows, int E,
+                   int64_t K, int64_t N, int dtype, void *state, void *workspace, size_t workspace_bytes,
+                   const int64_t *host_batch_sizes, void *stream);
+int dmoe_gmm_swiglu_keep(const void *a, const void *b, void *h, void *u, const int64_t *batch_sizes,
+                         int64_t rows, int E, int64_t K, int64_t I, int trans_b, int dtype,
+                         void *state, void *workspace, size_t workspace_bytes,
+                         const int64_t *host_batch_sizes, void *stream);
+int dmoe_gmm_swiglu_backward(const void *dh, const void *u, const void *a, const void *b, void *du, void *da, void *db,
+                             const int64_t *batch_sizes, int64_t rows, int E, int64_t K, int64_t I, int trans_b,
+                             int dtype, void *state, void *workspace, size_t workspace_bytes,
+                             const int64_t *host_batch_sizes, void *stream);
+int dmoe_zero_rows_behind(void *c, const int64_t *batch_sizes, int64_t rows, int E, int64_t d, int dtype, void *stream);
+
 /* ---- fp8 (e4m3) path: no counterpart in the reference ---------------------
  * Per-row quantisation: q[r, :] = fp8(x[r, :] / s[r]), s[r] = absmax(x[r, :]) / 448
  * (s = 1 for a zero row).  x is bf16 [rows, d]. */
