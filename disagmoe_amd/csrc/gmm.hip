@@ -683,6 +683,8 @@ extern "C" int dmoe_gmm_swiglu_keep(const void *a, const void *b, void *h, void 
     int rc = check_gmm("dmoe_gmm_swiglu_keep", a, b, h, batch_sizes, rows, E, K, I, 8);
     if (rc != DMOE_OK) return rc;
     DMOE_REQUIRE(rows == 0 || u != nullptr, DMOE_ERR_ARG, "dmoe_gmm_swiglu_keep: null pointer");
+    DMOE_REQUIRE((((uintptr_t)a | (uintptr_t)b | (uintptr_t)h | (uintptr_t)u) & 15) == 0, DMOE_ERR_ARG,
+                 "dmoe_gmm_swiglu_keep: a pointer is not 16-byte aligned");
     rc = dmoe_gmm(a, b, u, batch_sizes, rows, E, K, 2 * I, trans_b, dtype, state, workspace, workspace_bytes, host_batch_sizes, stream);
     if (rc != DMOE_OK || rows == 0) return rc;
     return launch_swiglu_forward(u, h, batch_sizes, rows, E, I, (hipStream_t)stream);
@@ -698,6 +700,7 @@ extern "C" int dmoe_gmm_wgrad(const void *a, const void *dc, void *db, const int
     DMOE_REQUIRE(batch_sizes != nullptr && db != nullptr && (rows == 0 || (a != nullptr && dc != nullptr)), DMOE_ERR_ARG,
                  "dmoe_gmm_wgrad: null pointer");
     DMOE_REQUIRE(db != a && db != dc, DMOE_ERR_ARG, "dmoe_gmm_wgrad: the result overlaps an input");
+    DMOE_REQUIRE((((uintptr_t)a | (uintptr_t)dc | (uintptr_t)db) & 15) == 0, DMOE_ERR_ARG, "dmoe_gmm_wgrad: a pointer is not 16-byte aligned");
     GmmArgs args{(const char *)a, (const char *)dc, (char *)db, batch_sizes, nullptr, nullptr, rows, E, (int)K, (int)N, (int)N};
     rc = bind_state(args, state, workspace, workspace_bytes, (hipStream_t)stream);
     if (rc != DMOE_OK) return rc;
@@ -714,6 +717,8 @@ extern "C" int dmoe_gmm_swiglu_backward(const void *dh, const void *u, const voi
     DMOE_REQUIRE(batch_sizes != nullptr && (da == nullptr || b != nullptr), DMOE_ERR_ARG, "dmoe_gmm_swiglu_backward: null pointer");
     DMOE_REQUIRE(rows == 0 || (dh != nullptr && u != nullptr && du != nullptr && (db == nullptr || a != nullptr)), DMOE_ERR_ARG,
                  "dmoe_gmm_swiglu_backward: null pointer");
+    DMOE_REQUIRE((((uintptr_t)dh | (uintptr_t)u | (uintptr_t)a | (uintptr_t)b | (uintptr_t)du | (uintptr_t)da | (uintptr_t)db) & 15) == 0,
+                 DMOE_ERR_ARG, "dmoe_gmm_swiglu_backward: a pointer is not 16-byte aligned");
     if (rows > 0) {
         DMOE_REQUIRE(du != u && du != dh && da != dh && da != a, DMOE_ERR_ARG, "dmoe_gmm_swiglu_backward: a result overlaps an input");
         rc = launch_swiglu_backward(dh, u, du, batch_sizes, rows, E, I, da, K, (hipStream_t)stream);

@@ -124,7 +124,7 @@ extern "C" int dmoe_zero_rows_behind(void *c, const int64_t *batch_sizes, int64_
     const int rc = check_rows_of("dmoe_zero_rows_behind", batch_sizes, rows, E, d);
     if (rc != DMOE_OK) return rc;
     if (rows == 0) return DMOE_OK;
-    DMOE_REQUIRE(c != nullptr, DMOE_ERR_ARG, "dmoe_zero_rows_behind: null pointer");
+    DMOE_REQUIRE(c != nullptr && ((uintptr_t)c & 15) == 0, DMOE_ERR_ARG, "dmoe_zero_rows_behind: null or unaligned pointer");
     hipLaunchKernelGGL(zero_behind_kernel, dim3(blocks_of(rows * (d / 8))), dim3(kSwThreads), 0, (hipStream_t)stream,
                        (u32x4 *)c, batch_sizes, E, rows, d / 8);
     DMOE_LAUNCH_CHECK("zero_behind_kernel");

@@ -6,7 +6,7 @@ library.  Everything runs on the current stream of ``a``'s device.
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -431,6 +431,145 @@ def gmm_fp8_swiglu(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_sc
                   *_state_args(a.device, workspace, arguments_ptr, _stream(a.device),
                                _host_sizes(batch_sizes, host_batch_sizes)))
     return c
+
+
+# ---- 4-bit weights with group scales: no counterpart in the reference --------
+
+class W4Weight(NamedTuple):
+    """4-bit weights of all experts, ``(q - z) * s`` for every group of ``group`` k of a column, in the
+    tiles that include/dmoe.h describes: ``codes [E, nt, kt, 1024]`` uint8, ``scales [E, nt, kt, 4,
+    128 / group, 4]`` bf16, ``zeros`` like the scales in uint8 or ``None`` (8 everywhere), for a logical
+    ``[E, N, K]`` with ``nt = ceil(N / 16)`` and ``kt = ceil(K / 128)``."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    zeros: Optional[torch.Tensor]
+    K: int
+    N: int
+    group: int
+
+
+def _w4_shapes(E: int, K: int, N: int, group: int):
+    if group not in (32, 64, 128):
+        raise ValueError(f"groups of 32, 64 or 128 weights, got {group}")
+    nt, kt = -(-N // 16), -(-K // 128)
+    return (E, nt, kt, 1024), (E, nt, kt, 4, 128 // group, 4)
+
+
+def _w4_empty(E: int, K: int, N: int, group: int, zeros: bool, device: torch.device) -> W4Weight:
+    codes, groups = _w4_shapes(E, K, N, group)
+    return W4Weight(torch.empty(codes, dtype=torch.uint8, device=device), torch.empty(groups, dtype=torch.bfloat16, device=device),
+                    torch.empty(groups, dtype=torch.uint8, device=device) if zeros else None, K, N, group)
+
+
+def _check_w4(w: W4Weight) -> int:
+    """The number of experts of a well-formed weight."""
+    E = w.codes.shape[0]
+    codes, groups = _w4_shapes(E, w.K, w.N, w.group)
+    device = w.codes.device
+    if device.type != "cuda":
+        raise RuntimeError("4-bit weights need device tensors; disagmoe_amd has no CPU fallback")
+    assert w.codes.shape == codes and w.codes.dtype == torch.uint8 and w.codes.is_contiguous(), f"codes are uint8 {codes}"
+    assert w.scales.shape == groups and w.scales.dtype == torch.bfloat16 and w.scales.is_contiguous() and w.scales.device == device, \
+        f"scales are bf16 {groups}"
+    if w.zeros is not None:
+        assert w.zeros.shape == groups and w.zeros.dtype == torch.uint8 and w.zeros.is_contiguous() and w.zeros.device == device, \
+            f"zeros are uint8 {groups}"
+    return E
+
+
+def _zeros_ptr(w: W4Weight):
+    return None if w.zeros is None else w.zeros.data_ptr()
+
+
+def quantize_weight_w4(w: torch.Tensor, group: int = 128, zeros: bool = False) -> W4Weight:
+    """Offline quantisation of ``w [E, K, N]`` bf16 to 4 bits: symmetric, ``s = absmax / 7`` over every
+    ``group`` k of a column, or with ``zeros`` from the smallest to the largest weight of the group
+    (``s = range / 15``; a weight of zero stays zero)."""
+    if not w.is_cuda:
+        raise RuntimeError("quantize_weight_w4 needs a device tensor; disagmoe_amd has no CPU fallback")
+    assert w.dim() == 3 and w.dtype == torch.bfloat16 and w.is_contiguous()
+    E, K, N = w.shape
+    out = _w4_empty(E, K, N, group, zeros, w.device)
+    with torch.cuda.device(w.device):
+        _lib.call("dmoe_w4_quant", w.data_ptr(), E, K, N, group, out.codes.data_ptr(), out.scales.data_ptr(), _zeros_ptr(out),
+                  _stream(w.device))
+    return out
+
+
+def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor], group: int) -> W4Weight:
+    """Lays out weights that are quantised already: ``codes [E, N, K]`` uint8 in 0..15, ``scales [E, N,
+    ceil(K / group)]``, ``zeros`` likewise in uint8 or ``None``.  Once per weight; any device."""
+    E, N, K = codes.shape
+    assert K % 8 == 0 and N % 8 == 0 and scales.shape == (E, N, -(-K // group)), "codes [E, N, K], scales [E, N, ceil(K / group)]"
+    out = _w4_empty(E, K, N, group, zeros is not None, codes.device)
+    (_, nt, kt, _), per = out.codes.shape, 128 // group
+    for e in range(E):
+        q = codes.new_zeros((nt * 16, kt * 128), dtype=torch.uint8)
+        q[:N, :K] = codes[e]
+        q = q.view(nt, 16, kt, 4, 4, 4, 2).permute(0, 2, 4, 1, 3, 6, 5).reshape(nt, kt, 4, 16, 4, 4, 2)
+        out.codes[e] = (q[..., 0] | (q[..., 1] << 4)).reshape(nt, kt, 1024)
+        for src, dst in ((scales, out.scales), (zeros, out.zeros)):
+            if src is None:
+                continue
+            s = dst.new_zeros((nt * 16, kt * per))
+            s[:N, :src.shape[2]] = src[e]
+            dst[e] = s.view(nt, 4, 4, kt, per).permute(0, 3, 1, 4, 2)
+    return out
+
+
+def dequantize_w4(w: W4Weight) -> torch.Tensor:
+    """``[E, N, K]`` bf16, each weight rounded once."""
+    E = _check_w4(w)
+    out = torch.empty((E, w.N, w.K), dtype=torch.bfloat16, device=w.codes.device)
+    with torch.cuda.device(w.codes.device):
+        _lib.call("dmoe_w4_dequant", w.codes.data_ptr(), w.scales.data_ptr(), _zeros_ptr(w), w.group, out.data_ptr(), None, E, w.K, w.N,
+                  _stream(w.codes.device))
+    return out
+
+
+def _gmm_w4(name: str, a: torch.Tensor, w: W4Weight, n_out: int, batch_sizes: torch.Tensor, c: Optional[torch.Tensor],
+            workspace: Optional[torch.Tensor], arguments_ptr: Optional[int], host_batch_sizes: Optional[torch.Tensor]) -> torch.Tensor:
+    E, device = _check_w4(w), w.codes.device
+    assert a.dim() == 2 and a.dtype == torch.bfloat16 and a.is_contiguous() and a.device == device, "a is bf16 [rows, K]"
+    rows = a.shape[0]
+    assert a.shape[1] == w.K, "contraction length mismatch"
+    assert batch_sizes.numel() == E
+    if c is None:
+        c = torch.empty((rows, n_out), dtype=a.dtype, device=device)
+    else:
+        assert c.is_contiguous() and c.dtype == a.dtype and c.device == device
+        assert c.dim() == 2 and c.shape[1] == n_out and c.shape[0] >= rows
+    bs, host = _sizes_on_device(batch_sizes, device), _host_sizes(batch_sizes, host_batch_sizes)
+    host_ptr = None if host is None else host.data_ptr()
+    need = _lib.c_size_t(0)
+    with torch.cuda.device(device):
+        stream = _stream(device)
+        _lib.call("dmoe_gmm_w4_wide_bytes", rows, E, w.K, w.N, host_ptr, _lib.ctypes.byref(need))
+        if need.value:   # bf16 weights of this call, and the state of the bf16 product
+            wide = torch.empty(need.value, dtype=torch.uint8, device=device)
+            more = (wide.data_ptr(), need.value, *_state_triple(device, workspace, arguments_ptr, stream))
+        else:
+            more = (None, 0, None, None, 0)
+        _lib.call(name, a.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), _zeros_ptr(w), w.group, c.data_ptr(), bs.data_ptr(),
+                  rows, E, w.K, n_out, *more, host_ptr, stream)
+    return c
+
+
+def gmm_w4(a: torch.Tensor, w: W4Weight, batch_sizes: torch.Tensor, c: Optional[torch.Tensor] = None,
+           workspace: Optional[torch.Tensor] = None, arguments_ptr: Optional[int] = None,
+           host_batch_sizes: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``c[o_e:o_e+n_e] = a[o_e:o_e+n_e] @ w[e].T`` on 4-bit weights, bf16 ``[rows, N]``.  From one row to
+    a prompt; many rows per expert go through bf16 weights that the call allocates and writes
+    (``E * N * K * 2`` bytes, for its own length).  The other arguments as :func:`gmm`'s."""
+    return _gmm_w4("dmoe_gmm_w4", a, w, w.N, batch_sizes, c, workspace, arguments_ptr, host_batch_sizes)
+
+
+def gmm_w4_swiglu(a: torch.Tensor, w: W4Weight, batch_sizes: torch.Tensor, c: Optional[torch.Tensor] = None,
+                  workspace: Optional[torch.Tensor] = None, arguments_ptr: Optional[int] = None,
+                  host_batch_sizes: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`gmm_swiglu` on 4-bit weights ``[E, 2I, K]``: bf16 ``[rows, I]``."""
+    assert w.N % 16 == 0, "the gate and the up columns are a multiple of 8 each"
+    return _gmm_w4("dmoe_gmm_w4_swiglu", a, w, w.N // 2, batch_sizes, c, workspace, arguments_ptr, host_batch_sizes)
 
 
 def set_tile_variant(variant: int) -> None:

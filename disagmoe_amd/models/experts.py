@@ -205,3 +205,33 @@ class MoEExpertsFP8(_GemmState, torch.nn.Module):
         h = gg.gmm_fp8_swiglu(xq, xs, self.w13_q, self.w13_scale, batch_sizes, **ws)
         hq, hs = gg.quantize_rows(h)
         return gg.gmm_fp8(hq, hs, self.w2_q, self.w2_scale, batch_sizes, **ws)
+
+
+class MoEExpertsW4(_GemmState, torch.nn.Module):
+    """4-bit experts (no counterpart in the reference): weights with a scale, and with ``zeros`` a zero
+    point, for every ``group`` weights along the contraction (``grouped_gemm.backend.W4Weight``, a little
+    over half a byte per weight), bf16 activations, bf16 in and out.  Takes bf16 weights ``w13 [E, d, 2I]``
+    and ``w2 [E, I, d]``, or ones that are quantised already."""
+
+    def __init__(self, w13, w2, group: int = 128, zeros: bool = False, workspace: Optional[torch.Tensor] = None,
+                 own_workspace: bool = False):
+        super().__init__()
+        q13 = w13 if isinstance(w13, gg.W4Weight) else gg.quantize_weight_w4(w13, group, zeros)
+        q2 = w2 if isinstance(w2, gg.W4Weight) else gg.quantize_weight_w4(w2, group, zeros)
+        assert q13.N == 2 * q2.K and q13.K == q2.N and q13.codes.shape[0] == q2.codes.shape[0], "w13 is [E, d, 2I], w2 is [E, I, d]"
+        self.num_experts, self.hidden_size, self.intermediate_size = q13.codes.shape[0], q13.K, q2.K
+        for name, q in (("w13", q13), ("w2", q2)):
+            self.register_buffer(f"{name}_codes", q.codes)
+            self.register_buffer(f"{name}_scales", q.scales)
+            self.register_buffer(f"{name}_zeros", q.zeros)
+        self._group13, self._group2 = q13.group, q2.group
+        self._init_gemm_state(q13.codes.device, workspace, own_workspace)
+
+    def forward(self, bs: int, hiddens: torch.Tensor, batch_sizes: torch.Tensor,
+                host_batch_sizes: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``MoEExperts.forward`` on the 4-bit weights: expert-sorted rows ``[R, d]`` to ``[R, d]``."""
+        ws = dict(self._gemm_state(), host_batch_sizes=host_batch_sizes)
+        d, inter = self.hidden_size, self.intermediate_size
+        w13 = gg.W4Weight(self.w13_codes, self.w13_scales, self.w13_zeros, d, 2 * inter, self._group13)
+        w2 = gg.W4Weight(self.w2_codes, self.w2_scales, self.w2_zeros, inter, d, self._group2)
+        return gg.gmm_w4(gg.gmm_w4_swiglu(hiddens, w13, batch_sizes, **ws), w2, batch_sizes, **ws)

@@ -336,6 +336,38 @@ int dmoe_gmm_fp8_swiglu(const void *a, const float *a_scale, const void *b, cons
                         int64_t I, void *state, void *workspace, size_t workspace_bytes,
                         const int64_t *host_batch_sizes, void *stream);
 
+/* ---- 4-bit weights with group scales: no counterpart in the reference --------
+ *     w[e, n, k] = (q[e, n, k] - z[e, n, k / group]) * s[e, n, k / group],    group 32, 64 or 128
+ * q in 0..15, s bf16, z uint8 in 0..15, or 8 everywhere (zeros == NULL).  The three lie in tiles of 16 columns n by 128 k,
+ * nt = ceil(N / 16) by kt = ceil(K / 128) of them, what reaches past N or K with code 0 and scale 0:
+ *   codes  [E, nt, kt, 64 lanes, 4 words]: word j of lane 16 g + r holds column r, k = 32 j + 8 g + i (i = 0 .. 7), code i in
+ *          nibble i / 2 for even and 4 + i / 2 for odd i;
+ *   scales [E, nt, kt, 4, 128 / group, 4]: column 4 q + x at [q][group of the tile][x]; zeros likewise.
+ * K % 8 == 0 and N % 8 == 0, N below 2^20.  16-byte aligned.
+ *
+ * dmoe_w4_bytes: the sizes of the three.  dmoe_w4_quant packs bf16 weights w [E, K, N] (the layout of dmoe_gmm): with
+ * `zeros` it spreads the 16 codes from the smallest to the largest weight of a group (zero included), without it
+ * symmetrically over +-7 steps.  dmoe_w4_dequant writes [E, N, K] bf16, rounded once; with batch_sizes only the experts
+ * that have rows.
+ *
+ * dmoe_gmm_w4 is c = a @ w[e]^T for a bf16 [rows, K], c bf16 [rows, N]; dmoe_gmm_w4_swiglu the gated form on w [E, 2I, K],
+ * h [rows, I], as dmoe_gmm_swiglu.  Few rows per expert: one kernel that reads the codes, in 32-bit sums of unrounded
+ * weights.  Many: where `wide` has dmoe_gmm_w4_wide_bytes(..) bytes (0: not needed), the weights of the experts that have
+ * rows are written there as bf16 and go through dmoe_gmm; without it the one kernel serves any number of rows.
+ * state, workspace and host_batch_sizes as for dmoe_gmm (the first two serve that form only). */
+int dmoe_w4_bytes(int E, int64_t K, int64_t N, int group, size_t *code_bytes, size_t *scale_bytes, size_t *zero_bytes);
+int dmoe_w4_quant(const void *w, int E, int64_t K, int64_t N, int group, void *codes, void *scales, void *zeros,
+                  void *stream);
+int dmoe_w4_dequant(const void *codes, const void *scales, const void *zeros, int group, void *out,
+                    const int64_t *batch_sizes, int E, int64_t K, int64_t N, void *stream);
+int dmoe_gmm_w4_wide_bytes(int64_t rows, int E, int64_t K, int64_t N, const int64_t *host_batch_sizes, size_t *bytes);
+int dmoe_gmm_w4(const void *a, const void *codes, const void *scales, const void *zeros, int group, void *c,
+                const int64_t *batch_sizes, int64_t rows, int E, int64_t K, int64_t N, void *wide, size_t wide_bytes,
+                void *state, void *workspace, size_t workspace_bytes, const int64_t *host_batch_sizes, void *stream);
+int dmoe_gmm_w4_swiglu(const void *a, const void *codes, const void *scales, const void *zeros, int group, void *h,
+                       const int64_t *batch_sizes, int64_t rows, int E, int64_t K, int64_t I, void *wide, size_t wide_bytes,
+                       void *state, void *workspace, size_t workspace_bytes, const int64_t *host_batch_sizes, void *stream);
+
 /* ---- gradients: no counterpart in the reference -----------------------------
  * Global norm of many gradients and clipping to a largest norm:
  *     norm = sqrt(sum over every element of every tensor of g^2)        (64-bit sums in a fixed order)

@@ -17,7 +17,8 @@ def test_host_side_argument_errors():
     assert wgrad(dtype=_lib.FP16) == _lib.ERR_DTYPE and wgrad(dtype=_lib.FP8_E4M3) == _lib.ERR_DTYPE
     for bad in (dict(K=60), dict(N=12), dict(K=0), dict(E=0), dict(E=1025), dict(rows=-1), dict(rows=1 << 31)):
         assert wgrad(**bad) == _lib.ERR_SHAPE, bad
-    for bad in (dict(a=None), dict(dc=None), dict(db=None), dict(bs=None), dict(db=p), dict(db=p + 0x1000)):
+    for bad in (dict(a=None), dict(dc=None), dict(db=None), dict(bs=None), dict(db=p), dict(db=p + 0x1000), dict(a=p + 8), dict(dc=p + 0x1002),
+                dict(db=p + 0x2004)):
         assert wgrad(**bad) == _lib.ERR_ARG, bad
 
     def keep(a=p, b=p, h=p + 0x1000, u=p + 0x2000, bs=p, rows=16, K=64, I=64, dtype=_lib.BF16):
@@ -25,7 +26,7 @@ def test_host_side_argument_errors():
 
     assert keep(dtype=_lib.FP16) == _lib.ERR_DTYPE
     assert keep(K=60) == _lib.ERR_SHAPE and keep(I=12) == _lib.ERR_SHAPE
-    for bad in (dict(a=None), dict(b=None), dict(h=None), dict(u=None), dict(bs=None)):
+    for bad in (dict(a=None), dict(b=None), dict(h=None), dict(u=None), dict(bs=None), dict(a=p + 2), dict(u=p + 0x2008)):
         assert keep(**bad) == _lib.ERR_ARG, bad
     assert keep(rows=0) == 0
 
@@ -36,7 +37,7 @@ def test_host_side_argument_errors():
     assert back(dtype=_lib.FP16) == _lib.ERR_DTYPE
     assert back(K=60) == _lib.ERR_SHAPE and back(I=12) == _lib.ERR_SHAPE
     for bad in (dict(dh=None), dict(u=None), dict(a=None), dict(b=None), dict(du=None), dict(bs=None), dict(du=p), dict(du=p + 0x1000),
-                dict(da=p), dict(da=p + 0x2000)):
+                dict(da=p), dict(da=p + 0x2000), dict(dh=p + 8), dict(db=p + 0x6002)):
         assert back(**bad) == _lib.ERR_ARG, bad
     assert back(da=None, db=None, rows=0) == 0
 

@@ -1,0 +1,285 @@
+"""4-bit products against the definition in 64 bits.
+
+Tolerances, element by element.  A bf16 result is off by half a step, 2^-8 of its value (``HALF``).  The one kernel keeps the
+weights as they are; it adds (16 + q) x over a group of G in fp32 (at most 31 |x| a term, n terms off by at most n 2^-24 of
+their magnitudes, counted twice for a matrix core that adds several terms at a time: ``ACC``), takes (16 + z) times the
+group's sum of x off, and adds the groups: ACC (G + 8) 47 sum s |x|, and ACC (K / G + 16) times the sum of the groups'
+magnitudes.  The form through bf16 weights rounds each of them once instead: HALF |w| under the same sum."""
+import pytest
+import torch
+
+from disagmoe_amd import _lib
+from disagmoe_amd.expert_layer import expert_layer_forward
+from disagmoe_amd.grouped_gemm import backend as gg
+from disagmoe_amd.models.experts import MoEExpertsW4
+from helpers import announce, dev, ragged_sizes
+from test_w4_host import unpack
+
+pytestmark = pytest.mark.gpu
+
+HALF = 2.0 ** -8
+ACC = 2 * 2.0 ** -24
+
+
+def _rand(shape, seed, std=1.0):
+    g = torch.Generator(device=dev()).manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device=dev()) * std).to(torch.bfloat16)
+
+
+def _weight(E, N, K, group, zeros, seed):
+    g = torch.Generator(device=dev()).manual_seed(seed)
+    groups = -(-K // group)
+    q = torch.randint(0, 16, (E, N, K), generator=g, device=dev(), dtype=torch.uint8)
+    s = (torch.rand(E, N, groups, generator=g, device=dev()) * 0.02 + 0.005).to(torch.bfloat16)
+    z = torch.randint(0, 16, (E, N, groups), generator=g, device=dev(), dtype=torch.uint8) if zeros else None
+    zs = torch.full_like(s, 8).double() if z is None else z.double()
+    spread = lambda v: v.double().repeat_interleave(group, 2)[:, :, :K]
+    return gg.pack_w4(q, s, z, group), (q.double() - spread(zs)) * spread(s), spread(s)
+
+
+def _spans(sizes):
+    o = 0
+    for e, n in enumerate(sizes.tolist()):
+        yield e, slice(o, o + n)
+        o += n
+
+
+def _check(got, x, w, s, sizes, group, swiglu, wide):
+    for e, at in _spans(sizes):
+        a = x[at].double()
+        want = a @ w[e].t()
+        mag = a.abs() @ w[e].abs().t()
+        off = ACC * (group + 8) * 47 * (a.abs() @ s[e].t()) + ACC * (a.shape[1] / group + 16) * mag
+        if wide:
+            off = off + (HALF + ACC * a.shape[1]) * mag
+        if swiglu:
+            I = w.shape[1] // 2
+            g, p = want[:, :I], want[:, I:]
+            sig = torch.sigmoid(g)
+            # (second-order terms: 5 % of the first-order ones)
+            off = 1.05 * ((p * sig * (1 + g * (1 - sig))).abs() * off[:, :I] + (g * sig).abs() * off[:, I:] + off[:, :I] * off[:, I:]) + 1e-6 * (g * p).abs()
+            want = g * sig * p
+        err = (got[at].double() - want).abs()
+        bad = ~(err <= off + HALF * (want.abs() + off) + 1e-37)
+        assert not bool(bad.any()), (e, int(bad.sum()), float(err[bad][0]), float(off[bad][0]), float(want[bad][0]))
+        if not wide and not swiglu and want.numel():
+            # every element's rounding is at most HALF of it, and so is the 2-norm's; the sums add a tenth at most here
+            assert float(err.norm()) <= 1.1 * HALF * float(want.norm()) + 1e-30
+
+
+SIZES = [[1], [0, 2, 0, 1], [15, 16, 17], [5, 0, 33, 64, 0, 65, 1], [3] * 40, [190, 2, 70]]
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("K,N", [(8, 16), (40, 48), (128, 272), (264, 128), (1408, 80), (2184, 144)])
+def test_small_sizes(K, N, group, zeros):
+    for sizes in SIZES:
+        announce(test="w4", sizes=str(sizes[:8]), K=K, N=N, group=group, zeros=zeros)
+        sizes = torch.tensor(sizes)
+        E, R = len(sizes), int(sizes.sum())
+        w, ref, s = _weight(E, N, K, group, zeros, seed=K + N)
+        x = _rand((R, K), R)
+        c = gg.gmm_w4(x, w, sizes)
+        assert c.shape == (R, N) and c.dtype == torch.bfloat16
+        _check(c, x, ref, s, sizes, group, False, False)
+        assert torch.equal(c, gg.gmm_w4(x, w, sizes.to(dev()), host_batch_sizes=sizes))
+        h = gg.gmm_w4_swiglu(x, w, sizes.to(dev()))
+        assert h.shape == (R, N // 2)
+        _check(h, x, ref, s, sizes, group, True, False)
+
+
+@pytest.mark.parametrize("rows_e", [1, 20, 50, 100])
+@pytest.mark.parametrize("swiglu", [False, True])
+def test_sizes_alone_on_the_device(rows_e, swiglu):
+    announce(test="w4_device_sizes", rows_e=rows_e, swiglu=swiglu)
+    # every row tile height, planned from rows / E alone, skewed and with empty experts
+    E, K, N, group = 8, 520, 208, 64
+    sizes = ragged_sizes(E, E * rows_e, seed=rows_e, empty_every=4)
+    w, ref, s = _weight(E, N, K, group, True, seed=rows_e)
+    x = _rand((E * rows_e, K), rows_e)
+    call = gg.gmm_w4_swiglu if swiglu else gg.gmm_w4
+    out = call(x, w, sizes.to(dev()))
+    _check(out, x, ref, s, sizes, group, swiglu, False)
+    # sizes on the host that say something else cost speed and nothing else (where they plan for few experts with many rows,
+    # the library says that it takes the form through bf16 weights: the roundings are that form's)
+    for wrong in ([0] * E, [E * rows_e] + [0] * (E - 1), [1] * E):
+        wrong, need = torch.tensor(wrong), _lib.c_size_t(0)
+        _lib.call("dmoe_gmm_w4_wide_bytes", E * rows_e, E, K, N, wrong.data_ptr(), _lib.ctypes.byref(need))
+        other = call(x, w, sizes.to(dev()), host_batch_sizes=wrong)
+        _check(other, x, ref, s, sizes, group, swiglu, need.value > 0)
+
+
+@pytest.mark.parametrize("swiglu", [False, True])
+@pytest.mark.parametrize("group,zeros", [(32, True), (128, False)])
+def test_many_rows(swiglu, group, zeros):
+    announce(test="w4_many_rows", swiglu=swiglu, group=group, zeros=zeros)
+    sizes = torch.tensor([400, 0, 1, 513])
+    E, K, N, R = 4, 392, 304, 914
+    w, ref, s = _weight(E, N, K, group, zeros, seed=3)
+    x = _rand((R, K), 4)
+    call = gg.gmm_w4_swiglu if swiglu else gg.gmm_w4
+    for bs in (sizes, sizes.to(dev())):
+        _check(call(x, w, bs), x, ref, s, sizes, group, swiglu, True)
+    size, ptr = gg.get_arguments(E, dev())
+    own = call(x, w, sizes, workspace=torch.empty(size, dtype=torch.uint8, device=dev()), arguments_ptr=ptr)
+    assert torch.equal(own, call(x, w, sizes))
+    gg.release_arguments(ptr)
+
+
+def test_rows_keep_apart_and_rows_behind():
+    announce(test="w4_apart")
+    sizes = torch.tensor([3, 0, 20, 7])
+    E, K, N, R = 4, 264, 64, 30
+    w, ref, s = _weight(E, N, K, 32, True, seed=5)
+    x = _rand((R + 9, K), 6)
+    clean = gg.gmm_w4(x, w, sizes)[:R].clone()
+    x[1], x[10], x[R:] = float("nan"), float("inf"), float("nan")
+    c = torch.full((R + 20, N), 7.0, dtype=torch.bfloat16, device=dev())
+    out = gg.gmm_w4(x, w, sizes, c=c)
+    assert out.data_ptr() == c.data_ptr() and bool((c[R:] == 7).all())
+    keep = [r for r in range(R) if r not in (1, 10)]
+    assert torch.equal(c[keep], clean[keep]) and not bool(c[[1, 10]].isfinite().any())
+    c.fill_(7)
+    gg.gmm_w4_swiglu(x, w, torch.zeros(E, dtype=torch.int64), c=c[:, :N // 2].contiguous())
+    assert bool((gg.gmm_w4(x, w, torch.zeros(E, dtype=torch.int64).to(dev()), c=c) == 7).all())
+    assert gg.gmm_w4(x[:0], w, torch.zeros(E, dtype=torch.int64)).shape == (0, N)
+    # sizes that overrun the rows are clamped
+    guard = torch.full((R + 4, N), 5.0, dtype=torch.bfloat16, device=dev())
+    gg.gmm_w4(x[:R].contiguous(), w, torch.tensor([3, 0, 20, 700]), c=guard)
+    assert torch.equal(guard[23:R], clean[23:]) and bool((guard[R:] == 5).all())
+
+
+def test_many_experts():
+    announce(test="w4_many_experts")
+    E, K, N = 300, 64, 32
+    sizes = ragged_sizes(E, 500, seed=9)
+    w, ref, s = _weight(E, N, K, 32, False, seed=8)
+    x = _rand((500, K), 9)
+    _check(gg.gmm_w4(x, w, sizes.to(dev())), x, ref, s, sizes, 32, False, False)
+
+
+def test_sums_that_nearly_cancel():
+    announce(test="w4_cancel")
+    # every code is the zero point: the weights are zero whatever the rows
+    E, K, N = 1, 512, 32
+    q = torch.full((E, N, K), 8, dtype=torch.uint8, device=dev())
+    s = torch.ones(E, N, K // 128, dtype=torch.bfloat16, device=dev())
+    x = _rand((5, K), 2) + 3
+    out = gg.gmm_w4(x, gg.pack_w4(q, s, None, 128), torch.tensor([5]))
+    assert bool((out.double().abs() <= ACC * 136 * 47 * x.double().abs().sum(1, keepdim=True)).all())
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("K,N", [(128, 48), (72, 24), (328, 136)])
+def test_quantisation(K, N, group, zeros):
+    announce(test="w4_quant", K=K, N=N, group=group, zeros=zeros)
+    E = 2
+    w = _rand((E, K, N), K, 0.02)
+    w[0, :, 3] = 0                                               # a column of zeros
+    w[1, :, 5] = w[1, :, 5].abs() + 0.01                         # one without a negative weight
+    w[0, 7, 7] = 4.0                                             # one with an outlier
+    p = gg.quantize_weight_w4(w, group, zeros)
+    q, s, z = unpack(p)
+    assert int(q.max()) <= 15 and bool((s.double() >= 0).all())
+    spread = lambda v: v.double().repeat_interleave(group, 2)[:, :, :K]
+    step = spread(s)
+    value = (q.double() - (8.0 if z is None else spread(z))) * step
+    wt = w.cpu().double().transpose(1, 2)
+    # off by half a step; at the ends by what rounding the step to bf16 moves them (7 or 15 steps by HALF each, with zero
+    # points half a step more, by which the zero point is off its place)
+    off = (0.5 + (15 * HALF + 0.5 if zeros else 7 * HALF)) * step + 1e-6
+    assert bool(((value - wt).abs() <= off).all()), float(((value - wt).abs() / step.clamp(min=1e-9)).max())
+    assert bool((value[0, 3] == 0).all())
+    assert torch.equal(gg.dequantize_w4(p).cpu(), value.to(torch.bfloat16))
+    again = gg.pack_w4(q, s, z, group)
+    assert torch.equal(again.codes, p.codes.cpu()) and torch.equal(again.scales, p.scales.cpu())
+
+
+@pytest.mark.parametrize("T", [1, 40, 700])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_layer(T, zeros):
+    announce(test="w4_layer", T=T, zeros=zeros)
+    # quantise, then the whole step: route -> permute -> 4-bit experts -> combine
+    E, d, I, k = 8, 256, 328, 2
+    w13, w2 = _rand((E, d, 2 * I), 1, 0.05), _rand((E, I, d), 2, 0.05)
+    layer = MoEExpertsW4(w13, w2, group=64, zeros=zeros)
+    assert sorted(n for n, _ in layer.named_buffers()) == sorted(
+        [f"{w}_{t}" for w in ("w13", "w2") for t in ("codes", "scales") + (("zeros",) if zeros else ())])
+    g = torch.Generator().manual_seed(T)
+    x = _rand((T, d), 3)
+    ids = torch.argsort(torch.rand(T, E, generator=g), dim=1)[:, :k].to(torch.int32).to(dev())
+    gates = torch.softmax(torch.randn(T, k, generator=g), 1).to(dev())
+    stages = {}
+    out = expert_layer_forward(layer, x, ids, gates, stages=stages)
+    b13 = gg.dequantize_w4(gg.quantize_weight_w4(w13, 64, zeros)).double()
+    b2 = gg.dequantize_w4(gg.quantize_weight_w4(w2, 64, zeros)).double()
+    xd, want = x.double(), torch.zeros(T, d, dtype=torch.float64, device=dev())
+    for j in range(k):
+        for t in range(T):
+            e = int(ids[t, j])
+            u = b13[e] @ xd[t]
+            want[t] += float(gates[t, j]) * (b2[e] @ (torch.nn.functional.silu(u[:I]) * u[I:]))
+    # roundings: the reference's weights, the intermediate, the rows and the sum: four of them, of the terms of sums of I
+    # and d elements that are as good as independent: a tenth of the largest value at most is never reached
+    assert float((out.double() - want).abs().max()) <= 4 * HALF * float(want.abs().max())
+    sizes = stages["batch_sizes"]
+    again = layer.forward(T * k, stages["permuted"], sizes, host_batch_sizes=sizes.cpu())
+    assert torch.equal(again, stages["expert_out"]) or T > 100
+    ready = MoEExpertsW4(gg.quantize_weight_w4(w13, 64, zeros), gg.quantize_weight_w4(w2, 64, zeros))
+    assert torch.equal(ready.forward(T * k, stages["permuted"], sizes), stages["expert_out"])
+
+
+@pytest.mark.parametrize("T", [6, 400])
+def test_graph_replays_and_streams(T):
+    announce(test="w4_graph", T=T)
+    E, d, I = 4, 256, 136
+    layer = MoEExpertsW4(_rand((E, d, 2 * I), 1, 0.05), _rand((E, I, d), 2, 0.05), group=32, zeros=True)
+    x = torch.zeros(T * 2, d, dtype=torch.bfloat16, device=dev())
+    sizes = torch.zeros(E, dtype=torch.int64, device=dev())
+    sizes[0] = T * 2
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer.forward(T * 2, x, sizes)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer.forward(T * 2, x, sizes)
+    for rep in range(4):
+        x.copy_(_rand((T * 2, d), rep))
+        sizes.copy_(ragged_sizes(E, T * 2, seed=rep, empty_every=rep + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        with torch.cuda.stream(side):
+            side.wait_stream(torch.cuda.default_stream())
+            want = layer.forward(T * 2, x, sizes)
+        side.synchronize()
+        assert torch.equal(got, want), rep
+
+
+def test_refusals():
+    announce(test="w4_refusals")
+    w, _, _ = _weight(2, 32, 64, 32, True, 1)
+    x, n = _rand((4, 64), 1), torch.tensor([2, 2])
+    for bad in (x.float(), x[:, :56], x.t().contiguous().t(), x.cpu()):
+        with pytest.raises(AssertionError):
+            gg.gmm_w4(bad, w, n)
+    for bad in (w._replace(K=72), w._replace(N=40), w._replace(group=64), w._replace(scales=w.scales.float()), w._replace(zeros=w.scales),
+                w._replace(codes=w.codes[:1])):
+        with pytest.raises(AssertionError):
+            gg.gmm_w4(x, bad, n)
+    with pytest.raises(ValueError):
+        gg.gmm_w4(x, w._replace(group=16), n)
+    with pytest.raises(AssertionError):
+        gg.gmm_w4(x, w, torch.tensor([4]))
+    w8, _, _ = _weight(2, 24, 64, 32, True, 1)
+    with pytest.raises(AssertionError):
+        gg.gmm_w4_swiglu(x, w8, n)
+    with pytest.raises(AssertionError):
+        gg.quantize_weight_w4(_rand((2, 64, 32), 1).float())
+    with pytest.raises(RuntimeError, match="multiple of 8"):
+        gg.quantize_weight_w4(_rand((1, 12, 16), 1))
