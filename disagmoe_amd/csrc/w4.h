@@ -8,11 +8,12 @@
 //   * the codes lie in tiles of 16 columns x 128 k, 1 KiB that a wavefront loads with one 16-byte instruction; lane
 //     16 g + r gets column r, its word j the 8 codes of k = 32 j + 8 g ..: an operand of v_mfma_f32_16x16x32_bf16;
 //   * a code becomes a bf16 without a conversion: bf16 16.0 has its units at bit 3, so nibble << 3 | 0x4180 is 16 + q
-//     exactly, two codes for one shift and one and-or.  The sum over a group then needs 16 + z times the group's sum of
-//     x taken off, which one more matrix instruction per k-step gives (weights of 1) to every lane that needs it:
-//         c += s (sum (16 + q) x - (16 + z) sum x)
-//     once for a group and four results a lane.  The weights are never rounded; the price is a sum whose terms are up to
-//     31 instead of 15 times |x|, some two bits of the 24 that fp32 holds;
+//     exactly, two codes for one shift and one and-or.  What that is too much, 16 + z times the group's sum of x, comes
+//     from one more matrix instruction per k-step, on weights of -24 (z = 8) or -16: its result is what the sums over the
+//     group begin with, so without zero points a group costs one fused multiply-add per result and lane:
+//         c += s (sum (16 + q) x - 24 sum x)     or     c += s (sum (16 + q) x - 16 sum x - z sum x)
+//     The weights are never rounded; the price is a sum whose terms are up to 31 instead of 15 times |x|, some two bits
+//     of the 24 that fp32 holds;
 //   * the wavefronts of a workgroup split k (chunk c goes to wavefront c mod WK, so that they read a contiguous stretch
 //     together) and meet in LDS, where the sums are added in the order of the wavefronts: many bytes in flight on a
 //     matrix of few columns, no atomics, the same bits every time.
@@ -77,9 +78,9 @@ __device__ __forceinline__ int w4_locate(const W4Args &p, int m, int &expert, in
         if (behind != 0 && tile_carry <= m) {
             const int at = __ffsll((unsigned long long)behind) - 1;
             const int in = m - (tile_carry + __shfl(tincl - mt, at, kWave));
-            expert = __builtin_amdgcn_readfirstlane(e0 + at);
-            row0 = __builtin_amdgcn_readfirstlane((int)__shfl(start, at, kWave) + in * BM);
-            const int left = __builtin_amdgcn_readfirstlane((int)__shfl(end, at, kWave)) - row0;
+            expert = e0 + at;
+            row0 = (int)__shfl(start, at, kWave) + in * BM;
+            const int left = (int)__shfl(end, at, kWave) - row0;
             rows = left < BM ? left : BM;
         }
         row_carry += __shfl(incl, kWave - 1, kWave);
@@ -88,142 +89,89 @@ __device__ __forceinline__ int w4_locate(const W4Args &p, int m, int &expert, in
     return __builtin_amdgcn_readfirstlane(tile_carry);
 }
 
-// FM row fragments of 16, FG column fragments of 16 per wavefront (SWIGLU: of the result, with as many of the gate and of
-// the up columns; SHIFT: the up columns begin in the middle of a tile, one more), WN wavefronts along the columns, WK
-// along k.
-template <int FM, int FG, int WN, int WK, int G, bool ZERO, bool SWIGLU, bool SHIFT>
-__global__ __launch_bounds__(WN *WK *kWave) void gmm_w4_kernel(const W4Args p) {
-    constexpr int BM = 16 * FM;
-    constexpr int NF = SWIGLU ? 2 * FG + (SHIFT ? 1 : 0) : FG;
-    constexpr int NG = kW4Chunk / G;          // groups of a chunk
-    constexpr int SG = G / 32;                // k-steps of a group
-    constexpr int BN = 16 * FG * WN;          // columns of the result per workgroup
-    constexpr int kPart = NF * BM * 16;       // floats that a wavefront brings to the meeting
-    static_assert(!SHIFT || SWIGLU, "only the gated form has two runs of columns");
-    extern __shared__ __attribute__((aligned(16))) float red[];
-
-    const int lane = lane_id();
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int wn = wave % WN, wk = wave / WN;
-    const int l16 = lane & 15, g16 = lane >> 4;
-
-    // workgroup -> (column tile, row tile): the row tiles of a column tile one after the other on one XCD, whose L2 then
-    // holds the column tile's codes
-    const int id = blockIdx.x;
-    const int oct = id / (kXcds * p.m_tiles), in = id - oct * (kXcds * p.m_tiles);
-    const int ntile = oct * kXcds + in % kXcds;
-    const int n0 = ntile * BN;
-    if (n0 >= p.n_out) return;
-    // (one round, unless the grid was laid out for sizes that say less than batch_sizes do)
-    for (int m_tile = in / kXcds, total = m_tile + 1; m_tile < total; m_tile += p.m_tiles) {
-    int e = 0, row0 = 0, rows = 0;
-    total = w4_locate<BM>(p, m_tile, e, row0, rows);
-    if (m_tile >= total) break;
-
-    // ---- where this wavefront's fragments lie ----
-    const int c0 = n0 + wn * (16 * FG);                       // its first column of the result
-    constexpr int kScaleTile = kW4Cols * NG;                  // scales of a tile
+// What a wavefront holds of one chunk of 128 k: the codes, scales and zero points of its NF fragments of 16 columns.
+template <int NF, int NG, bool ZERO>
+struct W4Weights {
+    u32x4 q[NF];
+    uint32_t s[NF][NG * 2];
+    uint32_t z[ZERO ? NF : 1][NG];
+};
+// Where they lie (wave-uniform), and how they are loaded.
+template <int NF, int NG, bool ZERO>
+struct W4Source {
     const char *code_at[NF], *scale_at[NF], *zero_at[NF];
-#pragma unroll
-    for (int f = 0; f < NF; ++f) {
-        int t = SWIGLU && f >= FG ? (p.n_out + c0) / 16 + (f - FG) : c0 / 16 + f;
+    static constexpr int kScaleTile = kW4Cols * NG;           // scales of a tile
+    __device__ __forceinline__ void aim(const W4Args &p, int f, int e, int t) {
         t = t < p.nt ? t : p.nt - 1;                          // past the end: read, never stored
         const size_t tile = ((size_t)e * p.nt + t) * p.kt;
         code_at[f] = p.codes + tile * kW4TileBytes;
         scale_at[f] = p.scales + tile * (kScaleTile * 2);
         zero_at[f] = ZERO ? p.zeros + tile * kScaleTile : nullptr;
     }
-    const char *x_at[FM];
-#pragma unroll
-    for (int i = 0; i < FM; ++i) {
-        const int m = i * 16 + l16;
-        x_at[i] = p.x + ((size_t)(row0 + (m < rows ? m : rows - 1)) * p.K + g16 * 8) * 2;   // past the end: the last row
-    }
-
-    struct Chunk {
-        u32x4 q[NF];
-        uint32_t s[NF][NG * 2];
-        uint32_t z[ZERO ? NF : 1][NG];
-        bf16x8 x[FM][4];
-    };
-    const int whole = p.K / kW4Chunk;                         // chunks that lie inside K
-    auto load = [&](Chunk &b, int c) {
+    __device__ __forceinline__ void load(W4Weights<NF, NG, ZERO> &b, int c, int lane) const {
 #pragma unroll
         for (int f = 0; f < NF; ++f) {
-            b.q[f] = *(const u32x4 *)(code_at[f] + (uint32_t)c * kW4TileBytes + lane * 16);
-            __builtin_memcpy(b.s[f], scale_at[f] + (uint32_t)c * (kScaleTile * 2) + g16 * (NG * 8), NG * 8);
-            if constexpr (ZERO) __builtin_memcpy(b.z[f], zero_at[f] + (uint32_t)c * kScaleTile + g16 * (NG * 4), NG * 4);
+            b.q[f] = *(const u32x4 *)(code_at[f] + ((uint32_t)c * kW4TileBytes + lane * 16));
+            __builtin_memcpy(b.s[f], scale_at[f] + ((uint32_t)c * (kScaleTile * 2) + (lane >> 4) * (NG * 8)), NG * 8);
+            if constexpr (ZERO) __builtin_memcpy(b.z[f], zero_at[f] + ((uint32_t)c * kScaleTile + (lane >> 4) * (NG * 4)), NG * 4);
         }
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                u32x4 v = {0, 0, 0, 0};
-                if (c < whole || c * kW4Chunk + j * 32 + g16 * 8 < p.K) v = *(const u32x4 *)(x_at[i] + (uint32_t)c * (kW4Chunk * 2) + j * 64);
-                __builtin_memcpy(&b.x[i][j], &v, 16);
-            }
-    };
-
-    f32x4 acc[NF][FM];
-#pragma unroll
-    for (int f = 0; f < NF; ++f)
-#pragma unroll
-        for (int i = 0; i < FM; ++i) acc[f][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const u32x4 one_bits = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-    bf16x8 ones;
-    __builtin_memcpy(&ones, &one_bits, 16);
-
-    auto compute = [&](const Chunk &b) {
-        float xs[FM][NG];                                     // the groups' sums of x in this lane's row
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                f32x4 t = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int j = g * SG; j < (g + 1) * SG; ++j) t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, b.x[i][j], t, 0, 0, 0);
-                xs[i][g] = ZERO ? t[0] : t[0] * 24.f;         // (no zero points: 16 + 8)
-            }
-#pragma unroll
-        for (int f = 0; f < NF; ++f)
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                f32x4 t[FM];
-#pragma unroll
-                for (int j = g * SG; j < (g + 1) * SG; ++j) {
-                    u32x4 w;
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) w[q] = w4_pair(b.q[f][j], q);
-                    bf16x8 wf;
-                    __builtin_memcpy(&wf, &w, 16);
-#pragma unroll
-                    for (int i = 0; i < FM; ++i)
-                        t[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, b.x[i][j], j == g * SG ? f32x4{0.f, 0.f, 0.f, 0.f} : t[i], 0, 0, 0);
-                }
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const uint32_t pair = b.s[f][g * 2 + x / 2];
-                    const float s = __uint_as_float(x & 1 ? pair & 0xffff0000u : pair << 16);
-                    const float off = ZERO ? 16.f + (float)((b.z[ZERO ? f : 0][g] >> (8 * x)) & 0xffu) : 0.f;
-#pragma unroll
-                    for (int i = 0; i < FM; ++i)
-                        acc[f][i][x] = fmaf(s, ZERO ? fmaf(-off, xs[i][g], t[i][x]) : t[i][x] - xs[i][g], acc[f][i][x]);
-                }
-            }
-    };
-
-    // one chunk ahead: the next one's loads are on their way while this one is worked on
-    Chunk even, odd;
-    int c = wk;
-    if (c < p.kt) load(even, c);
-    for (; c < p.kt; c += 2 * WK) {
-        if (c + WK < p.kt) load(odd, c + WK);
-        compute(even);
-        if (c + 2 * WK < p.kt) load(even, c + 2 * WK);
-        if (c + WK < p.kt) compute(odd);
     }
+};
 
-    // ---- the wavefronts that split k meet: red[wk][wn][fragment][row][16 columns] ----
+// acc[f][i] += the products of a chunk's weights with the row fragments x(i, j) of its k-steps j
+template <int FM, int NF, int NG, bool ZERO, typename X>
+__device__ __forceinline__ void w4_chunk(f32x4 (&acc)[NF][FM], const W4Weights<NF, NG, ZERO> &b, X &&x_of) {
+    constexpr int SG = 4 / NG;                                // k-steps of a group
+    const uint32_t less = ZERO ? 0xc180c180u : 0xc1c0c1c0u;   // -16 or -24 as two bf16
+    const u32x4 less4 = {less, less, less, less};
+    bf16x8 lf;
+    __builtin_memcpy(&lf, &less4, 16);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+        bf16x8 x[FM][SG];
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < SG; ++j) x[i][j] = x_of(i, g * SG + j);
+        f32x4 base[FM];                                       // -24 (-16) times the group's sum of x in this lane's row
+#pragma unroll
+        for (int i = 0; i < FM; ++i) base[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = g * SG; j < (g + 1) * SG; ++j)
+#pragma unroll
+            for (int i = 0; i < FM; ++i) base[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lf, x[i][j - g * SG], base[i], 0, 0, 0);
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            f32x4 t[FM];
+#pragma unroll
+            for (int j = g * SG; j < (g + 1) * SG; ++j) {
+                u32x4 w;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) w[q] = w4_pair(b.q[f][j], q);
+                bf16x8 wf;
+                __builtin_memcpy(&wf, &w, 16);
+#pragma unroll
+                for (int i = 0; i < FM; ++i) t[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, x[i][j - g * SG], j == g * SG ? base[i] : t[i], 0, 0, 0);
+            }
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const uint32_t pair = b.s[f][g * 2 + v / 2];
+                const float s = __uint_as_float(v & 1 ? pair & 0xffff0000u : pair << 16);
+                const float zs = ZERO ? (float)((b.z[ZERO ? f : 0][g] >> (8 * v)) & 0xffu) * 0.0625f : 0.f;   // z / 16, exactly
+#pragma unroll
+                for (int i = 0; i < FM; ++i) acc[f][i][v] = fmaf(s, ZERO ? fmaf(zs, base[i][v], t[i][v]) : t[i][v], acc[f][i][v]);
+            }
+            __builtin_amdgcn_sched_barrier(0);                // one fragment's sums in registers at a time
+        }
+    }
+}
+
+// The wavefronts that split k meet: red[wk][wn][fragment][row][16 columns].  Sums in the order of the wavefronts, the
+// gated form's activation, one rounding, out by quads of columns.
+template <int FM, int FG, int WN, int WK, bool SWIGLU, bool SHIFT, int NF>
+__device__ __forceinline__ void w4_finish(const W4Args &p, float *red, const f32x4 (&acc)[NF][FM], int wk, int wn, int row0, int rows, int n0) {
+    constexpr int BM = 16 * FM, BN = 16 * FG * WN, kPart = NF * BM * 16;
+    const int lane = lane_id(), l16 = lane & 15, g16 = lane >> 4;
     float *mine = red + (wk * WN + wn) * kPart;
 #pragma unroll
     for (int f = 0; f < NF; ++f)
@@ -253,14 +201,139 @@ __global__ __launch_bounds__(WN *WK *kWave) void gmm_w4_kernel(const W4Args p) {
         pk.y = pack_bf16x2(v[2], v[3]);
         *(uint2 *)((uint16_t *)p.c + (size_t)(row0 + m) * p.n_out + n0 + col) = pk;
     }
-    __syncthreads();                                          // read: the next round may bring its sums
+    __syncthreads();                                          // read: the LDS may be written again
+}
+
+// FM row fragments of 16, FG column fragments of 16 per wavefront (SWIGLU: of the result, with as many of the gate and of
+// the up columns; SHIFT: the up columns begin in the middle of a tile, one more), WN wavefronts along the columns, WK
+// along k.  Up to 32 rows (FM 1, 2): the rows come straight from the caches into registers and four (three)
+// wavefronts to a SIMD keep loads in flight.  64 rows (FM 4): the sums leave room for two, so weights and rows are fetched a
+// round ahead, and all wavefronts bring the WK chunks of a round into LDS, once for the WN wavefronts that read each.
+template <int FM, int FG, int WN, int WK, int G, bool ZERO, bool SWIGLU, bool SHIFT>
+__global__ __launch_bounds__(WN *WK *kWave) __attribute__((amdgpu_waves_per_eu(FM == 1 ? 4 : (FM == 2 ? 3 : 2))))
+void gmm_w4_kernel(const W4Args p) {
+    constexpr int BM = 16 * FM;
+    constexpr int NF = SWIGLU ? 2 * FG + (SHIFT ? 1 : 0) : FG;
+    constexpr int NG = kW4Chunk / G;          // groups of a chunk
+    constexpr int BN = 16 * FG * WN;          // columns of the result per workgroup
+    constexpr bool kShare = FM > 2;
+    static_assert(!SHIFT || SWIGLU, "only the gated form has two runs of columns");
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+
+    const int lane = lane_id();
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int wn = wave % WN, wk = wave / WN;
+    const int l16 = lane & 15, g16 = lane >> 4;
+
+    // workgroup -> (column tile, row tile): the row tiles of a column tile one after the other on one XCD, whose L2 then
+    // holds the column tile's codes
+    const int id = blockIdx.x;
+    const int oct = id / (kXcds * p.m_tiles), in = id - oct * (kXcds * p.m_tiles);
+    const int n0 = (oct * kXcds + in % kXcds) * BN;
+    if (n0 >= p.n_out) return;
+    // (one round, unless the grid was laid out for sizes that say less than batch_sizes do)
+    for (int m_tile = in / kXcds, total = m_tile + 1; m_tile < total; m_tile += p.m_tiles) {
+        int e = 0, row0 = 0, rows = 0;
+        total = w4_locate<BM>(p, m_tile, e, row0, rows);
+        if (m_tile >= total) break;
+        // (the same in every lane, which the compiler does not see through the search)
+        e = __builtin_amdgcn_readfirstlane(e); row0 = __builtin_amdgcn_readfirstlane(row0); rows = __builtin_amdgcn_readfirstlane(rows);
+        const int c0 = n0 + wn * (16 * FG);                   // this wavefront's first column of the result
+        W4Source<NF, NG, ZERO> src;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) src.aim(p, f, e, SWIGLU && f >= FG ? (p.n_out + c0) / 16 + (f - FG) : c0 / 16 + f);
+        f32x4 acc[NF][FM];
+#pragma unroll
+        for (int f = 0; f < NF; ++f)
+#pragma unroll
+            for (int i = 0; i < FM; ++i) acc[f][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const int whole = p.K / kW4Chunk;                     // chunks that lie inside K
+
+        if constexpr (!kShare) {
+            const char *x_at[FM];
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+                const int m = i * 16 + l16;
+                x_at[i] = p.x + ((size_t)(row0 + (m < rows ? m : rows - 1)) * p.K + g16 * 8) * 2;   // past the end: the last row
+            }
+#pragma unroll 1
+            for (int c = wk; c < p.kt; c += WK) {
+                W4Weights<NF, NG, ZERO> b;
+                src.load(b, c, lane);
+                bf16x8 x[FM][4];
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        u32x4 v = {0, 0, 0, 0};
+                        if (c < whole || c * kW4Chunk + j * 32 + g16 * 8 < p.K) v = *(const u32x4 *)(x_at[i] + ((uint32_t)c * (kW4Chunk * 2) + j * 64));
+                        __builtin_memcpy(&x[i][j], &v, 16);
+                    }
+                __builtin_amdgcn_sched_barrier(0);            // every load of the chunk is on its way
+                w4_chunk<FM>(acc, b, [&](int i, int j) { return x[i][j]; });
+            }
+        } else {
+            // A round brings WK chunks of BM rows x 256 bytes, kept in LDS with the 16-byte piece q of row r at q ^ (r & 15):
+            // the 16 rows of an operand read, 256 bytes apart, then lie in different banks.
+            constexpr int kRound = WK * BM * 256;
+            constexpr int kPieces = kRound / 16 / (WN * WK * kWave);   // of a thread
+            static_assert(kPieces * 16 * WN * WK * kWave == kRound, "whole pieces");
+            u32x4 px[kPieces];
+            auto load_x = [&](int c) {
+#pragma unroll
+                for (int u = 0; u < kPieces; ++u) {
+                    const int i = threadIdx.x + u * (WN * WK * kWave);
+                    const int m = (i / 16) % BM, k = (c + i / (16 * BM)) * kW4Chunk + (i % 16) * 8;
+                    px[u] = u32x4{0, 0, 0, 0};
+                    if (k < p.K) px[u] = *(const u32x4 *)(p.x + ((size_t)(row0 + (m < rows ? m : rows - 1)) * p.K + k) * 2);
+                }
+            };
+            auto store_x = [&](int buf) {
+#pragma unroll
+                for (int u = 0; u < kPieces; ++u) {
+                    const int i = threadIdx.x + u * (WN * WK * kWave);
+                    const int r = i / 16;                     // row of the round: chunk * BM + row
+                    *(u32x4 *)(smem + buf * kRound + r * 256 + (((i % 16) ^ (r & 15)) << 4)) = px[u];
+                }
+            };
+            W4Weights<NF, NG, ZERO> now, next;
+            load_x(0);
+            if (wk < p.kt) src.load(now, wk, lane);
+            store_x(0);
+            __syncthreads();
+            int buf = 0;
+            for (int c = 0; c < p.kt; c += WK, buf ^= 1) {    // the same rounds for every wavefront: they share the barriers
+                const bool more = c + WK < p.kt;
+                if (more) {
+                    load_x(c + WK);
+                    if (c + WK + wk < p.kt) src.load(next, c + WK + wk, lane);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                if (c + wk < p.kt) {
+                    const char *round = smem + buf * kRound + (wk * BM + l16) * 256;
+                    w4_chunk<FM>(acc, now, [&](int i, int j) {
+                        const u32x4 v = *(const u32x4 *)(round + i * (16 * 256) + (((j * 4 + g16) ^ l16) << 4));
+                        bf16x8 x;
+                        __builtin_memcpy(&x, &v, 16);
+                        return x;
+                    });
+                }
+                if (more) {
+                    store_x(buf ^ 1);
+                    now = next;
+                }
+                __syncthreads();
+            }
+        }
+        w4_finish<FM, FG, WN, WK, SWIGLU, SHIFT, NF>(p, (float *)smem, acc, wk, wn, row0, rows, n0);
     }
 }
 
 template <int FM, int FG, int WN, int WK, int G, bool ZERO, bool SWIGLU, bool SHIFT>
 static int launch_w4_one(const W4Args &args, hipStream_t stream) {
     constexpr int NF = SWIGLU ? 2 * FG + (SHIFT ? 1 : 0) : FG;
-    constexpr int lds = WN * WK * NF * 16 * FM * 16 * (int)sizeof(float);
+    constexpr int meet = WN * WK * NF * 16 * FM * 16 * (int)sizeof(float), rows = FM > 2 ? 2 * WK * 16 * FM * 256 : 0;
+    constexpr int lds = meet > rows ? meet : rows;
     static_assert(lds <= 160 * 1024, "LDS of a compute unit");
     auto kern = gmm_w4_kernel<FM, FG, WN, WK, G, ZERO, SWIGLU, SHIFT>;
     static unsigned long long configured = 0;   // devices on which the kernel's LDS size has been raised
@@ -277,7 +350,7 @@ template <int FM, int FG, int WN, int WK, int G, bool ZERO>
 static int launch_w4_form(const W4Args &args, bool swiglu, hipStream_t stream) {
     if (!swiglu) return launch_w4_one<FM, 2 * FG, WN, WK, G, ZERO, false, false>(args, stream);
     if (args.n_out % 16 == 0) return launch_w4_one<FM, FG, WN, WK, G, ZERO, true, false>(args, stream);
-    return launch_w4_one<FM, FG, WN, WK, G, ZERO, true, true>(args, stream);
+    return launch_w4_one<FM, FG / 2, WN, WK, G, ZERO, true, true>(args, stream);
 }
 
 template <int FM, int FG, int WN, int WK>

@@ -3,6 +3,6 @@
 
 namespace dmoe {
 
-int launch_w4_64(const W4Args &args, int group, bool swiglu, hipStream_t stream) { return launch_w4_rows<4, 2, 2, 4>(args, group, swiglu, stream); }
+int launch_w4_64(const W4Args &args, int group, bool swiglu, hipStream_t stream) { return launch_w4_rows<4, 2, 4, 2>(args, group, swiglu, stream); }
 
 }  // namespace dmoe
