@@ -32,7 +32,8 @@ constexpr int kDK32 = 32;          // k per stage of the global -> LDS bf16 kern
 __device__ __forceinline__ int swz(int row) { return (row >> 1) & 7; }
 __device__ __forceinline__ int lds_off(int row, int chunk) { return row * kRowBytes + ((chunk ^ swz(row)) << 4); }
 
-template <int BM, int BN, int WM, int WN, bool TRANS_B, bool SWIGLU, bool FP8>
+// KEEP (bf16, gated form): the fp32 sums also go to p.u, for the activation's gradient.
+template <int BM, int BN, int WM, int WN, bool TRANS_B, bool SWIGLU, bool FP8, bool KEEP = false>
 __global__ __launch_bounds__(WM *WN *kWave) __attribute__((amdgpu_waves_per_eu(WM *WN / 4, WM *WN / 4)))
 void gmm_kernel(const GmmArgs p) {
     constexpr int NT = WM * WN * kWave;          // threads
@@ -369,6 +370,13 @@ void gmm_kernel(const GmmArgs p) {
                             sb1[0] = t1.x; sb1[1] = t1.y; sb1[2] = t1.z; sb1[3] = t1.w;
                         }
                     }
+                    if constexpr (KEEP) {
+                        float *u = p.u + (long long)(row0 + r) * p.N + col;
+                        const f32x4 gate = {acc[i][j][g * 4], acc[i][j][g * 4 + 1], acc[i][j][g * 4 + 2], acc[i][j][g * 4 + 3]};
+                        const f32x4 up = {acc[i][j + FN / 2][g * 4], acc[i][j + FN / 2][g * 4 + 1], acc[i][j + FN / 2][g * 4 + 2], acc[i][j + FN / 2][g * 4 + 3]};
+                        *(f32x4 *)u = gate;
+                        *(f32x4 *)(u + n_out) = up;
+                    }
                     float v[4];
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
@@ -391,12 +399,12 @@ void gmm_kernel(const GmmArgs p) {
     sched_finish(p.sched, tid == 0, draw, streams, total);
 }
 
-template <int BM, int BN, int WM, int WN, bool TRANS_B, bool SWIGLU, bool FP8>
+template <int BM, int BN, int WM, int WN, bool TRANS_B, bool SWIGLU, bool FP8, bool KEEP = false>
 static int launch_one(const GmmArgs &args, hipStream_t stream) {
     constexpr int NT = WM * WN * kWave;
     static_assert(BN == 256, "launch_grid counts tiles of 256 columns");
     const size_t lds = 2 * (size_t)(BM + BN) * kRowBytes;
-    auto kern = gmm_kernel<BM, BN, WM, WN, TRANS_B, SWIGLU, FP8>;
+    auto kern = gmm_kernel<BM, BN, WM, WN, TRANS_B, SWIGLU, FP8, KEEP>;
     static unsigned long long configured = 0;   // devices on which the kernel's LDS size has been raised
     DMOE_HIP(raise_dynamic_lds((const void *)kern, (int)lds, &configured));
     const long long grid = launch_grid(args, BM, SWIGLU, 64, false, device_cus());
@@ -467,7 +475,7 @@ static int own_slot(hipStream_t stream, SchedSlot **out) {
 
 static int bind_state(GmmArgs &args, void *state, void *workspace, size_t workspace_bytes, hipStream_t stream) {
     args.arrive = nullptr; args.partials = nullptr; args.partial_bytes = 0;
-    args.a_rows = nullptr; args.a_src_rows = 0;
+    args.a_rows = nullptr; args.a_src_rows = 0; args.u = nullptr;
     if (state == nullptr) return own_slot(stream, &args.sched);
     DMOE_REQUIRE(((uintptr_t)state & 255) == 0, DMOE_ERR_WORKSPACE, "grouped GEMM: the state block must be 256-byte aligned");
     args.sched = (SchedSlot *)state;
@@ -563,6 +571,18 @@ static int launch_by_rows(const GmmArgs &args, hipStream_t stream) {
     if (L.kernel == kKernelWave128Fp8) return launch_wave128_fp8(args, SWIGLU, stream);
     if constexpr (FP8) return launch_direct_fp8(args, L.tile_rows, SWIGLU, stream);
     else return launch_direct_bf16(args, L.tile_rows, TRANS_B, SWIGLU, stream);
+}
+
+// The gated form that also leaves its fp32 sums in args.u.
+template <bool TRANS_B>
+static int launch_keep(const GmmArgs &args, hipStream_t stream) {
+    GmmLaunch L = choose_launch(args, TRANS_B, true, false);
+    if (L.kernel == kKernelStaged) {
+        if (L.tile_rows == 64) return launch_one<64, 256, 1, 4, TRANS_B, true, false, true>(args, stream);
+        if (L.tile_rows == 128) return launch_one<128, 256, 1, 4, TRANS_B, true, false, true>(args, stream);
+        return launch_one<256, 256, 2, 4, TRANS_B, true, false, true>(args, stream);
+    }
+    return launch_direct_keep(args, L.tile_rows, TRANS_B, stream);
 }
 
 static int check_shape(const char *who, int64_t rows, int E, int64_t K, int64_t N, int align) {
@@ -676,18 +696,24 @@ extern "C" int dmoe_gmm_swiglu(const void *a, const void *b, void *h, const int6
                    : launch_by_rows<false, true, false>(args, (hipStream_t)stream);
 }
 
-extern "C" int dmoe_gmm_swiglu_keep(const void *a, const void *b, void *h, void *u, const int64_t *batch_sizes, int64_t rows, int E,
+extern "C" int dmoe_gmm_swiglu_keep(const void *a, const void *b, void *h, float *u, const int64_t *batch_sizes, int64_t rows, int E,
                                     int64_t K, int64_t I, int trans_b, int dtype, void *state, void *workspace,
                                     size_t workspace_bytes, const int64_t *host_batch_sizes, void *stream) {
+    const HostSizes known(host_batch_sizes);
     DMOE_REQUIRE(dtype == DMOE_BF16, DMOE_ERR_DTYPE, "dmoe_gmm_swiglu_keep: dtype %d (bf16 only)", dtype);
     int rc = check_gmm("dmoe_gmm_swiglu_keep", a, b, h, batch_sizes, rows, E, K, I, 8);
     if (rc != DMOE_OK) return rc;
     DMOE_REQUIRE(rows == 0 || u != nullptr, DMOE_ERR_ARG, "dmoe_gmm_swiglu_keep: null pointer");
     DMOE_REQUIRE((((uintptr_t)a | (uintptr_t)b | (uintptr_t)h | (uintptr_t)u) & 15) == 0, DMOE_ERR_ARG,
                  "dmoe_gmm_swiglu_keep: a pointer is not 16-byte aligned");
-    rc = dmoe_gmm(a, b, u, batch_sizes, rows, E, K, 2 * I, trans_b, dtype, state, workspace, workspace_bytes, host_batch_sizes, stream);
-    if (rc != DMOE_OK || rows == 0) return rc;
-    return launch_swiglu_forward(u, h, batch_sizes, rows, E, I, (hipStream_t)stream);
+    if (rows == 0) return DMOE_OK;
+    GmmArgs args{(const char *)a, (const char *)b, (char *)h, batch_sizes, nullptr, nullptr, rows, E, (int)K, (int)(2 * I), (int)I};
+    rc = bind_state(args, state, workspace, workspace_bytes, (hipStream_t)stream);
+    if (rc != DMOE_OK) return rc;
+    args.u = u;
+    rc = trans_b ? launch_keep<true>(args, (hipStream_t)stream) : launch_keep<false>(args, (hipStream_t)stream);
+    if (rc != DMOE_OK) return rc;
+    return dmoe_zero_rows_behind(h, batch_sizes, rows, E, I, dtype, stream);
 }
 
 extern "C" int dmoe_gmm_wgrad(const void *a, const void *dc, void *db, const int64_t *batch_sizes, int64_t rows, int E,
@@ -707,7 +733,7 @@ extern "C" int dmoe_gmm_wgrad(const void *a, const void *dc, void *db, const int
     return launch_wgrad(args, (hipStream_t)stream);
 }
 
-extern "C" int dmoe_gmm_swiglu_backward(const void *dh, const void *u, const void *a, const void *b, void *du, void *da, void *db,
+extern "C" int dmoe_gmm_swiglu_backward(const void *dh, const float *u, const void *a, const void *b, void *du, void *da, void *db,
                                         const int64_t *batch_sizes, int64_t rows, int E, int64_t K, int64_t I, int trans_b,
                                         int dtype, void *state, void *workspace, size_t workspace_bytes,
                                         const int64_t *host_batch_sizes, void *stream) {
@@ -720,7 +746,7 @@ extern "C" int dmoe_gmm_swiglu_backward(const void *dh, const void *u, const voi
     DMOE_REQUIRE((((uintptr_t)dh | (uintptr_t)u | (uintptr_t)a | (uintptr_t)b | (uintptr_t)du | (uintptr_t)da | (uintptr_t)db) & 15) == 0,
                  DMOE_ERR_ARG, "dmoe_gmm_swiglu_backward: a pointer is not 16-byte aligned");
     if (rows > 0) {
-        DMOE_REQUIRE(du != u && du != dh && da != dh && da != a, DMOE_ERR_ARG, "dmoe_gmm_swiglu_backward: a result overlaps an input");
+        DMOE_REQUIRE(du != (const void *)u && du != dh && da != dh && da != a, DMOE_ERR_ARG, "dmoe_gmm_swiglu_backward: a result overlaps an input");
         rc = launch_swiglu_backward(dh, u, du, batch_sizes, rows, E, I, da, K, (hipStream_t)stream);
         if (rc == DMOE_OK && da != nullptr)
             rc = dmoe_gmm(du, b, da, batch_sizes, rows, E, 2 * I, K, !trans_b, dtype, state, workspace, workspace_bytes, host_batch_sizes, stream);

@@ -37,6 +37,8 @@ struct GmmArgs {
     // (gmm_tile256_kernel's gathering form) row r of the product is row a_rows[r] of `a`, which has a_src_rows rows
     const int32_t *a_rows;
     long long a_src_rows;
+    // (the gated form's KEEP builds) u [rows, N] in fp32: the sums that the activation is taken of, for its gradient
+    float *u;
 };
 
 // ---- work distribution ---------------------------------------------------------------------------
@@ -361,14 +363,14 @@ inline long long launch_grid(const GmmArgs &args, int tile_rows, bool swiglu, in
 }
 
 int launch_direct_bf16(const GmmArgs &args, int tile_rows, bool trans_b, bool swiglu, hipStream_t stream);
+int launch_direct_keep(const GmmArgs &args, int tile_rows, bool trans_b, hipStream_t stream);
 int launch_direct_fp8(const GmmArgs &args, int tile_rows, bool swiglu, hipStream_t stream);
 int launch_tile256_fp8(const GmmArgs &args, bool swiglu, hipStream_t stream);
 int launch_wave128(const GmmArgs &args, bool swiglu, hipStream_t stream);
 int launch_wave128_fp8(const GmmArgs &args, bool swiglu, hipStream_t stream);
 int launch_tile256_rows(const GmmArgs &args, hipStream_t stream);
 int launch_wgrad(const GmmArgs &args, hipStream_t stream);
-int launch_swiglu_backward(const void *dh, const void *u, void *du, const int64_t *batch_sizes, int64_t rows, int E, int64_t I,
+int launch_swiglu_backward(const void *dh, const float *u, void *du, const int64_t *batch_sizes, int64_t rows, int E, int64_t I,
                            void *da, int64_t K, hipStream_t stream);
-int launch_swiglu_forward(const void *u, void *h, const int64_t *batch_sizes, int64_t rows, int E, int64_t I, hipStream_t stream);
 
 }  // namespace dmoe

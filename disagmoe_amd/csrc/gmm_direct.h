@@ -79,7 +79,8 @@ constexpr int kStageB = kDN * kDK * 2;     // 16 KiB of B per stage
 // NP = 0: every wavefront copies its share of a stage and computes.  NP = 2: wavefronts NW and NW + 1 only copy
 // (and draw the work items), the first NW only compute: a copy that waits for room in the memory pipeline then holds
 // up no MFMA, which is what small tiles on weights streamed from HBM need.
-template <int kDM, int NW, int WM, bool TRANS_B, bool SWIGLU, bool FP8, int NP = 0>
+// KEEP (bf16, gated form): the fp32 sums also go to p.u, for the activation's gradient.
+template <int kDM, int NW, int WM, bool TRANS_B, bool SWIGLU, bool FP8, int NP = 0, bool KEEP = false>
 __global__ __launch_bounds__((NW + NP) * 64) __attribute__((amdgpu_waves_per_eu((NW + NP + 3) / 4, (NW + NP + 3) / 4)))
 void gmm_direct_kernel(const GmmArgs p) {
     constexpr int kStageK = FP8 ? 64 : kDK;               // k per stage: 64 bytes per row either way
@@ -98,6 +99,7 @@ void gmm_direct_kernel(const GmmArgs p) {
     constexpr int kStage = kStageA + kStageB;
     constexpr int kStages = kDM == 256 ? 4 : (kDM == 128 ? 5 : 6);
     constexpr int BNO = SWIGLU ? kDN / 2 : kDN;
+    static_assert(!KEEP || (SWIGLU && !FP8), "only the gated form has something to keep");
     static_assert(kDM == 64 || kDM == 128 || kDM == 256, "tile rows");
     static_assert((NW == 4 || NW == 8) && WM * WN == NW && CA >= 1 && FM >= 1 && FN >= 2 && NR <= NM, "wave layout");
     static_assert(NP == 0 || (NP == 2 && NW == 4 && !FP8), "copying wavefronts: two, beside four computing ones");
@@ -529,6 +531,16 @@ void gmm_direct_kernel(const GmmArgs p) {
                                 }
                             }
                             float v[4];
+                            if constexpr (KEEP) {
+                                const int col = col0 + kgrp * 4 + j * 32 + g * 8;
+                                if (row_ok && col < n_out) {
+                                    float *u = p.u + (long long)(cur_row0 + r) * p.N + col;
+                                    const f32x4 gate = {acc[i][j][g * 4], acc[i][j][g * 4 + 1], acc[i][j][g * 4 + 2], acc[i][j][g * 4 + 3]};
+                                    const f32x4 up = {acc[i][j + FN / 2][g * 4], acc[i][j + FN / 2][g * 4 + 1], acc[i][j + FN / 2][g * 4 + 2], acc[i][j + FN / 2][g * 4 + 3]};
+                                    *(f32x4 *)u = gate;
+                                    *(f32x4 *)(u + n_out) = up;
+                                }
+                            }
 #pragma unroll
                             for (int x = 0; x < 4; ++x) {
                                 if (SWIGLU) {
@@ -610,11 +622,11 @@ void gmm_direct_kernel(const GmmArgs p) {
     sched_finish(p.sched, drawer, draw, streams, total);
 }
 
-template <int kDM, int NW, int WM, bool TRANS_B, bool SWIGLU, bool FP8, int NP = 0>
+template <int kDM, int NW, int WM, bool TRANS_B, bool SWIGLU, bool FP8, int NP = 0, bool KEEP = false>
 static int launch_direct_one(const GmmArgs &args, hipStream_t stream) {
     constexpr int kStages = kDM == 256 ? 4 : (kDM == 128 ? 5 : 6);
     const size_t lds = (size_t)kStages * (kDM * kDK * 2 + kStageB);
-    auto kern = gmm_direct_kernel<kDM, NW, WM, TRANS_B, SWIGLU, FP8, NP>;
+    auto kern = gmm_direct_kernel<kDM, NW, WM, TRANS_B, SWIGLU, FP8, NP, KEEP>;
     static unsigned long long configured = 0;   // devices on which the kernel's LDS size has been raised
     DMOE_HIP(raise_dynamic_lds((const void *)kern, (int)lds, &configured));
     const long long grid = launch_grid(args, kDM, SWIGLU, FP8 ? 64 : kDK, true, device_cus());

@@ -30,7 +30,8 @@ namespace dmoe {
 // routed rows by expert needs no launch and no copy of the rows.  A tile's row numbers are fetched and waited for before
 // the epilogue of the tile before it, when nothing else of the wavefront is in flight: behind the epilogue the same
 // wait would also be one for the epilogue's stores.
-template <bool TRANS_B, bool SWIGLU, bool GATHER = false>
+// KEEP (gated form): the fp32 sums also go to p.u, for the activation's gradient.
+template <bool TRANS_B, bool SWIGLU, bool GATHER = false, bool KEEP = false>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void gmm_tile256_kernel(const GmmArgs p) {
     constexpr int kDM = 256, NW = 8, WN = 4;
@@ -45,6 +46,7 @@ void gmm_tile256_kernel(const GmmArgs p) {
     constexpr int kStage = kStageA + kStageB;
     constexpr int kStages = 4;
     constexpr int BNO = SWIGLU ? kDN / 2 : kDN;
+    static_assert(!KEEP || SWIGLU, "only the gated form has something to keep");
     static_assert(CA == 2 && CB == 2 && (kStages - 1) * kLoads <= 63, "copies per stage");
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ int s_tile_start[kMaxGroups + 1];
@@ -372,6 +374,16 @@ void gmm_tile256_kernel(const GmmArgs p) {
                 for (int ii = 0; ii < 2; ++ii) {
                     const int i = i2 * 2 + ii;
                     const int row = ii * 16 + l16;
+                    if constexpr (KEEP) {
+                        // 16 bytes per lane, 64 of a row; the fragment beside it fills the line
+                        const int r = wm * TM + i * 16 + l16;
+#pragma unroll
+                        for (int j = 0; j < FN; ++j) {
+                            const int col = col0 + (j % FNO) * 16 + g16 * 4;
+                            if (r < cur_rows_e && col < n_out)
+                                __builtin_nontemporal_store(acc[i][j], (f32x4 *)(p.u + (long long)(cur_row0 + r) * p.N + (j < FNO ? 0 : n_out) + col));
+                        }
+                    }
 #pragma unroll
                     for (int j = 0; j < FNO; ++j) {
                         float v[4];
@@ -421,10 +433,10 @@ void gmm_tile256_kernel(const GmmArgs p) {
     sched_finish(p.sched, drawer, draw, streams, total);
 }
 
-template <bool TRANS_B, bool SWIGLU, bool GATHER = false>
+template <bool TRANS_B, bool SWIGLU, bool GATHER = false, bool KEEP = false>
 static int launch_tile256_one(const GmmArgs &args, hipStream_t stream) {
     const size_t lds = (size_t)4 * (256 * kDK * 2 + kStageB);
-    auto kern = gmm_tile256_kernel<TRANS_B, SWIGLU, GATHER>;
+    auto kern = gmm_tile256_kernel<TRANS_B, SWIGLU, GATHER, KEEP>;
     static unsigned long long configured = 0;   // devices on which the kernel's LDS size has been raised
     DMOE_HIP(raise_dynamic_lds((const void *)kern, (int)lds, &configured));
     const long long grid = launch_grid(args, 256, SWIGLU, kDK, true, device_cus());

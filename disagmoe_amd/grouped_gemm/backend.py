@@ -241,7 +241,7 @@ def gmm_swiglu_keep(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor,
                     workspace: Optional[torch.Tensor] = None, arguments_ptr: Optional[int] = None,
                     host_batch_sizes: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """:func:`gmm_swiglu` for a step whose gradient will be asked for: ``(h [rows, I], u [rows, 2I])``
-    with ``u = gmm(a, b)`` in bf16.  Rows of ``h`` past ``sum(batch_sizes)`` are zero."""
+    with ``u = gmm(a, b)`` in fp32.  Rows of ``h`` past ``sum(batch_sizes)`` are zero."""
     device = _check_operands(a, b, torch.bfloat16)
     rows, K = a.shape
     E = b.shape[0]
@@ -249,7 +249,7 @@ def gmm_swiglu_keep(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor,
     assert (b.shape[2] if trans_b else b.shape[1]) == K, "contraction length mismatch"
     assert N2 % 2 == 0 and batch_sizes.numel() == E
     h = torch.empty((rows, N2 // 2), dtype=a.dtype, device=device)
-    u = torch.empty((rows, N2), dtype=a.dtype, device=device)
+    u = torch.empty((rows, N2), dtype=torch.float32, device=device)
     bs = _sizes_on_device(batch_sizes, device)
     with torch.cuda.device(device):
         _lib.call("dmoe_gmm_swiglu_keep", a.data_ptr(), b.data_ptr(), h.data_ptr(), u.data_ptr(), bs.data_ptr(), rows, E, K, N2 // 2,
@@ -269,9 +269,9 @@ def gmm_swiglu_backward(dh: torch.Tensor, u: torch.Tensor, a: torch.Tensor, b: t
     E, inter = b.shape[0], dh.shape[1]
     assert b.shape == ((E, 2 * inter, K) if trans_b else (E, K, 2 * inter)) and batch_sizes.numel() == E
     assert dh.shape == (rows, inter) and u.shape == (rows, 2 * inter), "dh is [rows, I], u is [rows, 2I]"
-    assert dh.dtype == torch.bfloat16 and u.dtype == torch.bfloat16 and dh.device == device and u.device == device
+    assert dh.dtype == torch.bfloat16 and u.dtype == torch.float32 and dh.device == device and u.device == device
     assert dh.is_contiguous() and u.is_contiguous()
-    du = torch.empty_like(u)
+    du = torch.empty((rows, 2 * inter), dtype=torch.bfloat16, device=device)
     da = torch.empty_like(a) if need_da else None
     db = torch.empty_like(b) if need_db else None
     bs = _sizes_on_device(batch_sizes, device)

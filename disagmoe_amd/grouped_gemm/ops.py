@@ -75,7 +75,7 @@ def gmm_swiglu(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor, tran
                workspace: Optional[torch.Tensor] = None, arguments_ptr: Optional[int] = None,
                host_batch_sizes: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Differentiable ``backend.gmm_swiglu``: ``silu(u[:, :I]) * u[:, I:]`` for ``u = gmm(a, b)``,
-    ``b [E, K, 2I]`` (``[E, 2I, K]`` with ``trans_b``).  Keeps ``u`` in bf16 (4 bytes per element of
+    ``b [E, K, 2I]`` (``[E, 2I, K]`` with ``trans_b``).  Keeps ``u`` in fp32 (8 bytes per element of
     the result) for the backward pass; without a gradient to come it is ``backend.gmm_swiglu``."""
     backend._check_operands(a, b, torch.bfloat16)
     sizes, host = _on_device(batch_sizes, host_batch_sizes, a.device)

@@ -288,7 +288,7 @@ int dmoe_gmm_swiglu_rows(const void *x, const int32_t *row_token, int64_t T, con
  *   the other trans_b.  state, workspace and host_batch_sizes as for dmoe_gmm.
  *
  * The gated block h = silu(g) p, [g | p] = u = a @ b[e], as one differentiable step:
- *   dmoe_gmm_swiglu_keep is dmoe_gmm_swiglu that also leaves u [rows, 2I] in bf16.
+ *   dmoe_gmm_swiglu_keep is dmoe_gmm_swiglu that also leaves u [rows, 2I] in fp32.
  *   dmoe_gmm_swiglu_backward takes that u and a gradient dh [rows, I] of h; with s = sigmoid(g)
  *     du[r, n] = dh p s (1 + g (1 - s)),  du[r, I + n] = dh g s          (fp32, one rounding)
  *   goes to du [rows, 2I] (the caller's, any contents), and from it, where they are not NULL,
@@ -299,11 +299,11 @@ int dmoe_gmm_swiglu_rows(const void *x, const int32_t *row_token, int64_t T, con
 int dmoe_gmm_wgrad(const void *a, const void *dc, void *db, const int64_t *batch_sizes, int64_t rows, int E,
                    int64_t K, int64_t N, int dtype, void *state, void *workspace, size_t workspace_bytes,
                    const int64_t *host_batch_sizes, void *stream);
-int dmoe_gmm_swiglu_keep(const void *a, const void *b, void *h, void *u, const int64_t *batch_sizes,
+int dmoe_gmm_swiglu_keep(const void *a, const void *b, void *h, float *u, const int64_t *batch_sizes,
                          int64_t rows, int E, int64_t K, int64_t I, int trans_b, int dtype,
                          void *state, void *workspace, size_t workspace_bytes,
                          const int64_t *host_batch_sizes, void *stream);
-int dmoe_gmm_swiglu_backward(const void *dh, const void *u, const void *a, const void *b, void *du, void *da, void *db,
+int dmoe_gmm_swiglu_backward(const void *dh, const float *u, const void *a, const void *b, void *du, void *da, void *db,
                              const int64_t *batch_sizes, int64_t rows, int E, int64_t K, int64_t I, int trans_b,
                              int dtype, void *state, void *workspace, size_t workspace_bytes,
                              const int64_t *host_batch_sizes, void *stream);

@@ -54,12 +54,12 @@ def _check_block(u, h, da, db, a, b, dh, sizes):
         x, w, d = a[at].double(), b[e].double(), dh[at].double()
         want_u = x @ w
         off_u = ACC * (x.shape[1] + 4) * (x.abs() @ w.abs())
-        _close(u[at], want_u, off_u, "u")
+        assert u.dtype == torch.float32 and bool(((u[at].double() - want_u).abs() <= off_u + 2.0 ** -24 * want_u.abs()).all())
         g, p = want_u[:, :I], want_u[:, I:]
         s = torch.sigmoid(g)
         slope = (p * s * (1 + g * (1 - s))).abs()
-        # (h may be taken from u before or after it is rounded; second-order terms: 1 % of the first-order ones)
-        off_h = 1.01 * (slope * (off_u + HALF * want_u.abs())[:, :I] + (g * s).abs() * (off_u + HALF * want_u.abs())[:, I:])
+        # (second-order terms: 1 % of the first-order ones)
+        off_h = 1.01 * (slope * off_u[:, :I] + (g * s).abs() * off_u[:, I:])
         _close(h[at], g * s * p, off_h + 1e-6 * (g * s * p).abs() + 2e-4 * HALF * p.abs(), "h")
         g, p = u[at].double()[:, :I], u[at].double()[:, I:]
         s = torch.sigmoid(g)
@@ -146,8 +146,7 @@ def test_gated_block(E, R, K, I, trans_b):
     assert torch.equal(torch.autograd.grad(y, w, dh)[0], db)
     with torch.no_grad():
         fused = ops.gmm_swiglu(x, w, sizes, trans_b=trans_b)
-    ok = (fused.double() - y.double()).abs() <= 4 * HALF * y.double().abs() + 0.02 * y.double().abs().max()
-    assert bool(ok.all()) and not fused.requires_grad
+    assert torch.equal(fused, y) and not fused.requires_grad     # the same sums, kept or not
 
 
 def test_gated_block_where_the_gate_saturates():
@@ -186,8 +185,8 @@ def test_gradient_against_differences():
     for g, dx, dw in ((da, va, 0 * vb), (db, 0 * va, vb)):
         v = dx if g is da else dw
         slope = (f(a.double() + t * dx, b.double() + t * dw) - f(a.double() - t * dx, b.double() - t * dw)) / (2 * t)
-        # every gradient element is off by at most 4 roundings (u twice: gate and up, du, itself) of the terms in its sum;
-        # as independent errors of the n elements they add like sqrt(n), 6 of their deviations are allowed
+        # every gradient element is off by at most 2 roundings (du, itself) of the terms in its sum; as independent errors of
+        # the n elements they add like sqrt(n), 6 of their deviations are allowed, and as much for the terms' spread
         off = 6 * 4 * HALF * float((g.double() * v).square().sum().sqrt()) + 6 * 4 * HALF * float(v.square().sum().sqrt() * g.double().square().mean().sqrt())
         assert abs(slope - float((g.double() * v).sum())) <= off, (slope, float((g.double() * v).sum()), off)
 
