@@ -381,7 +381,7 @@ void gmm_tile256_kernel(const GmmArgs p) {
                         for (int j = 0; j < FN; ++j) {
                             const int col = col0 + (j % FNO) * 16 + g16 * 4;
                             if (r < cur_rows_e && col < n_out)
-                                __builtin_nontemporal_store(acc[i][j], (f32x4 *)(p.u + (long long)(cur_row0 + r) * p.N + (j < FNO ? 0 : n_out) + col));
+                                *(f32x4 *)(p.u + (long long)(cur_row0 + r) * p.N + (j < FNO ? 0 : n_out) + col) = acc[i][j];
                         }
                     }
 #pragma unroll

@@ -42,9 +42,20 @@ struct W4Args {
     int m_tiles;                              // row tiles of the grid
 };
 
-__device__ __forceinline__ uint32_t w4_pair(uint32_t word, int p) {   // 16 + q of nibbles p and p + 4 as two bf16
+// 16 + q of nibbles p and p + 4 as two bf16.  The mask sits in a scalar and the 16s in a vector register: an instruction
+// with two literals does not exist, and with them the compiler takes two (`mask`, `bias`: w4_constants).
+__device__ __forceinline__ uint32_t w4_pair(uint32_t word, int p, uint32_t mask, uint32_t bias) {
     const uint32_t v = p == 0 ? word << 3 : word >> (4 * p - 3);
-    return (v & 0x00780078u) | 0x41804180u;
+    return (v & mask) | bias;
+}
+struct W4Constants {
+    uint32_t mask, bias;
+};
+__device__ __forceinline__ W4Constants w4_constants() {
+    W4Constants k;
+    asm("s_mov_b32 %0, 0x00780078" : "=s"(k.mask));
+    asm("v_mov_b32 %0, 0x41804180" : "=v"(k.bias));
+    return k;
 }
 
 // Row tile number `m` of all experts' row tiles of BM rows: its expert, first row and rows, and how many row tiles there are
@@ -108,19 +119,25 @@ struct W4Source {
         scale_at[f] = p.scales + tile * (kScaleTile * 2);
         zero_at[f] = ZERO ? p.zeros + tile * kScaleTile : nullptr;
     }
+    __device__ __forceinline__ void load_codes(W4Weights<NF, NG, ZERO> &b, int f, int c, int lane) const {
+        b.q[f] = *(const u32x4 *)(code_at[f] + ((uint32_t)c * kW4TileBytes + lane * 16));
+    }
+    __device__ __forceinline__ void load_scales(W4Weights<NF, NG, ZERO> &b, int f, int c, int lane) const {
+        __builtin_memcpy(b.s[f], scale_at[f] + ((uint32_t)c * (kScaleTile * 2) + (lane >> 4) * (NG * 8)), NG * 8);
+        if constexpr (ZERO) __builtin_memcpy(b.z[f], zero_at[f] + ((uint32_t)c * kScaleTile + (lane >> 4) * (NG * 4)), NG * 4);
+    }
     __device__ __forceinline__ void load(W4Weights<NF, NG, ZERO> &b, int c, int lane) const {
 #pragma unroll
         for (int f = 0; f < NF; ++f) {
-            b.q[f] = *(const u32x4 *)(code_at[f] + ((uint32_t)c * kW4TileBytes + lane * 16));
-            __builtin_memcpy(b.s[f], scale_at[f] + ((uint32_t)c * (kScaleTile * 2) + (lane >> 4) * (NG * 8)), NG * 8);
-            if constexpr (ZERO) __builtin_memcpy(b.z[f], zero_at[f] + ((uint32_t)c * kScaleTile + (lane >> 4) * (NG * 4)), NG * 4);
+            load_codes(b, f, c, lane);
+            load_scales(b, f, c, lane);
         }
     }
 };
 
 // acc[f][i] += the products of a chunk's weights with the row fragments x(i, j) of its k-steps j
 template <int FM, int NF, int NG, bool ZERO, typename X>
-__device__ __forceinline__ void w4_chunk(f32x4 (&acc)[NF][FM], const W4Weights<NF, NG, ZERO> &b, X &&x_of) {
+__device__ __forceinline__ void w4_chunk(f32x4 (&acc)[NF][FM], const W4Weights<NF, NG, ZERO> &b, const W4Constants &k, X &&x_of) {
     constexpr int SG = 4 / NG;                                // k-steps of a group
     const uint32_t less = ZERO ? 0xc180c180u : 0xc1c0c1c0u;   // -16 or -24 as two bf16
     const u32x4 less4 = {less, less, less, less};
@@ -140,6 +157,9 @@ __device__ __forceinline__ void w4_chunk(f32x4 (&acc)[NF][FM], const W4Weights<N
         for (int j = g * SG; j < (g + 1) * SG; ++j)
 #pragma unroll
             for (int i = 0; i < FM; ++i) base[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lf, x[i][j - g * SG], base[i], 0, 0, 0);
+        float less_x[FM];                                     // (ZERO) minus that sum
+#pragma unroll
+        for (int i = 0; i < FM; ++i) less_x[i] = ZERO ? base[i][0] * 0.0625f : 0.f;
 #pragma unroll
         for (int f = 0; f < NF; ++f) {
             f32x4 t[FM];
@@ -147,7 +167,7 @@ __device__ __forceinline__ void w4_chunk(f32x4 (&acc)[NF][FM], const W4Weights<N
             for (int j = g * SG; j < (g + 1) * SG; ++j) {
                 u32x4 w;
 #pragma unroll
-                for (int q = 0; q < 4; ++q) w[q] = w4_pair(b.q[f][j], q);
+                for (int q = 0; q < 4; ++q) w[q] = w4_pair(b.q[f][j], q, k.mask, k.bias);
                 bf16x8 wf;
                 __builtin_memcpy(&wf, &w, 16);
 #pragma unroll
@@ -157,13 +177,102 @@ __device__ __forceinline__ void w4_chunk(f32x4 (&acc)[NF][FM], const W4Weights<N
             for (int v = 0; v < 4; ++v) {
                 const uint32_t pair = b.s[f][g * 2 + v / 2];
                 const float s = __uint_as_float(v & 1 ? pair & 0xffff0000u : pair << 16);
-                const float zs = ZERO ? (float)((b.z[ZERO ? f : 0][g] >> (8 * v)) & 0xffu) * 0.0625f : 0.f;   // z / 16, exactly
+                const float z = ZERO ? (float)((b.z[ZERO ? f : 0][g] >> (8 * v)) & 0xffu) : 0.f;
 #pragma unroll
-                for (int i = 0; i < FM; ++i) acc[f][i][v] = fmaf(s, ZERO ? fmaf(zs, base[i][v], t[i][v]) : t[i][v], acc[f][i][v]);
+                for (int i = 0; i < FM; ++i) acc[f][i][v] = fmaf(s, ZERO ? fmaf(z, less_x[i], t[i][v]) : t[i][v], acc[f][i][v]);
             }
             __builtin_amdgcn_sched_barrier(0);                // one fragment's sums in registers at a time
         }
     }
+}
+
+// The same for 64 rows, as one pipeline: a matrix instruction occupies its unit for 16 cycles and a vector instruction its
+// own for 4, so behind each of the former stand the vector instructions that prepare and finish its neighbours: a quarter
+// of the next operand's unpacking, a share of the fold of the fragment before.  A fragment's codes and scales of chunk
+// `c_next` are loaded over those of this chunk once they have been used.
+template <int NF, int NG, bool ZERO, typename X>
+__device__ __forceinline__ void w4_chunk_64(f32x4 (&acc)[NF][4], W4Weights<NF, NG, ZERO> &b, const W4Source<NF, NG, ZERO> &src, int c_next,
+                                            int lane, const W4Constants &k, X &&x_of) {
+    constexpr int FM = 4;
+    constexpr int SG = 4 / NG;                                // k-steps of a group
+    constexpr int XB = NG == 1 || ZERO ? 1 : 2;               // groups of x held; the zero points' registers leave room for one
+    const uint32_t less = ZERO ? 0xc180c180u : 0xc1c0c1c0u;   // -16 or -24 as two bf16
+    const u32x4 less4 = {less, less, less, less};
+    bf16x8 lf;
+    __builtin_memcpy(&lf, &less4, 16);
+    bf16x8 x[XB][SG][FM];
+    auto read_x = [&](int g) {
+#pragma unroll
+        for (int j = 0; j < SG; ++j)
+#pragma unroll
+            for (int i = 0; i < FM; ++i) x[g % XB][j][i] = x_of(i, g * SG + j);
+    };
+#pragma unroll
+    for (int g = 0; g < XB; ++g) read_x(g);
+    u32x4 w;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) w[q] = w4_pair(b.q[0][0], q, k.mask, k.bias);
+    f32x4 t[2][FM], base[FM];
+    float less_x[2][FM];                                      // (ZERO) minus the group's sum of x; the group before is still read
+    // element v of row fragment i of the sums of (group, fragment) number n
+    auto fold = [&](int n, int i, int v) {
+        const int g = n / NF, f = n % NF;
+        const uint32_t pair = b.s[f][g * 2 + v / 2];
+        const float s = __uint_as_float(v & 1 ? pair & 0xffff0000u : pair << 16);
+        const float z = ZERO ? (float)((b.z[ZERO ? f : 0][g] >> (8 * v)) & 0xffu) : 0.f;
+        acc[f][i][v] = fmaf(s, ZERO ? fmaf(z, less_x[g & 1][i], t[n & 1][i][v]) : t[n & 1][i][v], acc[f][i][v]);
+    };
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+#pragma unroll
+        for (int j = 0; j < SG; ++j)
+#pragma unroll
+            for (int i = 0; i < FM; ++i)                      // -24 (-16) times the group's sum of x in this lane's row
+                base[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lf, x[g % XB][j][i], j == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : base[i], 0, 0, 0);
+        if constexpr (ZERO) {
+#pragma unroll
+            for (int i = 0; i < FM; ++i) less_x[g & 1][i] = base[i][0] * 0.0625f;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            const int n = g * NF + f;
+#pragma unroll
+            for (int j = 0; j < SG; ++j) {
+                // the operand behind this one
+                const int fn = j + 1 < SG ? f : (f + 1 < NF ? f + 1 : 0), jn = j + 1 < SG ? g * SG + j + 1 : (f + 1 < NF ? g * SG : (g + 1) * SG);
+                const bool more = jn < 4;
+                bf16x8 wf;
+                __builtin_memcpy(&wf, &w, 16);
+                u32x4 wn = w;
+#pragma unroll
+                for (int i = 0; i < FM; ++i) {
+                    t[n & 1][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, x[g % XB][j][i], j == 0 ? base[i] : t[n & 1][i], 0, 0, 0);
+                    if (more) wn[i] = w4_pair(b.q[fn][jn], i, k.mask, k.bias);
+                    if (n > 0) {
+                        constexpr int kShare = 4 / SG;        // of the 16 elements, over SG * 4 instructions
+#pragma unroll
+                        for (int u = 0; u < kShare; ++u) {
+                            const int at = (j * FM + i) * kShare + u;
+                            fold(n - 1, at % FM, at / FM);
+                        }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                w = wn;
+            }
+            if (g == NG - 1) {
+                src.load_codes(b, f, c_next, lane);
+                if (f > 0) src.load_scales(b, f - 1, c_next, lane);
+            }
+        }
+        if (g + XB < NG) read_x(g + XB);
+    }
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+#pragma unroll
+        for (int i = 0; i < FM; ++i) fold(NG * NF - 1, i, v);
+    src.load_scales(b, NF - 1, c_next, lane);
 }
 
 // The wavefronts that split k meet: red[wk][wn][fragment][row][16 columns].  Sums in the order of the wavefronts, the
@@ -204,13 +313,16 @@ __device__ __forceinline__ void w4_finish(const W4Args &p, float *red, const f32
     __syncthreads();                                          // read: the LDS may be written again
 }
 
+// Wavefronts to a SIMD: as many as the registers of the form allow without spills.
+constexpr int w4_waves(int FM) { return FM == 1 ? 4 : (FM == 2 ? 3 : 2); }
+
 // FM row fragments of 16, FG column fragments of 16 per wavefront (SWIGLU: of the result, with as many of the gate and of
 // the up columns; SHIFT: the up columns begin in the middle of a tile, one more), WN wavefronts along the columns, WK
 // along k.  Up to 32 rows (FM 1, 2): the rows come straight from the caches into registers and four (three)
 // wavefronts to a SIMD keep loads in flight.  64 rows (FM 4): the sums leave room for two, so weights and rows are fetched a
 // round ahead, and all wavefronts bring the WK chunks of a round into LDS, once for the WN wavefronts that read each.
 template <int FM, int FG, int WN, int WK, int G, bool ZERO, bool SWIGLU, bool SHIFT>
-__global__ __launch_bounds__(WN *WK *kWave) __attribute__((amdgpu_waves_per_eu(FM == 1 ? 4 : (FM == 2 ? 3 : 2))))
+__global__ __launch_bounds__(WN *WK *kWave) __attribute__((amdgpu_waves_per_eu(w4_waves(FM))))
 void gmm_w4_kernel(const W4Args p) {
     constexpr int BM = 16 * FM;
     constexpr int NF = SWIGLU ? 2 * FG + (SHIFT ? 1 : 0) : FG;
@@ -224,6 +336,7 @@ void gmm_w4_kernel(const W4Args p) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int wn = wave % WN, wk = wave / WN;
     const int l16 = lane & 15, g16 = lane >> 4;
+    const W4Constants consts = w4_constants();
 
     // workgroup -> (column tile, row tile): the row tiles of a column tile one after the other on one XCD, whose L2 then
     // holds the column tile's codes
@@ -270,7 +383,7 @@ void gmm_w4_kernel(const W4Args p) {
                         __builtin_memcpy(&x[i][j], &v, 16);
                     }
                 __builtin_amdgcn_sched_barrier(0);            // every load of the chunk is on its way
-                w4_chunk<FM>(acc, b, [&](int i, int j) { return x[i][j]; });
+                w4_chunk<FM>(acc, b, consts, [&](int i, int j) { return x[i][j]; });
             }
         } else {
             // A round brings WK chunks of BM rows x 256 bytes, kept in LDS with the 16-byte piece q of row r at q ^ (r & 15):
@@ -278,50 +391,51 @@ void gmm_w4_kernel(const W4Args p) {
             constexpr int kRound = WK * BM * 256;
             constexpr int kPieces = kRound / 16 / (WN * WK * kWave);   // of a thread
             static_assert(kPieces * 16 * WN * WK * kWave == kRound, "whole pieces");
+            constexpr int kPass = WN * WK * kWave / 16;       // rows that the threads bring at a time, 16 threads each
+            static_assert(BM % kPass == 0, "a piece's row is the same in every chunk of the round");
+            const int r16 = threadIdx.x / 16, q16 = threadIdx.x % 16;
+            const char *x_tile = p.x + (size_t)row0 * p.K * 2;
+            uint32_t x_off[BM / kPass];                       // of this thread's rows in the tile; past the end: the last row
+#pragma unroll
+            for (int u = 0; u < BM / kPass; ++u) {
+                const int m = r16 + u * kPass;
+                x_off[u] = (uint32_t)(m < rows ? m : rows - 1) * (uint32_t)p.K * 2 + q16 * 16;
+            }
             u32x4 px[kPieces];
             auto load_x = [&](int c) {
 #pragma unroll
                 for (int u = 0; u < kPieces; ++u) {
-                    const int i = threadIdx.x + u * (WN * WK * kWave);
-                    const int m = (i / 16) % BM, k = (c + i / (16 * BM)) * kW4Chunk + (i % 16) * 8;
+                    const int ch = c + u / (BM / kPass);
                     px[u] = u32x4{0, 0, 0, 0};
-                    if (k < p.K) px[u] = *(const u32x4 *)(p.x + ((size_t)(row0 + (m < rows ? m : rows - 1)) * p.K + k) * 2);
+                    if (ch * kW4Chunk + q16 * 8 < p.K) px[u] = *(const u32x4 *)(x_tile + (x_off[u % (BM / kPass)] + (uint32_t)ch * (kW4Chunk * 2)));
                 }
             };
+            char *const x_to = smem + r16 * 256 + ((q16 ^ (r16 & 15)) << 4);   // rows kPass apart share the place in a row
             auto store_x = [&](int buf) {
 #pragma unroll
-                for (int u = 0; u < kPieces; ++u) {
-                    const int i = threadIdx.x + u * (WN * WK * kWave);
-                    const int r = i / 16;                     // row of the round: chunk * BM + row
-                    *(u32x4 *)(smem + buf * kRound + r * 256 + (((i % 16) ^ (r & 15)) << 4)) = px[u];
-                }
+                for (int u = 0; u < kPieces; ++u) *(u32x4 *)(x_to + buf * kRound + u * (kPass * 256)) = px[u];
             };
-            W4Weights<NF, NG, ZERO> now, next;
+            W4Weights<NF, NG, ZERO> b;
             load_x(0);
-            if (wk < p.kt) src.load(now, wk, lane);
+            src.load(b, wk < p.kt ? wk : p.kt - 1, lane);
             store_x(0);
             __syncthreads();
             int buf = 0;
             for (int c = 0; c < p.kt; c += WK, buf ^= 1) {    // the same rounds for every wavefront: they share the barriers
                 const bool more = c + WK < p.kt;
-                if (more) {
-                    load_x(c + WK);
-                    if (c + WK + wk < p.kt) src.load(next, c + WK + wk, lane);
-                }
+                if (more) load_x(c + WK);
                 __builtin_amdgcn_sched_barrier(0);
                 if (c + wk < p.kt) {
                     const char *round = smem + buf * kRound + (wk * BM + l16) * 256;
-                    w4_chunk<FM>(acc, now, [&](int i, int j) {
+                    const int c_next = c + WK + wk < p.kt ? c + WK + wk : p.kt - 1;   // (behind the last one: loaded, not used)
+                    w4_chunk_64(acc, b, src, c_next, lane, consts, [&](int i, int j) {
                         const u32x4 v = *(const u32x4 *)(round + i * (16 * 256) + (((j * 4 + g16) ^ l16) << 4));
                         bf16x8 x;
                         __builtin_memcpy(&x, &v, 16);
                         return x;
                     });
                 }
-                if (more) {
-                    store_x(buf ^ 1);
-                    now = next;
-                }
+                if (more) store_x(buf ^ 1);
                 __syncthreads();
             }
         }
