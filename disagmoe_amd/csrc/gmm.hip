@@ -415,13 +415,6 @@ static int launch_one(const GmmArgs &args, hipStream_t stream) {
 
 static int g_variant = 0;  // tuning hook, see dmoe_gmm_tune
 thread_local const int64_t *t_host_sizes = nullptr;
-namespace {
-// the host copy of the sizes for the length of one call
-struct HostSizes {
-    explicit HostSizes(const int64_t *p) { t_host_sizes = p; }
-    ~HostSizes() { t_host_sizes = nullptr; }
-};
-}  // namespace
 
 // ---- where a launch keeps its counters ----------------------------------------------------------------
 // With a state block of the caller: there, the split tiles' arrival counters behind them, and the partial sums in
@@ -473,7 +466,7 @@ static int own_slot(hipStream_t stream, SchedSlot **out) {
     return DMOE_OK;
 }
 
-static int bind_state(GmmArgs &args, void *state, void *workspace, size_t workspace_bytes, hipStream_t stream) {
+int bind_state(GmmArgs &args, void *state, void *workspace, size_t workspace_bytes, hipStream_t stream) {
     args.arrive = nullptr; args.partials = nullptr; args.partial_bytes = 0;
     args.a_rows = nullptr; args.a_src_rows = 0; args.u = nullptr;
     if (state == nullptr) return own_slot(stream, &args.sched);

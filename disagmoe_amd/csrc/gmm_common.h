@@ -9,6 +9,7 @@
 namespace dmoe {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -370,6 +371,13 @@ int launch_wave128(const GmmArgs &args, bool swiglu, hipStream_t stream);
 int launch_wave128_fp8(const GmmArgs &args, bool swiglu, hipStream_t stream);
 int launch_tile256_rows(const GmmArgs &args, hipStream_t stream);
 int launch_wgrad(const GmmArgs &args, hipStream_t stream);
+int launch_tile256_half(const GmmArgs &args, bool swiglu, hipStream_t stream);
+int bind_state(GmmArgs &args, void *state, void *workspace, size_t workspace_bytes, hipStream_t stream);
+// The caller's copy of the sizes on the host for the length of one call.
+struct HostSizes {
+    explicit HostSizes(const int64_t *p) { t_host_sizes = p; }
+    ~HostSizes() { t_host_sizes = nullptr; }
+};
 int launch_swiglu_backward(const void *dh, const float *u, void *du, const int64_t *batch_sizes, int64_t rows, int E, int64_t I,
                            void *da, int64_t K, hipStream_t stream);
 

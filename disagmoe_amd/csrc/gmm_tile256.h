@@ -31,7 +31,8 @@ namespace dmoe {
 // the epilogue of the tile before it, when nothing else of the wavefront is in flight: behind the epilogue the same
 // wait would also be one for the epilogue's stores.
 // KEEP (gated form): the fp32 sums also go to p.u, for the activation's gradient.
-template <bool TRANS_B, bool SWIGLU, bool GATHER = false, bool KEEP = false>
+// HALF (trans_b): fp16 operands whose rows and columns carry fp32 scales, c = (a @ b[e]^T) a_scale[r] b_scale[e, n] in bf16.
+template <bool TRANS_B, bool SWIGLU, bool GATHER = false, bool KEEP = false, bool HALF = false>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void gmm_tile256_kernel(const GmmArgs p) {
     constexpr int kDM = 256, NW = 8, WN = 4;
@@ -47,6 +48,7 @@ void gmm_tile256_kernel(const GmmArgs p) {
     constexpr int kStages = 4;
     constexpr int BNO = SWIGLU ? kDN / 2 : kDN;
     static_assert(!KEEP || SWIGLU, "only the gated form has something to keep");
+    static_assert(!HALF || (TRANS_B && !KEEP && !GATHER), "fp16 operands are K-contiguous");
     static_assert(CA == 2 && CB == 2 && (kStages - 1) * kLoads <= 63, "copies per stage");
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ int s_tile_start[kMaxGroups + 1];
@@ -266,6 +268,7 @@ void gmm_tile256_kernel(const GmmArgs p) {
         WorkItem next_item{};                              // GATHER: the next item, located before this one's epilogue
         const int cur_row0 = row0, cur_rows_e = rows_e, cur_n0 = n0;
         const int cur_part = part, cur_split_tile = split_tile, cur_S = S;
+        const int cur_e = e;
         // 16-row fragments of this wavefront that hold at least one valid row (a short last tile skips the rest)
         int nfr = ((rows_e < kDM ? rows_e : kDM) - wm * TM + 15) / 16;
         nfr = __builtin_amdgcn_readfirstlane(nfr < 0 ? 0 : (nfr > FM ? FM : nfr));
@@ -318,7 +321,10 @@ void gmm_tile256_kernel(const GmmArgs p) {
 #pragma unroll
                     for (int jj = 0; jj < FN; ++jj) {
                         const int j = (i & 1) ? FN - 1 - jj : jj;
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j], fa[i], acc[i][j], 0, 0, 0);
+                        if constexpr (HALF)
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, fb[j]), __builtin_bit_cast(f16x8, fa[i]), acc[i][j], 0, 0, 0);
+                        else
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j], fa[i], acc[i][j], 0, 0, 0);
                     }
                 });
                 __builtin_amdgcn_s_setprio(0);
@@ -384,6 +390,17 @@ void gmm_tile256_kernel(const GmmArgs p) {
                                 *(f32x4 *)(p.u + (long long)(cur_row0 + r) * p.N + (j < FNO ? 0 : n_out) + col) = acc[i][j];
                         }
                     }
+                    if constexpr (HALF) {
+                        // rows and columns outside the tile read a valid neighbour's scale; their results are never stored
+                        const int r = wm * TM + i * 16 + l16;
+                        const float sa = p.a_scale[cur_row0 + (r < cur_rows_e ? r : 0)];
+#pragma unroll
+                        for (int j = 0; j < FN; ++j) {
+                            const int col = col0 + (j % FNO) * 16 + g16 * 4;
+                            const f32x4 sb = *(const f32x4 *)(p.b_scale + (long long)cur_e * p.N + (j < FNO ? 0 : n_out) + (col < n_out ? col : cur_n0));
+                            acc[i][j] *= sb * sa;
+                        }
+                    }
 #pragma unroll
                     for (int j = 0; j < FNO; ++j) {
                         float v[4];
@@ -433,10 +450,10 @@ void gmm_tile256_kernel(const GmmArgs p) {
     sched_finish(p.sched, drawer, draw, streams, total);
 }
 
-template <bool TRANS_B, bool SWIGLU, bool GATHER = false, bool KEEP = false>
+template <bool TRANS_B, bool SWIGLU, bool GATHER = false, bool KEEP = false, bool HALF = false>
 static int launch_tile256_one(const GmmArgs &args, hipStream_t stream) {
     const size_t lds = (size_t)4 * (256 * kDK * 2 + kStageB);
-    auto kern = gmm_tile256_kernel<TRANS_B, SWIGLU, GATHER, KEEP>;
+    auto kern = gmm_tile256_kernel<TRANS_B, SWIGLU, GATHER, KEEP, HALF>;
     static unsigned long long configured = 0;   // devices on which the kernel's LDS size has been raised
     DMOE_HIP(raise_dynamic_lds((const void *)kern, (int)lds, &configured));
     const long long grid = launch_grid(args, 256, SWIGLU, kDK, true, device_cus());

@@ -186,14 +186,13 @@ __device__ __forceinline__ void w4_chunk(f32x4 (&acc)[NF][FM], const W4Weights<N
     }
 }
 
-// The same for 64 rows, as one pipeline: a matrix instruction occupies its unit for 16 cycles and a vector instruction its
+// The same for tiles of 64 rows of which the first FM * 16 are there, as one pipeline: a matrix instruction occupies its unit for 16 cycles and a vector instruction its
 // own for 4, so behind each of the former stand the vector instructions that prepare and finish its neighbours: a quarter
 // of the next operand's unpacking, a share of the fold of the fragment before.  A fragment's codes and scales of chunk
 // `c_next` are loaded over those of this chunk once they have been used.
-template <int NF, int NG, bool ZERO, typename X>
+template <int FM, int NF, int NG, bool ZERO, typename X>
 __device__ __forceinline__ void w4_chunk_64(f32x4 (&acc)[NF][4], W4Weights<NF, NG, ZERO> &b, const W4Source<NF, NG, ZERO> &src, int c_next,
                                             int lane, const W4Constants &k, X &&x_of) {
-    constexpr int FM = 4;
     constexpr int SG = 4 / NG;                                // k-steps of a group
     constexpr int XB = NG == 1 || ZERO ? 1 : 2;               // groups of x held; the zero points' registers leave room for one
     const uint32_t less = ZERO ? 0xc180c180u : 0xc1c0c1c0u;   // -16 or -24 as two bf16
@@ -248,9 +247,12 @@ __device__ __forceinline__ void w4_chunk_64(f32x4 (&acc)[NF][4], W4Weights<NF, N
 #pragma unroll
                 for (int i = 0; i < FM; ++i) {
                     t[n & 1][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, x[g % XB][j][i], j == 0 ? base[i] : t[n & 1][i], 0, 0, 0);
-                    if (more) wn[i] = w4_pair(b.q[fn][jn], i, k.mask, k.bias);
+                    if (more) {
+#pragma unroll
+                        for (int q = 4 * i / FM; q < 4 * (i + 1) / FM; ++q) wn[q] = w4_pair(b.q[fn][jn], q, k.mask, k.bias);
+                    }
                     if (n > 0) {
-                        constexpr int kShare = 4 / SG;        // of the 16 elements, over SG * 4 instructions
+                        constexpr int kShare = 4 / SG;        // of the 4 FM elements, over SG FM instructions
 #pragma unroll
                         for (int u = 0; u < kShare; ++u) {
                             const int at = (j * FM + i) * kShare + u;
@@ -415,29 +417,36 @@ void gmm_w4_kernel(const W4Args p) {
 #pragma unroll
                 for (int u = 0; u < kPieces; ++u) *(u32x4 *)(x_to + buf * kRound + u * (kPass * 256)) = px[u];
             };
-            W4Weights<NF, NG, ZERO> b;
-            load_x(0);
-            src.load(b, wk < p.kt ? wk : p.kt - 1, lane);
-            store_x(0);
-            __syncthreads();
-            int buf = 0;
-            for (int c = 0; c < p.kt; c += WK, buf ^= 1) {    // the same rounds for every wavefront: they share the barriers
-                const bool more = c + WK < p.kt;
-                if (more) load_x(c + WK);
-                __builtin_amdgcn_sched_barrier(0);
-                if (c + wk < p.kt) {
-                    const char *round = smem + buf * kRound + (wk * BM + l16) * 256;
-                    const int c_next = c + WK + wk < p.kt ? c + WK + wk : p.kt - 1;   // (behind the last one: loaded, not used)
-                    w4_chunk_64(acc, b, src, c_next, lane, consts, [&](int i, int j) {
-                        const u32x4 v = *(const u32x4 *)(round + i * (16 * 256) + (((j * 4 + g16) ^ l16) << 4));
-                        bf16x8 x;
-                        __builtin_memcpy(&x, &v, 16);
-                        return x;
-                    });
-                }
-                if (more) store_x(buf ^ 1);
+            auto rounds = [&](auto fm_tag) {                  // with the row fragments that hold a row
+                constexpr int kFrags = decltype(fm_tag)::value;
+                W4Weights<NF, NG, ZERO> b;
+                load_x(0);
+                src.load(b, wk < p.kt ? wk : p.kt - 1, lane);
+                store_x(0);
                 __syncthreads();
-            }
+                int buf = 0;
+                for (int c = 0; c < p.kt; c += WK, buf ^= 1) {   // the same rounds for every wavefront: they share the barriers
+                    const bool more = c + WK < p.kt;
+                    if (more) load_x(c + WK);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (c + wk < p.kt) {
+                        const char *round = smem + buf * kRound + (wk * BM + l16) * 256;
+                        const int c_next = c + WK + wk < p.kt ? c + WK + wk : p.kt - 1;   // (behind the last one: loaded, not used)
+                        w4_chunk_64<kFrags>(acc, b, src, c_next, lane, consts, [&](int i, int j) {
+                            const u32x4 v = *(const u32x4 *)(round + i * (16 * 256) + (((j * 4 + g16) ^ l16) << 4));
+                            bf16x8 x;
+                            __builtin_memcpy(&x, &v, 16);
+                            return x;
+                        });
+                    }
+                    if (more) store_x(buf ^ 1);
+                    __syncthreads();
+                }
+            };
+            if (rows > 48) rounds(std::integral_constant<int, 4>{});
+            else if (rows > 32) rounds(std::integral_constant<int, 3>{});
+            else if (rows > 16) rounds(std::integral_constant<int, 2>{});
+            else rounds(std::integral_constant<int, 1>{});
         }
         w4_finish<FM, FG, WN, WK, SWIGLU, SHIFT, NF>(p, (float *)smem, acc, wk, wn, row0, rows, n0);
     }
@@ -464,7 +473,7 @@ template <int FM, int FG, int WN, int WK, int G, bool ZERO>
 static int launch_w4_form(const W4Args &args, bool swiglu, hipStream_t stream) {
     if (!swiglu) return launch_w4_one<FM, 2 * FG, WN, WK, G, ZERO, false, false>(args, stream);
     if (args.n_out % 16 == 0) return launch_w4_one<FM, FG, WN, WK, G, ZERO, true, false>(args, stream);
-    return launch_w4_one<FM, FG / 2, WN, WK, G, ZERO, true, true>(args, stream);
+    return launch_w4_one<FM, (FG > 1 ? FG / 2 : 1), WN, WK, G, ZERO, true, true>(args, stream);
 }
 
 template <int FM, int FG, int WN, int WK>

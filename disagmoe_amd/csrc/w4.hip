@@ -73,33 +73,111 @@ __global__ __launch_bounds__(kWave) void w4_quant_kernel(const uint16_t *__restr
     *(u32x4 *)(codes + tile * kW4TileBytes + lane * 16) = u32x4{words[0], words[1], words[2], words[3]};
 }
 
-// out [E, N, K] = (q - z) s, rounded once to bf16; a wavefront takes tiles of one run of columns.  Only the experts that
-// have rows, if batch_sizes is given.
-__global__ __launch_bounds__(256) void w4_dequant_kernel(const char *__restrict__ codes, const char *__restrict__ scales, const char *__restrict__ zeros,
-                                                        uint16_t *__restrict__ out, const int64_t *__restrict__ batch_sizes, int K, int N,
-                                                        int nt, int kt, int group) {
-    const int lane = lane_id(), r = lane & 15, g16 = lane >> 4;
-    const int e = blockIdx.z;
+// The weights of a tile, 16 columns x 128 k, as 16-bit values: a wavefront unpacks them in their lanes' order, passes them
+// through 4 KiB of LDS of its own and writes whole lines of [E, N, K], 4 columns of 256 bytes an instruction.  Only the
+// experts that have rows, if batch_sizes is given.  Bound by the 2 bytes written per weight.
+//   HALF false: out = bf16((q - z) s), rounded once.
+//   HALF true:  out = fp16((q - z) s / f), col_scale[e, n] = f, the power of two below the column's largest scale: the values
+//               are rounded to 11 bits where the 8 of bf16 would show in the product (relative error of the gated form
+//               2.5e-3 instead of 1.7e-3, the rounding of its results alone), and f keeps them in fp16's range.
+template <bool HALF>
+__global__ __launch_bounds__(256) void w4_widen_kernel(const char *__restrict__ codes, const uint16_t *__restrict__ scales, const uint8_t *__restrict__ zeros,
+                                                      uint16_t *__restrict__ out, float *__restrict__ col_scale, const int64_t *__restrict__ batch_sizes,
+                                                      int K, int N, int nt, int kt, int group) {
+    __shared__ __attribute__((aligned(16))) char stage[4][4096];
+    __shared__ uint16_t largest[kW4Cols][16];
+    const int lane = lane_id(), r = lane & 15, g16 = lane >> 4, wave = threadIdx.x / kWave;
+    const int e = blockIdx.y, t = blockIdx.x;
     if (batch_sizes != nullptr && batch_sizes[e] <= 0) return;
-    const int c = blockIdx.x * 4 + threadIdx.x / kWave, t = blockIdx.y;
-    const int n = t * kW4Cols + r;
-    if (c >= kt || n >= N) return;
-    const int64_t tile = ((int64_t)e * nt + t) * kt + c;
-    const u32x4 q = *(const u32x4 *)(codes + tile * kW4TileBytes + lane * 16);
     const int ng = kW4Chunk / group;
-    uint16_t *row = out + ((int64_t)e * N + n) * K;
+    const int64_t first = ((int64_t)e * nt + t) * kt;          // tile (t, 0) of the expert
+    float inv = 1.f;
+    if constexpr (HALF) {
+        // the column's largest scale, as bf16 bits (scales are not negative): 16 threads a column
+        const int col = threadIdx.x / 16;
+        uint32_t most = 0;
+        for (int i = threadIdx.x % 16; i < kt * ng; i += 16) {
+            const uint32_t s = scales[(first + i / ng) * (kW4Cols * ng) + (col >> 2) * (ng * 4) + (i % ng) * 4 + (col & 3)] & 0x7fffu;
+            most = s > most ? s : most;
+        }
+        largest[col][threadIdx.x % 16] = (uint16_t)most;
+        __syncthreads();
+        uint32_t top = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int k = c * kW4Chunk + j * 32 + g16 * 8;
-        if (k >= K) continue;
-        const int64_t at = tile * (kW4Cols * ng) + (r >> 2) * (ng * 4) + (j * 32 / group) * 4 + (r & 3);
-        const float s = bf16_to_f32(((const uint16_t *)scales)[at]);
-        const float z = zeros != nullptr ? (float)((const uint8_t *)zeros)[at] : 8.f;
-        u32x4 v;
+        for (int i = 0; i < 16; ++i) top = largest[r][i] > top ? largest[r][i] : top;
+        int exponent = (int)(top >> 7);
+        exponent = exponent < 1 ? 127 : (exponent > 253 ? 253 : exponent);   // all zero: 1; infinite: whatever, it stays so
+        inv = __uint_as_float((uint32_t)(254 - exponent) << 23);
+        if (wave == 0 && g16 == 0 && t * kW4Cols + r < N) col_scale[(int64_t)e * N + t * kW4Cols + r] = __uint_as_float((uint32_t)exponent << 23);
+    }
+    char *mine = stage[wave];
+    for (int c = wave; c < kt; c += 4) {
+        const int64_t tile = first + c;
+        const u32x4 q = *(const u32x4 *)(codes + tile * kW4TileBytes + lane * 16);
 #pragma unroll
-        for (int p = 0; p < 4; ++p)
-            v[p] = pack_bf16x2(((float)((q[j] >> (4 * p)) & 15u) - z) * s, ((float)((q[j] >> (4 * p + 16)) & 15u) - z) * s);
-        *(u32x4 *)(row + k) = v;
+        for (int j = 0; j < 4; ++j) {
+            const int64_t at = tile * (kW4Cols * ng) + (r >> 2) * (ng * 4) + (j * 32 / group) * 4 + (r & 3);
+            const float s = bf16_to_f32(scales[at]) * inv;
+            const float z = zeros != nullptr ? (float)zeros[at] : 8.f;
+            u32x4 v;
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                const float lo = ((float)((q[j] >> (4 * p)) & 15u) - z) * s, hi = ((float)((q[j] >> (4 * p + 16)) & 15u) - z) * s;
+                if constexpr (HALF) {
+                    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+                    v[p] = __builtin_bit_cast(uint32_t, (f16x2{(_Float16)lo, (_Float16)hi}));
+                } else {
+                    v[p] = pack_bf16x2(lo, hi);
+                }
+            }
+            *(u32x4 *)(mine + r * 256 + (((j * 4 + g16) ^ r) << 4)) = v;       // piece p of row r at p ^ r: no bank twice
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = i * 4 + g16, n = t * kW4Cols + row, k = c * kW4Chunk + r * 8;
+            const u32x4 v = *(const u32x4 *)(mine + row * 256 + ((r ^ row) << 4));
+            if (n < N && k < K) __builtin_nontemporal_store(v, (u32x4 *)(out + ((int64_t)e * N + n) * K + k));
+        }
+    }
+}
+
+// out = fp16(x / f), row_scale[r] = f, the power of two below the row's largest magnitude: exact but for values 2^14 times
+// smaller than that, which lose what lies below 2^-24 of it.  One workgroup per row.
+__global__ __launch_bounds__(256) void w4_half_rows_kernel(const u32x4 *__restrict__ x, u32x4 *__restrict__ out, float *__restrict__ row_scale, int vecs) {
+    __shared__ uint32_t part[4];
+    const int64_t row = blockIdx.x;
+    uint32_t most = 0;
+    for (int i = threadIdx.x; i < vecs; i += 256) {
+        const u32x4 v = x[row * vecs + i];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const uint32_t lo = v[p] & 0x7fffu, hi = (v[p] >> 16) & 0x7fffu;
+            most = lo > most ? lo : most;
+            most = hi > most ? hi : most;
+        }
+    }
+#pragma unroll
+    for (int s = kWave / 2; s > 0; s >>= 1) {
+        const uint32_t o = __shfl_xor(most, s, kWave);
+        most = o > most ? o : most;
+    }
+    if (lane_id() == 0) part[threadIdx.x / kWave] = most;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) most = part[i] > most ? part[i] : most;
+    int exponent = (int)(most >> 7);
+    exponent = exponent < 1 ? 127 : (exponent > 253 ? 253 : exponent);       // a row of zeros: 1; not finite: it stays so
+    const float inv = __uint_as_float((uint32_t)(254 - exponent) << 23);
+    if (threadIdx.x == 0) row_scale[row] = __uint_as_float((uint32_t)exponent << 23);
+    for (int i = threadIdx.x; i < vecs; i += 256) {
+        const u32x4 v = x[row * vecs + i];
+        u32x4 o;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+            o[p] = __builtin_bit_cast(uint32_t, (f16x2{(_Float16)(__uint_as_float(v[p] << 16) * inv), (_Float16)(__uint_as_float(v[p] & 0xffff0000u) * inv)}));
+        }
+        out[row * vecs + i] = o;
     }
 }
 
@@ -115,15 +193,33 @@ static bool aligned(const void *p, int bytes) { return ((uintptr_t)p & (uintptr_
 
 static int tiles_of(int64_t n, int tile) { return (int)((n + tile - 1) / tile); }
 
+static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+// Where the form for many rows keeps what it writes: fp16 weights and rows, and their scales.
+struct WideLayout {
+    size_t weights, col_scales, rows, row_scales, bytes;
+};
+static WideLayout wide_layout(int64_t rows, int E, int64_t K, int64_t N) {
+    WideLayout w;
+    w.weights = 0;
+    w.col_scales = up256((size_t)E * N * K * 2);
+    w.rows = w.col_scales + up256((size_t)E * N * 4);
+    w.row_scales = w.rows + up256((size_t)rows * K * 2);
+    w.bytes = w.row_scales + up256((size_t)rows * 4);
+    return w;
+}
+
 struct W4Form {
-    bool wide;        // through bf16 weights and the bf16 product
+    bool wide;        // through fp16 weights
     int tile_rows;
     int m_tiles;
 };
-// Rows per expert decide.  The direct form reads the codes once for every row tile of an expert; past kWideRows rows the
-// bf16 product on weights that are written out first is the faster one.
-constexpr int kWideRows = 192;
-static W4Form choose_w4(int64_t rows, int E, const int64_t *host_sizes) {
+// Rows per expert decide.  The one kernel unpacks the codes again for every 64 rows and folds every group; from some number of
+// rows on the product on weights that are written out first is the faster one, the sooner the shorter the groups.  Measured,
+// us of the one kernel / through 16-bit weights: K 4096, N 28672, 8 experts, groups of 128: 256 rows 596 / 1203, 512 1144 / 1244,
+// 1024 2280 / 1973; groups of 32: 256 rows 774 / 1219, 512 1524 / 1262; K 2048, N 2816, 64 experts, groups of 128: 256 rows
+// 381 / 548, 512 748 / 602; groups of 32: 256 rows 480 / 553, 512 951 / 611.
+static long long wide_rows(int group) { return group == 128 ? 512 : (group == 64 ? 448 : 384); }
+static W4Form choose_w4(int64_t rows, int E, int64_t K, int64_t N, int group, const int64_t *host_sizes) {
     long long busy = E < rows ? E : rows;
     if (host_sizes != nullptr) {
         busy = 0;
@@ -132,7 +228,7 @@ static W4Form choose_w4(int64_t rows, int E, const int64_t *host_sizes) {
     if (busy < 1) busy = 1;
     const long long avg = (rows + busy - 1) / busy;
     W4Form f;
-    f.wide = avg > kWideRows;
+    f.wide = avg > wide_rows(group) && K % 32 == 0 && K * N * 2 < (1ll << 32);   // (what the 256-row tile takes)
     f.tile_rows = avg <= 16 ? 16 : (avg <= 32 ? 32 : 64);
     // row tiles: those of the sizes, or at most one short one for every expert with rows
     long long m = rows / f.tile_rows + (E < rows ? E : rows);
@@ -163,12 +259,22 @@ static int gmm_w4(const char *who, const void *a, const void *codes, const void 
     DMOE_REQUIRE(aligned(a, 16) && aligned(codes, 16) && aligned(scales, 16) && aligned(zeros, 16) && aligned(c, 16) && aligned(wide, 16),
                  DMOE_ERR_ARG, "%s: a pointer is not 16-byte aligned", who);
     if (rows == 0) return DMOE_OK;
-    const W4Form f = choose_w4(rows, E, host_batch_sizes);
-    if (f.wide && wide != nullptr && wide_bytes >= (size_t)E * N * K * 2) {
-        rc = dmoe_w4_dequant(codes, scales, zeros, group, wide, batch_sizes, E, K, N, stream);
-        if (rc != DMOE_OK) return rc;
-        return swiglu ? dmoe_gmm_swiglu(a, wide, c, batch_sizes, rows, E, K, n_out, 1, DMOE_BF16, state, workspace, workspace_bytes, host_batch_sizes, stream)
-                      : dmoe_gmm(a, wide, c, batch_sizes, rows, E, K, N, 1, DMOE_BF16, state, workspace, workspace_bytes, host_batch_sizes, stream);
+    const W4Form f = choose_w4(rows, E, K, N, group, host_batch_sizes);
+    const WideLayout at = wide_layout(rows, E, K, N);
+    if (f.wide && wide != nullptr && wide_bytes >= at.bytes) {
+        char *w = (char *)wide;
+        const int nt = tiles_of(N, kW4Cols), kt = tiles_of(K, kW4Chunk);
+        hipLaunchKernelGGL(w4_widen_kernel<true>, dim3(nt, E), dim3(256), 0, (hipStream_t)stream, (const char *)codes, (const uint16_t *)scales,
+                           (const uint8_t *)zeros, (uint16_t *)(w + at.weights), (float *)(w + at.col_scales), batch_sizes, (int)K, (int)N, nt, kt, group);
+        DMOE_LAUNCH_CHECK("w4_widen_kernel");
+        hipLaunchKernelGGL(w4_half_rows_kernel, dim3((unsigned)rows), dim3(256), 0, (hipStream_t)stream, (const u32x4 *)a, (u32x4 *)(w + at.rows),
+                           (float *)(w + at.row_scales), (int)(K / 8));
+        DMOE_LAUNCH_CHECK("w4_half_rows_kernel");
+        const HostSizes known(host_batch_sizes);
+        GmmArgs args{w + at.rows, w + at.weights, (char *)c, batch_sizes, (const float *)(w + at.row_scales), (const float *)(w + at.col_scales), rows, E,
+                     (int)K, (int)N, (int)n_out};
+        rc = bind_state(args, state, workspace, workspace_bytes, (hipStream_t)stream);
+        return rc != DMOE_OK ? rc : launch_tile256_half(args, swiglu, (hipStream_t)stream);
     }
     W4Args args{(const char *)a, (const char *)codes, (const char *)scales, (const char *)zeros, (char *)c, batch_sizes, rows, E, (int)K, (int)N,
                 (int)n_out, tiles_of(N, kW4Cols), tiles_of(K, kW4Chunk), f.m_tiles};
@@ -213,18 +319,17 @@ extern "C" int dmoe_w4_dequant(const void *codes, const void *scales, const void
     DMOE_REQUIRE(codes && scales && out, DMOE_ERR_ARG, "dmoe_w4_dequant: null pointer");
     DMOE_REQUIRE(aligned(codes, 16) && aligned(scales, 16) && aligned(out, 16), DMOE_ERR_ARG, "dmoe_w4_dequant: a pointer is not 16-byte aligned");
     const int nt = tiles_of(N, kW4Cols), kt = tiles_of(K, kW4Chunk);
-    DMOE_REQUIRE(nt < 65536, DMOE_ERR_SHAPE, "dmoe_w4_dequant: N=%lld", (long long)N);
-    hipLaunchKernelGGL(w4_dequant_kernel, dim3((kt + 3) / 4, nt, E), dim3(256), 0, (hipStream_t)stream, (const char *)codes, (const char *)scales,
-                       (const char *)zeros, (uint16_t *)out, batch_sizes, (int)K, (int)N, nt, kt, group);
-    DMOE_LAUNCH_CHECK("w4_dequant_kernel");
+    hipLaunchKernelGGL(w4_widen_kernel<false>, dim3(nt, E), dim3(256), 0, (hipStream_t)stream, (const char *)codes, (const uint16_t *)scales,
+                       (const uint8_t *)zeros, (uint16_t *)out, (float *)nullptr, batch_sizes, (int)K, (int)N, nt, kt, group);
+    DMOE_LAUNCH_CHECK("w4_widen_kernel");
     return DMOE_OK;
 }
 
-extern "C" int dmoe_gmm_w4_wide_bytes(int64_t rows, int E, int64_t K, int64_t N, const int64_t *host_batch_sizes, size_t *bytes) {
-    const int rc = check_w4("dmoe_gmm_w4_wide_bytes", E, K, N, 128);
+extern "C" int dmoe_gmm_w4_wide_bytes(int64_t rows, int E, int64_t K, int64_t N, int group, const int64_t *host_batch_sizes, size_t *bytes) {
+    const int rc = check_w4("dmoe_gmm_w4_wide_bytes", E, K, N, group);
     if (rc != DMOE_OK) return rc;
     DMOE_REQUIRE(bytes != nullptr && rows >= 0 && rows < (1ll << 31), DMOE_ERR_ARG, "dmoe_gmm_w4_wide_bytes: bad rows or null output");
-    *bytes = choose_w4(rows, E, host_batch_sizes).wide ? (size_t)E * N * K * 2 : 0;
+    *bytes = choose_w4(rows, E, K, N, group, host_batch_sizes).wide ? wide_layout(rows, E, K, N).bytes : 0;
     return DMOE_OK;
 }
 

@@ -544,8 +544,8 @@ def _gmm_w4(name: str, a: torch.Tensor, w: W4Weight, n_out: int, batch_sizes: to
     need = _lib.c_size_t(0)
     with torch.cuda.device(device):
         stream = _stream(device)
-        _lib.call("dmoe_gmm_w4_wide_bytes", rows, E, w.K, w.N, host_ptr, _lib.ctypes.byref(need))
-        if need.value:   # bf16 weights of this call, and the state of the bf16 product
+        _lib.call("dmoe_gmm_w4_wide_bytes", rows, E, w.K, w.N, w.group, host_ptr, _lib.ctypes.byref(need))
+        if need.value:   # 16-bit weights and rows of this call, and the state of the product on them
             wide = torch.empty(need.value, dtype=torch.uint8, device=device)
             more = (wide.data_ptr(), need.value, *_state_triple(device, workspace, arguments_ptr, stream))
         else:
@@ -559,8 +559,8 @@ def gmm_w4(a: torch.Tensor, w: W4Weight, batch_sizes: torch.Tensor, c: Optional[
            workspace: Optional[torch.Tensor] = None, arguments_ptr: Optional[int] = None,
            host_batch_sizes: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``c[o_e:o_e+n_e] = a[o_e:o_e+n_e] @ w[e].T`` on 4-bit weights, bf16 ``[rows, N]``.  From one row to
-    a prompt; many rows per expert go through bf16 weights that the call allocates and writes
-    (``E * N * K * 2`` bytes, for its own length).  The other arguments as :func:`gmm`'s."""
+    a prompt; many rows per expert go through 16-bit weights that the call allocates and writes
+    (``E * N * K * 2`` bytes and a little, for its own length).  The other arguments as :func:`gmm`'s."""
     return _gmm_w4("dmoe_gmm_w4", a, w, w.N, batch_sizes, c, workspace, arguments_ptr, host_batch_sizes)
 
 

@@ -351,16 +351,18 @@ int dmoe_gmm_fp8_swiglu(const void *a, const float *a_scale, const void *b, cons
  * that have rows.
  *
  * dmoe_gmm_w4 is c = a @ w[e]^T for a bf16 [rows, K], c bf16 [rows, N]; dmoe_gmm_w4_swiglu the gated form on w [E, 2I, K],
- * h [rows, I], as dmoe_gmm_swiglu.  Few rows per expert: one kernel that reads the codes, in 32-bit sums of unrounded
- * weights.  Many: where `wide` has dmoe_gmm_w4_wide_bytes(..) bytes (0: not needed), the weights of the experts that have
- * rows are written there as bf16 and go through dmoe_gmm; without it the one kernel serves any number of rows.
+ * h [rows, I], as dmoe_gmm_swiglu.  Few rows per expert: one kernel that reads the codes, 32-bit sums of unrounded weights.
+ * Many: where `wide` (any contents) has dmoe_gmm_w4_wide_bytes(..) bytes (0: not needed), the weights of
+ * the experts that have rows, rounded to the 11 bits of fp16, and the rows are written there with scales that are powers
+ * of two and go through the bf16 product's 256-row tile; without it the one kernel serves any number of rows.
  * state, workspace and host_batch_sizes as for dmoe_gmm (the first two serve that form only). */
 int dmoe_w4_bytes(int E, int64_t K, int64_t N, int group, size_t *code_bytes, size_t *scale_bytes, size_t *zero_bytes);
 int dmoe_w4_quant(const void *w, int E, int64_t K, int64_t N, int group, void *codes, void *scales, void *zeros,
                   void *stream);
 int dmoe_w4_dequant(const void *codes, const void *scales, const void *zeros, int group, void *out,
                     const int64_t *batch_sizes, int E, int64_t K, int64_t N, void *stream);
-int dmoe_gmm_w4_wide_bytes(int64_t rows, int E, int64_t K, int64_t N, const int64_t *host_batch_sizes, size_t *bytes);
+int dmoe_gmm_w4_wide_bytes(int64_t rows, int E, int64_t K, int64_t N, int group, const int64_t *host_batch_sizes,
+                           size_t *bytes);
 int dmoe_gmm_w4(const void *a, const void *codes, const void *scales, const void *zeros, int group, void *c,
                 const int64_t *batch_sizes, int64_t rows, int E, int64_t K, int64_t N, void *wide, size_t wide_bytes,
                 void *state, void *workspace, size_t workspace_bytes, const int64_t *host_batch_sizes, void *stream);

@@ -4,7 +4,9 @@ Tolerances, element by element.  A bf16 result is off by half a step, 2^-8 of it
 weights as they are; it adds (16 + q) x over a group of G in fp32 (at most 31 |x| a term, n terms off by at most n 2^-24 of
 their magnitudes, counted twice for a matrix core that adds several terms at a time: ``ACC``), takes (16 + z) times the
 group's sum of x off, and adds the groups: ACC (G + 8) 47 sum s |x|, and ACC (K / G + 16) times the sum of the groups'
-magnitudes.  The form through bf16 weights rounds each of them once instead: HALF |w| under the same sum."""
+magnitudes.  The form for many rows rounds each weight to fp16 (2^-11 of it at most), after scaling a column by a power of
+two below its largest scale and a row by one below its largest value, so that what is tiny beside those loses what lies
+below 2^-24 of them: 2^-11 |w| |x| + 2^-24 (16 max s |x| + |w| max |x|) under the sum, and K products added in fp32."""
 import pytest
 import torch
 
@@ -51,7 +53,8 @@ def _check(got, x, w, s, sizes, group, swiglu, wide):
         mag = a.abs() @ w[e].abs().t()
         off = ACC * (group + 8) * 47 * (a.abs() @ s[e].t()) + ACC * (a.shape[1] / group + 16) * mag
         if wide:
-            off = off + (HALF + ACC * a.shape[1]) * mag
+            off = (2.0 ** -11 + ACC * (a.shape[1] + 4)) * mag
+            off = off + 2.0 ** -24 * (a.abs().sum(1, keepdim=True) * 16 * s[e].max(1).values + a.abs().max(1, keepdim=True).values * w[e].abs().sum(1))
         if swiglu:
             I = w.shape[1] // 2
             g, p = want[:, :I], want[:, I:]
@@ -62,7 +65,7 @@ def _check(got, x, w, s, sizes, group, swiglu, wide):
         err = (got[at].double() - want).abs()
         bad = ~(err <= off + HALF * (want.abs() + off) + 1e-37)
         assert not bool(bad.any()), (e, int(bad.sum()), float(err[bad][0]), float(off[bad][0]), float(want[bad][0]))
-        if not wide and not swiglu and want.numel():
+        if not swiglu and want.numel():
             # every element's rounding is at most HALF of it, and so is the 2-norm's; the sums add a tenth at most here
             assert float(err.norm()) <= 1.1 * HALF * float(want.norm()) + 1e-30
 
@@ -105,26 +108,62 @@ def test_sizes_alone_on_the_device(rows_e, swiglu):
     # the library says that it takes the form through bf16 weights: the roundings are that form's)
     for wrong in ([0] * E, [E * rows_e] + [0] * (E - 1), [1] * E):
         wrong, need = torch.tensor(wrong), _lib.c_size_t(0)
-        _lib.call("dmoe_gmm_w4_wide_bytes", E * rows_e, E, K, N, wrong.data_ptr(), _lib.ctypes.byref(need))
+        _lib.call("dmoe_gmm_w4_wide_bytes", E * rows_e, E, K, N, group, wrong.data_ptr(), _lib.ctypes.byref(need))
         other = call(x, w, sizes.to(dev()), host_batch_sizes=wrong)
         _check(other, x, ref, s, sizes, group, swiglu, need.value > 0)
 
 
 @pytest.mark.parametrize("swiglu", [False, True])
-@pytest.mark.parametrize("group,zeros", [(32, True), (128, False)])
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, False), (128, True)])
 def test_many_rows(swiglu, group, zeros):
     announce(test="w4_many_rows", swiglu=swiglu, group=group, zeros=zeros)
-    sizes = torch.tensor([400, 0, 1, 513])
-    E, K, N, R = 4, 392, 304, 914
+    sizes = torch.tensor([1400, 0, 1, 1513])
+    E, K, N, R = 4, 416, 304, 2914
     w, ref, s = _weight(E, N, K, group, zeros, seed=3)
     x = _rand((R, K), 4)
     call = gg.gmm_w4_swiglu if swiglu else gg.gmm_w4
     for bs in (sizes, sizes.to(dev())):
+        need = _lib.c_size_t(0)
+        _lib.call("dmoe_gmm_w4_wide_bytes", R, E, K, N, group, None, _lib.ctypes.byref(need))
+        assert need.value > 0                                    # the form for many rows
         _check(call(x, w, bs), x, ref, s, sizes, group, swiglu, True)
     size, ptr = gg.get_arguments(E, dev())
     own = call(x, w, sizes, workspace=torch.empty(size, dtype=torch.uint8, device=dev()), arguments_ptr=ptr)
     assert torch.equal(own, call(x, w, sizes))
     gg.release_arguments(ptr)
+    # without room for 16-bit weights the one kernel takes any number of rows
+    c = torch.empty(R, N // 2 if swiglu else N, dtype=torch.bfloat16, device=dev())
+    _lib.call("dmoe_gmm_w4_swiglu" if swiglu else "dmoe_gmm_w4", x.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(),
+              None if w.zeros is None else w.zeros.data_ptr(), group, c.data_ptr(), sizes.to(dev()).data_ptr(), R, E, K, c.shape[1], None, 0,
+              None, None, 0, None, torch.cuda.current_stream().cuda_stream)
+    _check(c, x, ref, s, sizes, group, swiglu, False)
+
+
+@pytest.mark.parametrize("rows", [40, 1100])
+def test_range_of_values(rows):
+    announce(test="w4_range", rows=rows)
+    # rows and columns of any size, values far apart in one row and one column, zeros, and what is not finite stays in its row
+    K, N, group = 256, 64, 64
+    sizes = torch.tensor([rows])
+    x = _rand((rows, K), 1)
+    x[0] *= 1e30
+    x[1] *= 1e-30
+    x[2] = 0
+    x[3, ::2] *= 1e-6
+    x[4, 5] = 1e4
+    q = torch.randint(0, 16, (1, N, K), device=dev(), dtype=torch.uint8)
+    s = torch.full((1, N, K // group), 0.01, device=dev())
+    s[0, 0], s[0, 1], s[0, 2, 1:], s[0, 3] = 1e6, 1e-25, 1e-7, 0
+    s = s.to(torch.bfloat16)
+    w = gg.pack_w4(q, s, None, group)
+    sd = s.double().repeat_interleave(group, 2)
+    out = gg.gmm_w4(x, w, sizes)
+    _check(out, x, (q.double() - 8) * sd, sd, sizes, group, False, rows > 512)
+    assert bool((out[2] == 0).all()) and bool((out[:, 3] == 0).all())
+    x[7, 3], x[8, 9] = float("inf"), float("nan")
+    again = gg.gmm_w4(x, w, sizes)
+    keep = [r for r in range(rows) if r not in (7, 8)]
+    assert torch.equal(again[keep], out[keep]) and not bool(again[8].isfinite().any()) and not bool(again[7, 4:].isfinite().any())
 
 
 def test_rows_keep_apart_and_rows_behind():

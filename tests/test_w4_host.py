@@ -29,11 +29,14 @@ def test_host_side_argument_errors():
     assert lib.dmoe_w4_quant(p, 2, 64, 64, 64, None, p, None, None) == _lib.ERR_ARG
     assert lib.dmoe_w4_dequant(p, p, None, 64, p + 8, None, 2, 64, 64, None) == _lib.ERR_ARG
     need = ctypes.c_size_t(1)
-    assert lib.dmoe_gmm_w4_wide_bytes(8, 8, 64, 64, None, ctypes.byref(need)) == 0 and need.value == 0
-    assert lib.dmoe_gmm_w4_wide_bytes(1 << 20, 8, 64, 64, None, ctypes.byref(need)) == 0 and need.value == 8 * 64 * 64 * 2
+    assert lib.dmoe_gmm_w4_wide_bytes(8, 8, 64, 64, 128, None, ctypes.byref(need)) == 0 and need.value == 0
+    up = lambda n: -(-n // 256) * 256                             # weights, their scales, rows, their scales
+    wide = lambda rows: up(8 * 64 * 64 * 2) + up(8 * 64 * 4) + up(rows * 64 * 2) + up(rows * 4)
+    assert lib.dmoe_gmm_w4_wide_bytes(1 << 20, 8, 64, 64, 128, None, ctypes.byref(need)) == 0 and need.value == wide(1 << 20)
+    assert lib.dmoe_gmm_w4_wide_bytes(1 << 20, 8, 72, 64, 128, None, ctypes.byref(need)) == 0 and need.value == 0     # K % 32
     sizes = (ctypes.c_int64 * 8)(*([0] * 7 + [4000]))             # one expert has all the rows
-    assert lib.dmoe_gmm_w4_wide_bytes(4000, 8, 64, 64, sizes, ctypes.byref(need)) == 0 and need.value == 8 * 64 * 64 * 2
-    assert lib.dmoe_gmm_w4_wide_bytes(-1, 8, 64, 64, None, ctypes.byref(need)) == _lib.ERR_ARG
+    assert lib.dmoe_gmm_w4_wide_bytes(4000, 8, 64, 64, 128, sizes, ctypes.byref(need)) == 0 and need.value == wide(4000)
+    assert lib.dmoe_gmm_w4_wide_bytes(-1, 8, 64, 64, 128, None, ctypes.byref(need)) == _lib.ERR_ARG
 
 
 def unpack(w):
