@@ -4,11 +4,12 @@
 //
 // Bound by memory: the norm reads every gradient once, the scaling reads and writes it once (and does neither where the
 // norm is below the limit).  The list of tensors travels in the launch's arguments (kPerLaunch of them at a time), so
-// nothing has to be uploaded, kept alive or looked up by address and a recorded launch holds its own list.  A tensor is
-// cut in chunks of 64 KiB of whole 16-byte vectors of its memory; its first and last vector may be partly its own and
-// are then taken element by element.  Squares are added in 64 bits: they are exact there, so neither large nor tiny
-// gradients leave the range, and every workgroup leaves its sum at a place of its own that the reader adds up in a fixed
-// order: the same gradients give the same bits.
+// nothing has to be uploaded, kept alive or looked up by address and a recorded launch holds its own list.  The tensors'
+// memory, in whole 16-byte vectors one tensor behind the other, is dealt out to the workgroups in equal stretches; a
+// tensor's first and last vector may be partly its own and are then taken element by element.  The scaling walks each
+// stretch backwards: what the norm read last is what the last-level cache still has.  Squares are added in 64 bits: they
+// are exact there, so neither large nor tiny gradients leave the range, and every workgroup leaves its sum at a place of
+// its own that the reader adds up in a fixed order: the same gradients give the same bits.
 #include <algorithm>
 #include <exception>
 #include <utility>
@@ -22,19 +23,19 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kGradThreads = 256;
 constexpr int kGradSlots = 1024;                 // workgroups of a launch at most = partial sums
-constexpr int kChunkVecs = 4096;                 // 16-byte vectors of a chunk
+constexpr int kLeastVecs = 1024;                 // 16-byte vectors of a workgroup's stretch at least
 constexpr int kUnroll = 4;                       // vectors of a thread in flight
 constexpr int kPerLaunch = 160;                  // tensors in one launch's arguments (below 4 KiB)
 static_assert(kGradSlots * sizeof(double) == DMOE_GRAD_WORKSPACE_BYTES, "workspace as dmoe.h states it");
 
 struct GradTable {
     char *data[kPerLaunch];
-    int64_t bytes[kPerLaunch];
-    int chunk_start[kPerLaunch + 1];
-    uint8_t type[kPerLaunch];                    // DMOE_BF16, DMOE_FP16, DMOE_FP32
+    int64_t bytes[kPerLaunch];                   // of a tensor; its type (DMOE_BF16, DMOE_FP16, DMOE_FP32) in the top byte
+    int64_t vec_start[kPerLaunch + 1];           // vectors before the tensor
     int n;
 };
-static_assert(sizeof(GradTable) <= 3800, "launch arguments");
+static_assert(sizeof(GradTable) <= 3900, "launch arguments");
+constexpr int64_t kBytesMask = (1ll << 56) - 1;
 
 template <int kType> struct Elem;
 template <> struct Elem<DMOE_FP32> {
@@ -90,25 +91,28 @@ __device__ __forceinline__ u32x4 pack(const float (&f)[8]) {
 }
 
 // The vectors [v0, v0 + count) of tensor memory [data, data + bytes), vector 0 holding its first byte: whole ones to
-// `vec(address)`, the elements of one that lies partly outside to `one(address)`.
-template <int kType, typename Vec, typename One>
-__device__ __forceinline__ void for_vectors(char *data, int64_t bytes, int64_t v0, int count, Vec &&vec, One &&one) {
+// `vec(addresses, whether whole)`, the elements of one that lies partly outside to `one(address)`.  kBackwards: from the
+// last to the first.
+template <int kType, bool kBackwards, typename Vec, typename One>
+__device__ __forceinline__ void for_vectors(char *data, int64_t bytes, int64_t v0, int64_t count, Vec &&vec, One &&one) {
     constexpr int kBytes = Elem<kType>::kBytes;
-    char *const base = (char *)((uintptr_t)data & ~(uintptr_t)15);
+    constexpr int kStep = kGradThreads * kUnroll;
+    char *const base = (char *)((uintptr_t)data & ~(uintptr_t)15) + v0 * 16;
     char *const end = data + bytes;
-    for (int i0 = threadIdx.x; i0 < count; i0 += kGradThreads * kUnroll) {
+    for (int64_t i0 = 0; i0 < count; i0 += kStep) {
         char *at[kUnroll];
-        bool whole[kUnroll];
+        bool whole[kUnroll], there[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-            const int i = i0 + u * kGradThreads;
-            at[u] = base + (v0 + i) * 16;
-            whole[u] = i < count && at[u] >= data && at[u] + 16 <= end;
+            const int64_t k = i0 + u * kGradThreads + threadIdx.x, i = kBackwards ? count - 1 - k : k;
+            there[u] = k < count;
+            at[u] = base + i * 16;
+            whole[u] = there[u] && at[u] >= data && at[u] + 16 <= end;
         }
         vec(at, whole);
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-            if (whole[u] || i0 + u * kGradThreads >= count) continue;
+            if (whole[u] || !there[u]) continue;
             for (char *p = at[u] < data ? data : at[u]; p < at[u] + 16 && p < end; p += kBytes) one(p);
         }
     }
@@ -127,29 +131,30 @@ __device__ __forceinline__ double block_sum(double v) {
     return v;
 }
 
-// f(type tag, data, bytes, first vector, vectors) for every chunk of this workgroup
-template <typename F>
-__device__ __forceinline__ void for_chunks(const GradTable &t, F &&f) {
-    for (int c = blockIdx.x; c < t.chunk_start[t.n]; c += gridDim.x) {
-        int lo = 0, hi = t.n;                     // the last tensor whose first chunk is not behind c
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (t.chunk_start[mid] <= c) lo = mid; else hi = mid;
-        }
-        char *data = t.data[lo];
-        const int64_t bytes = t.bytes[lo];
-        const int64_t vecs = ((int64_t)((uintptr_t)data & 15) + bytes + 15) / 16;
-        const int64_t v0 = (int64_t)(c - t.chunk_start[lo]) * kChunkVecs;
-        const int count = (int)(vecs - v0 < kChunkVecs ? vecs - v0 : kChunkVecs);
-        f(t.type[lo], data, bytes, v0, count);
+// f(type, data, bytes, first vector, vectors) for the tensors' parts in this workgroup's stretch
+template <bool kBackwards, typename F>
+__device__ __forceinline__ void for_parts(const GradTable &t, F &&f) {
+    const int64_t total = t.vec_start[t.n], share = total / gridDim.x, rest = total % gridDim.x;
+    const int64_t b = blockIdx.x, lo = b * share + (b < rest ? b : rest), hi = lo + share + (b < rest ? 1 : 0);
+    if (lo >= hi) return;
+    const int64_t look = kBackwards ? hi - 1 : lo;
+    int at = 0, above = t.n;                      // the last tensor whose first vector is not behind `look`
+    while (above - at > 1) {
+        const int mid = (at + above) >> 1;
+        if (t.vec_start[mid] <= look) at = mid; else above = mid;
+    }
+    for (; kBackwards ? at >= 0 && t.vec_start[at + 1] > lo : at < t.n && t.vec_start[at] < hi; at += kBackwards ? -1 : 1) {
+        const int64_t first = t.vec_start[at], last = t.vec_start[at + 1];
+        const int64_t v0 = (lo > first ? lo : first), v1 = (hi < last ? hi : last);
+        f((int)(t.bytes[at] >> 56), t.data[at], t.bytes[at] & kBytesMask, v0 - first, v1 - v0);
     }
 }
 
 template <int kType>
-__device__ __forceinline__ double chunk_squares(char *data, int64_t bytes, int64_t v0, int count) {
+__device__ __forceinline__ double part_squares(char *data, int64_t bytes, int64_t v0, int64_t count) {
     double sum[kUnroll] = {};
     auto add = [](double &s, float v) { s = fma((double)v, (double)v, s); };
-    for_vectors<kType>(data, bytes, v0, count,
+    for_vectors<kType, false>(data, bytes, v0, count,
         [&](char *(&at)[kUnroll], const bool (&whole)[kUnroll]) {
             u32x4 v[kUnroll];
 #pragma unroll
@@ -169,13 +174,13 @@ __device__ __forceinline__ double chunk_squares(char *data, int64_t bytes, int64
     return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
-// slots[b] (+)= the squares of workgroup b's chunks
+// slots[b] (+)= the squares of workgroup b's stretch
 __global__ __launch_bounds__(kGradThreads) void grad_squares_kernel(const GradTable t, double *slots, int first) {
     double sum = 0;
-    for_chunks(t, [&](int type, char *data, int64_t bytes, int64_t v0, int count) {
-        if (type == DMOE_FP32) sum += chunk_squares<DMOE_FP32>(data, bytes, v0, count);
-        else if (type == DMOE_BF16) sum += chunk_squares<DMOE_BF16>(data, bytes, v0, count);
-        else sum += chunk_squares<DMOE_FP16>(data, bytes, v0, count);
+    for_parts<false>(t, [&](int type, char *data, int64_t bytes, int64_t v0, int64_t count) {
+        if (type == DMOE_FP32) sum += part_squares<DMOE_FP32>(data, bytes, v0, count);
+        else if (type == DMOE_BF16) sum += part_squares<DMOE_BF16>(data, bytes, v0, count);
+        else sum += part_squares<DMOE_FP16>(data, bytes, v0, count);
     });
     sum = block_sum(sum);
     if (threadIdx.x == 0) slots[blockIdx.x] = first ? sum : slots[blockIdx.x] + sum;
@@ -193,8 +198,8 @@ __global__ __launch_bounds__(kGradThreads) void grad_norm_kernel(const double *s
 }
 
 template <int kType>
-__device__ __forceinline__ void scale_chunk(char *data, int64_t bytes, int64_t v0, int count, float coef) {
-    for_vectors<kType>(data, bytes, v0, count,
+__device__ __forceinline__ void scale_part(char *data, int64_t bytes, int64_t v0, int64_t count, float coef) {
+    for_vectors<kType, true>(data, bytes, v0, count,
         [&](char *(&at)[kUnroll], const bool (&whole)[kUnroll]) {
             u32x4 v[kUnroll];
 #pragma unroll
@@ -222,10 +227,10 @@ __global__ __launch_bounds__(kGradThreads) void grad_scale_kernel(const GradTabl
     const double ratio = max_norm / (total + 1e-6);
     if (ratio >= 1.0) return;                     // (not so where the ratio is NaN: the gradients become NaN then)
     const float coef = (float)ratio;
-    for_chunks(t, [&](int type, char *data, int64_t bytes, int64_t v0, int count) {
-        if (type == DMOE_FP32) scale_chunk<DMOE_FP32>(data, bytes, v0, count, coef);
-        else if (type == DMOE_BF16) scale_chunk<DMOE_BF16>(data, bytes, v0, count, coef);
-        else scale_chunk<DMOE_FP16>(data, bytes, v0, count, coef);
+    for_parts<true>(t, [&](int type, char *data, int64_t bytes, int64_t v0, int64_t count) {
+        if (type == DMOE_FP32) scale_part<DMOE_FP32>(data, bytes, v0, count, coef);
+        else if (type == DMOE_BF16) scale_part<DMOE_BF16>(data, bytes, v0, count, coef);
+        else scale_part<DMOE_FP16>(data, bytes, v0, count, coef);
     });
 }
 
@@ -255,28 +260,26 @@ static int64_t bytes_of(const dmoe_grad &g) { return g.numel * (g.dtype == DMOE_
 static std::vector<GradTable> tables_of(const dmoe_grad *grads, int64_t n, int *blocks) {
     std::vector<GradTable> out;
     GradTable t{};
-    int64_t chunks = 0, most = 1;
+    int64_t vecs = 0, most = 1;
     auto flush = [&]() {
-        t.chunk_start[t.n] = (int)chunks;
-        if (chunks > most) most = chunks;
+        t.vec_start[t.n] = vecs;
+        if (vecs > most) most = vecs;
         out.push_back(t);
         t.n = 0;
-        chunks = 0;
+        vecs = 0;
     };
     for (int64_t i = 0; i < n; ++i) {
         if (grads[i].numel == 0) continue;
+        if (t.n == kPerLaunch) flush();
         const int64_t bytes = bytes_of(grads[i]);
-        const int64_t vecs = ((int64_t)((uintptr_t)grads[i].data & 15) + bytes + 15) / 16;
-        const int64_t own = (vecs + kChunkVecs - 1) / kChunkVecs;
-        if (t.n == kPerLaunch || chunks + own > (1 << 30)) flush();
         t.data[t.n] = (char *)grads[i].data;
-        t.bytes[t.n] = bytes;
-        t.type[t.n] = (uint8_t)grads[i].dtype;
-        t.chunk_start[t.n] = (int)chunks;
+        t.bytes[t.n] = bytes | (int64_t)grads[i].dtype << 56;
+        t.vec_start[t.n] = vecs;
         ++t.n;
-        chunks += own;
+        vecs += ((int64_t)((uintptr_t)grads[i].data & 15) + bytes + 15) / 16;
     }
     if (t.n > 0 || out.empty()) flush();
+    most = (most + kLeastVecs - 1) / kLeastVecs;
     *blocks = (int)(most < kGradSlots ? most : kGradSlots);
     return out;
 }

@@ -30,22 +30,27 @@ def _dense(g: torch.Tensor) -> bool:
 def _table(grads: List[torch.Tensor]):
     """(device, host array of dmoe_grad) of the gradients."""
     device = grads[0].device
-    for g in grads:
-        if not g.is_cuda:
+    if device.type != "cuda":
+        raise RuntimeError("gradient norms need device tensors; disagmoe_amd has no CPU fallback")
+    index = device.index
+    if any(i != index for i in map(torch.Tensor.get_device, grads)):
+        other = next(g.device for g in grads if g.device != device)
+        if other.type != "cuda":
             raise RuntimeError("gradient norms need device tensors; disagmoe_amd has no CPU fallback")
-        if g.device != device:
-            raise ValueError(f"gradients on {device} and {g.device}: one call handles one device")
-        if g.layout != torch.strided:
-            raise TypeError(f"gradients must be strided tensors, got {g.layout}")
-        if not g.is_contiguous() and g.numel() and not _dense(g):
-            raise ValueError(f"a gradient of shape {tuple(g.shape)} with strides {g.stride()} does not fill its memory")
+        raise ValueError(f"gradients on {device} and {other}: one call handles one device")
+    if not all(map(torch.Tensor.is_contiguous, grads)):
+        for g in grads:
+            if g.layout is not torch.strided:
+                raise TypeError(f"gradients must be strided tensors, got {g.layout}")
+            if g.numel() and not _dense(g):
+                raise ValueError(f"a gradient of shape {tuple(g.shape)} with strides {g.stride()} does not fill its memory")
     try:
         kinds = [_DTYPES[g.dtype] for g in grads]
     except KeyError as e:
         raise TypeError(f"gradients must be fp32, bf16 or fp16, got {e.args[0]}") from None
     table = np.empty(len(grads), dtype=_GRAD)
-    table["data"] = [g.data_ptr() for g in grads]
-    table["numel"] = [g.numel() for g in grads]
+    table["data"] = list(map(torch.Tensor.data_ptr, grads))
+    table["numel"] = list(map(torch.Tensor.numel, grads))
     table["dtype"] = kinds
     return device, table
 
