@@ -381,13 +381,19 @@ void gmm_tile256_kernel(const GmmArgs p) {
                     const int i = i2 * 2 + ii;
                     const int row = ii * 16 + l16;
                     if constexpr (KEEP) {
-                        // 16 bytes per lane, 64 of a row; the fragment beside it fills the line
-                        const int r = wm * TM + i * 16 + l16;
+                        // the sums in whole lines: 16 rows of 128 bytes of the gate columns, then of the up columns, through
+                        // the wavefront's 4 KiB, the 16-byte chunk c of row r at c ^ (r & 7)
+                        char *keep = smem + (cur_S % kStages) * kStage + wave * 4096;
 #pragma unroll
-                        for (int j = 0; j < FN; ++j) {
-                            const int col = col0 + (j % FNO) * 16 + g16 * 4;
+                        for (int j = 0; j < FN; ++j)
+                            *(f32x4 *)(keep + (j / FNO) * 2048 + l16 * 128 + ((((j % FNO) * 4 + g16) ^ (l16 & 7)) << 4)) = acc[i][j];
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const int kr = (q & 1) * 8 + lane / 8, kc = lane & 7;
+                            const f32x4 val = *(const f32x4 *)(keep + (q >> 1) * 2048 + kr * 128 + ((kc ^ (kr & 7)) << 4));
+                            const int r = wm * TM + i * 16 + kr, col = col0 + kc * 4;
                             if (r < cur_rows_e && col < n_out)
-                                *(f32x4 *)(p.u + (long long)(cur_row0 + r) * p.N + (j < FNO ? 0 : n_out) + col) = acc[i][j];
+                                __builtin_nontemporal_store(val, (f32x4 *)(p.u + (long long)(cur_row0 + r) * p.N + (q >> 1) * n_out + col));
                         }
                     }
                     if constexpr (HALF) {

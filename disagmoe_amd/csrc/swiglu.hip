@@ -107,7 +107,9 @@ extern "C" int dmoe_zero_rows_behind(void *c, const int64_t *batch_sizes, int64_
     if (rc != DMOE_OK) return rc;
     if (rows == 0) return DMOE_OK;
     DMOE_REQUIRE(c != nullptr && ((uintptr_t)c & 15) == 0, DMOE_ERR_ARG, "dmoe_zero_rows_behind: null or unaligned pointer");
-    hipLaunchKernelGGL(zero_behind_kernel, dim3(blocks_of(rows * (d / 8))), dim3(kSwThreads), 0, (hipStream_t)stream,
+    // (most often there is nothing to do: one workgroup per compute unit finds out soonest)
+    const unsigned blocks = blocks_of(rows * (d / 8)), cus = (unsigned)device_cus();
+    hipLaunchKernelGGL(zero_behind_kernel, dim3(blocks < cus ? blocks : cus), dim3(kSwThreads), 0, (hipStream_t)stream,
                        (u32x4 *)c, batch_sizes, E, rows, d / 8);
     DMOE_LAUNCH_CHECK("zero_behind_kernel");
     return DMOE_OK;
