@@ -26,7 +26,7 @@ void gmm_wgrad_kernel(const GmmArgs p) {
     constexpr int kImage = BT * kDK * 2;                 // 16 KiB per operand and stage
     constexpr int kStage = 2 * kImage;
     constexpr int kStages = 4;
-    extern __shared__ __attribute__((aligned(16))) char smem[];
+    extern __shared__ __attribute__((aligned(1024))) char smem[];   // (operand addresses are taken apart by bits below)
     __shared__ int s_tile_start[kMaxGroups + 1];
     __shared__ int s_row_start[kMaxGroups + 1];
     __shared__ long long s_item;
@@ -59,11 +59,9 @@ void gmm_wgrad_kernel(const GmmArgs p) {
         const int r = g16 * 8 + (l16 >> 2);
         return r * 512 + (((col >> 3) ^ kn_swizzle(r)) * 16) + (col & 7) * 2;
     };
-    int fa_off[FM], fb_off[FN];
-#pragma unroll
-    for (int i = 0; i < FM; ++i) fa_off[i] = read_off(wm * TM + i * 16);
-#pragma unroll
-    for (int j = 0; j < FN; ++j) fb_off[j] = kImage + read_off(wn * TN + j * 16);
+    // the next fragment is 16 columns, 2 chunks, further on: bits 5 .. 7 of the address, which the swizzle flips and nothing
+    // else touches, so fragment i is read at the first one's address ^ 32 i
+    const uint32_t fa_0 = smem_addr + read_off(wm * TM), fb_0 = smem_addr + kImage + read_off(wn * TN);
 
     // ---- state of the item whose copies are being issued ----
     int e = 0, k0 = 0, n0 = 0, rows_e = 0, S = 0, pre = 0;
@@ -71,8 +69,8 @@ void gmm_wgrad_kernel(const GmmArgs p) {
     uint32_t a_col = 0, d_col = 0;                         // byte offset of this lane's 16 bytes in a row
     auto open_item = [&](long long q) {
         const long long L = item_order(q, G, total);
-        e = (int)(L / per_expert);
-        const int idx = (int)(L - e * per_expert);
+        e = __builtin_amdgcn_readfirstlane((int)(L / per_expert));
+        const int idx = __builtin_amdgcn_readfirstlane((int)(L - e * per_expert));
         // bands of 4 k-tiles, their n-tiles one after the other, a band's k-tiles innermost: what shares an operand slice
         // runs side by side on one XCD
         constexpr int kBand = 4;
@@ -103,14 +101,27 @@ void gmm_wgrad_kernel(const GmmArgs p) {
             copy_g2lds_16<kImage + c * kBlock>(rr * pitch_d + d_col, db, lds);
         });
     };
-    auto issue_prologue = [&]() {
-        for (int s = 0; s < pre; ++s) issue_copies(s);
+    // until at most n stages' copies of this wavefront are outstanding, and kStores stores issued between them
+    auto wait_ahead = [&](int n, auto stores_tag) {
+        constexpr int st = decltype(stores_tag)::value;
+        if (n >= 3) DMOE_WAIT_VMCNT(3 * kLoads + st);
+        else if (n == 2) DMOE_WAIT_VMCNT(2 * kLoads + st);
+        else if (n == 1) DMOE_WAIT_VMCNT(kLoads + st);
+        else DMOE_WAIT_VMCNT(st);
     };
-    auto wait_ahead = [&](int n) {
-        if (n >= 3) DMOE_WAIT_VMCNT(3 * kLoads);
-        else if (n == 2) DMOE_WAIT_VMCNT(2 * kLoads);
-        else if (n == 1) DMOE_WAIT_VMCNT(kLoads);
-        else DMOE_WAIT_VMCNT(0);
+    constexpr std::integral_constant<int, 0> no_stores{};
+    constexpr std::integral_constant<int, 16> the_stores{};
+    // An item's first three stages are copied before the epilogue of the item before it, the fourth behind it, where the LDS
+    // that the epilogue passes its rows through is free again: with contractions of some 30 stages the way there and back
+    // would otherwise be a tenth of a tile.  The 16 stores of that epilogue lie between them in the order in which a
+    // wavefront's accesses complete, and the waits for stages 1 and 2 need not be waits for the stores too (`behind`: the
+    // epilogue wrote a whole tile, so it was 16 of them).
+    bool behind = false;
+    auto issue_early = [&]() {
+        for (int s = 0; s < (pre < 3 ? pre : 3); ++s) issue_copies(s);
+    };
+    auto issue_late = [&]() {
+        if (pre > 3) issue_copies(3);
     };
 
     unsigned int draw = 0;
@@ -119,7 +130,8 @@ void gmm_wgrad_kernel(const GmmArgs p) {
     long long q = blockIdx.x;
     if (q < total) {
         open_item(q);
-        issue_prologue();
+        issue_early();
+        issue_late();
     }
 
     while (q < total) {
@@ -144,9 +156,10 @@ void gmm_wgrad_kernel(const GmmArgs p) {
         };
         const bool ragged = (cur_rows & (kDK - 1)) != 0;
         bf16x8 fa[FM], fb[FN];
-        auto read_operand = [&](bf16x8 &f, const char *src) {
-            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3))) *)DMOE_LDS_PTR(src));
-            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3))) *)DMOE_LDS_PTR(src + 4 * 512));
+        auto read_operand = [&](bf16x8 &f, uint32_t src) {
+            typedef s16x4 __attribute__((address_space(3))) *lds_ptr;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(uintptr_t)src);
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(uintptr_t)(src + 4 * 512));
             const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
             __builtin_memcpy(&f, &v, 16);
         };
@@ -154,17 +167,21 @@ void gmm_wgrad_kernel(const GmmArgs p) {
         auto stage = [&](int s, auto refill_tag, int ahead, bool next) {
             constexpr bool kRefill = decltype(refill_tag)::value;
             auto landed = [&]() {
-                if constexpr (kRefill) DMOE_WAIT_VMCNT((kStages - 2) * kLoads);
-                else {
-                    wait_ahead(ahead);
+                const bool early = behind && s < 2;        // stage s + 1 was copied before the last epilogue
+                if constexpr (kRefill) {
+                    if (early) DMOE_WAIT_VMCNT((kStages - 2) * kLoads + 16);
+                    else DMOE_WAIT_VMCNT((kStages - 2) * kLoads);
+                } else {
+                    if (early) wait_ahead(ahead, the_stores);
+                    else wait_ahead(ahead, no_stores);
                     if (ragged && s + 1 == cur_S - 1) clear_behind(s + 1);
                 }
             };
-            const char *t = smem + (s % kStages) * kStage;
+            const uint32_t slot = (uint32_t)(s % kStages) * kStage;
 #pragma unroll
-            for (int i = 0; i < FM; ++i) read_operand(fa[i], t + fa_off[i]);
+            for (int i = 0; i < FM; ++i) read_operand(fa[i], (fa_0 + slot) ^ (i * 32));
 #pragma unroll
-            for (int j = 0; j < FN; ++j) read_operand(fb[j], t + fb_off[j]);
+            for (int j = 0; j < FN; ++j) read_operand(fb[j], (fb_0 + slot) ^ (j * 32));
             if constexpr (kRefill) issue_copies(s + kStages - 1);
             if (next && wm == 1) landed();
             __builtin_amdgcn_sched_barrier(0);
@@ -186,25 +203,40 @@ void gmm_wgrad_kernel(const GmmArgs p) {
             __builtin_amdgcn_sched_barrier(0);
         };
         if (cur_S > 0) {
-            wait_ahead(pre - 1);
+            if (behind) wait_ahead(pre - 1, the_stores);
+            else wait_ahead(pre - 1, no_stores);
             if (ragged && cur_S == 1) clear_behind(0);
             __syncthreads();
             if (wm == 1) __syncthreads();                  // the half that runs a phase behind
-            int s = 0;
-            stage(0, std::false_type{}, (cur_S - 2 < kStages - 2 ? cur_S - 2 : kStages - 2), cur_S > 1);
-            for (s = 1; s + kStages - 1 < cur_S; ++s) stage(s, std::true_type{}, 0, true);
-            for (; s < cur_S; ++s) {
+            auto ahead_of = [&](int s) {                   // stages behind s + 1 that may be in flight when s + 1 has to be there
                 const int left = cur_S - 1 - s;
-                stage(s, std::false_type{}, left - 1 < kStages - 2 ? left - 1 : kStages - 2, left > 0);
-            }
+                return left - 1 < kStages - 2 ? left - 1 : kStages - 2;
+            };
+            stage(0, std::false_type{}, ahead_of(0), cur_S > 1);
+            int s = 1;
+            for (; s + kStages - 1 < cur_S; ++s) stage(s, std::true_type{}, 0, true);
+            for (; s < cur_S; ++s) stage(s, std::false_type{}, ahead_of(s), s + 1 < cur_S);
             if (wm == 0) __syncthreads();
+        }
+        // ---- the next item and its first copies ----
+        if (drawer) s_item = sched_item(draw, streams);
+        __syncthreads();                                   // also: the last stage has been read by everyone
+        q = (long long)to_scalar((uint64_t)s_item);
+        if (q < total) {
+            if (drawer) draw = sched_draw(p.sched, streams);
+            open_item(q);
+            issue_early();
         }
 
         // ---- epilogue: lane l holds, of fragment (i, j), row i * 16 + l % 16 (of K) and the 4 columns j * 16 + (l / 16) * 4 ..;
         // 32 rows at a time through 4 KiB of LDS that belong to the wavefront, out by whole 128-byte lines ----
-        char *stg = smem + (cur_S % kStages) * kStage + wave * 4096;
-        const int col0 = cur_n0 + wn * TN;
-        uint16_t *out = (uint16_t *)p.c + ((long long)cur_e * p.K + cur_k0) * p.N;
+        char *stg = smem + 3 * kStage + wave * 4096;
+        // (the rows' addresses as a scalar that moves and one offset per lane: 16 addresses a lane would not stay in registers)
+        const bool whole = cur_k0 + BT <= p.K && cur_n0 + BT <= p.N;
+        const int out_col = cur_n0 + wn * TN + (lane % 8) * 8;
+        const uint32_t out_off = (uint32_t)(lane / 8) * pitch_d + (uint32_t)out_col * 2;
+        uint64_t out_row = to_scalar((uint64_t)(uintptr_t)p.c + ((uint64_t)cur_e * p.K + cur_k0 + wm * TM) * pitch_d);
+        int rows_left = p.K - cur_k0 - wm * TM;            // of the result, from the one out_row is at
 #pragma unroll
         for (int i2 = 0; i2 < FM / 2; ++i2) {
 #pragma unroll
@@ -223,20 +255,15 @@ void gmm_wgrad_kernel(const GmmArgs p) {
             for (int t = 0; t < 4; ++t) {
                 const int row = t * 8 + lane / 8, c = lane % 8;
                 const u32x4 val = *(const u32x4 *)(stg + row * 128 + ((c ^ ((row >> 1) & 7)) << 4));
-                const int krow = wm * TM + i2 * 32 + row, gcol = col0 + c * 8;
-                if (cur_k0 + krow >= p.K || gcol >= p.N) continue;
-                *(u32x4 *)(out + (long long)krow * p.N + gcol) = val;
+                if (whole || (lane / 8 < rows_left && out_col < p.N)) *(u32x4 *)((char *)out_row + out_off) = val;
+                out_row += 8ull * pitch_d;
+                rows_left -= 8;
             }
         }
 
-        if (drawer) s_item = sched_item(draw, streams);
-        __syncthreads();   // also: the last stage has been read by everyone and the staged rows have been read back
-        q = (long long)to_scalar((uint64_t)s_item);
-        if (q < total) {
-            if (drawer) draw = sched_draw(p.sched, streams);
-            open_item(q);
-            issue_prologue();
-        }
+        behind = whole;
+        __syncthreads();                                   // the staged rows have been read back by everyone
+        if (q < total) issue_late();
     }
     sched_finish(p.sched, drawer, draw, streams, total);
 }
