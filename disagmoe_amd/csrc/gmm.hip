@@ -468,7 +468,7 @@ static int own_slot(hipStream_t stream, SchedSlot **out) {
 
 int bind_state(GmmArgs &args, void *state, void *workspace, size_t workspace_bytes, hipStream_t stream) {
     args.arrive = nullptr; args.partials = nullptr; args.partial_bytes = 0;
-    args.a_rows = nullptr; args.a_src_rows = 0; args.u = nullptr;
+    args.a_rows = nullptr; args.a_src_rows = 0; args.u = nullptr; args.split = 1;
     if (state == nullptr) return own_slot(stream, &args.sched);
     DMOE_REQUIRE(((uintptr_t)state & 255) == 0, DMOE_ERR_WORKSPACE, "grouped GEMM: the state block must be 256-byte aligned");
     args.sched = (SchedSlot *)state;

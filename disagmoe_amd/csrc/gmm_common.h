@@ -40,6 +40,8 @@ struct GmmArgs {
     long long a_src_rows;
     // (the gated form's KEEP builds) u [rows, N] in fp32: the sums that the activation is taken of, for its gradient
     float *u;
+    // (weight gradients) pieces that every tile's contraction is cut into
+    int split;
 };
 
 // ---- work distribution ---------------------------------------------------------------------------

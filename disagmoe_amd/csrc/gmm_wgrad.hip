@@ -15,6 +15,17 @@
 
 namespace dmoe {
 
+// Tile number idx of an expert's result.  Bands of 4 k-tiles, their n-tiles one after the other, a band's k-tiles innermost:
+// what shares an operand slice runs side by side on one XCD.
+__device__ __forceinline__ void wgrad_tile(int idx, int kt_n, int nt_n, int &k0, int &n0) {
+    constexpr int kBand = 4;
+    const int band = idx / (kBand * nt_n);
+    const int width = kt_n - band * kBand < kBand ? kt_n - band * kBand : kBand;
+    const int in = idx - band * kBand * nt_n;
+    n0 = (in / width) * 256;
+    k0 = (band * kBand + in % width) * 256;
+}
+
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void gmm_wgrad_kernel(const GmmArgs p) {
     constexpr int BT = 256, NW = 8, WN = 4;
@@ -42,8 +53,10 @@ void gmm_wgrad_kernel(const GmmArgs p) {
 
     const int kt_n = (p.K + BT - 1) / BT, nt_n = (p.N + BT - 1) / BT;
     const long long per_expert = (long long)kt_n * nt_n;
-    const long long total = per_expert * E;
+    const long long tiles = per_expert * E;
     const int G = gridDim.x;
+    const int split = p.split;                             // pieces of every tile's contraction (wgrad_split)
+    const long long total = tiles * split;
     const uint32_t pitch_a = (uint32_t)p.K * 2, pitch_d = (uint32_t)p.N * 2;
     const uint32_t smem_addr = lds_addr(smem);
     const int streams = (G % kXcds == 0) ? kXcds : 1;
@@ -64,24 +77,30 @@ void gmm_wgrad_kernel(const GmmArgs p) {
     const uint32_t fa_0 = smem_addr + read_off(wm * TM), fb_0 = smem_addr + kImage + read_off(wn * TN);
 
     // ---- state of the item whose copies are being issued ----
-    int e = 0, k0 = 0, n0 = 0, rows_e = 0, S = 0, pre = 0;
+    int e = 0, k0 = 0, n0 = 0, rows_e = 0, S = 0, pre = 0;   // (rows_e and S: of its piece)
+    int part = -1, split_tile = 0;
     uint64_t a_base = 0, d_base = 0;
     uint32_t a_col = 0, d_col = 0;                         // byte offset of this lane's 16 bytes in a row
     auto open_item = [&](long long q) {
-        const long long L = item_order(q, G, total);
+        long long L = item_order(q, G, total);
+        if (split > 1) {                                   // the same piece of all tiles side by side
+            part = __builtin_amdgcn_readfirstlane((int)(L / tiles));
+            L -= part * tiles;
+            split_tile = __builtin_amdgcn_readfirstlane((int)L);
+        }
         e = __builtin_amdgcn_readfirstlane((int)(L / per_expert));
         const int idx = __builtin_amdgcn_readfirstlane((int)(L - e * per_expert));
-        // bands of 4 k-tiles, their n-tiles one after the other, a band's k-tiles innermost: what shares an operand slice
-        // runs side by side on one XCD
-        constexpr int kBand = 4;
-        const int band = idx / (kBand * nt_n);
-        const int width = kt_n - band * kBand < kBand ? kt_n - band * kBand : kBand;
-        const int in = idx - band * kBand * nt_n;
-        n0 = (in / width) * BT;
-        k0 = (band * kBand + in % width) * BT;
-        const int row0 = __builtin_amdgcn_readfirstlane(s_row_start[e]);
+        wgrad_tile(idx, kt_n, nt_n, k0, n0);
+        int row0 = __builtin_amdgcn_readfirstlane(s_row_start[e]);
         rows_e = __builtin_amdgcn_readfirstlane(s_row_start[e + 1]) - row0;
         S = (rows_e + kDK - 1) / kDK;
+        if (split > 1) {                                   // stages [S part / split, S (part + 1) / split) of the tile
+            const int lo = (int)((long long)S * part / split), hi = (int)((long long)S * (part + 1) / split);
+            row0 += lo * kDK;
+            rows_e = (hi < S ? hi * kDK : rows_e) - lo * kDK;
+            S = hi - lo;
+            if (S == 0) rows_e = 0;
+        }
         pre = S < kStages ? S : kStages;
         a_base = to_scalar((uint64_t)(uintptr_t)p.a + (uint64_t)row0 * pitch_a);
         d_base = to_scalar((uint64_t)(uintptr_t)p.b + (uint64_t)row0 * pitch_d);
@@ -135,7 +154,7 @@ void gmm_wgrad_kernel(const GmmArgs p) {
     }
 
     while (q < total) {
-        const int cur_e = e, cur_k0 = k0, cur_n0 = n0, cur_S = S, cur_rows = rows_e;
+        const int cur_e = e, cur_k0 = k0, cur_n0 = n0, cur_S = S, cur_rows = rows_e, cur_part = part, cur_split_tile = split_tile;
         f32x4 acc[FM][FN];
 #pragma unroll
         for (int i = 0; i < FM; ++i)
@@ -230,6 +249,15 @@ void gmm_wgrad_kernel(const GmmArgs p) {
 
         // ---- epilogue: lane l holds, of fragment (i, j), row i * 16 + l % 16 (of K) and the 4 columns j * 16 + (l / 16) * 4 ..;
         // 32 rows at a time through 4 KiB of LDS that belong to the wavefront, out by whole 128-byte lines ----
+        behind = false;
+        if (cur_part >= 0) {
+            // a piece: its fp32 sums as they lie in the registers, for wgrad_join_kernel
+            f32x4 *sums = (f32x4 *)p.partials + (((size_t)cur_part * tiles + cur_split_tile) * NW + wave) * (FM * FN * kWave) + lane;
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) sums[(i * FN + j) * kWave] = acc[i][j];
+        } else {
         char *stg = smem + 3 * kStage + wave * 4096;
         // (the rows' addresses as a scalar that moves and one offset per lane: 16 addresses a lane would not stay in registers)
         const bool whole = cur_k0 + BT <= p.K && cur_n0 + BT <= p.N;
@@ -262,21 +290,78 @@ void gmm_wgrad_kernel(const GmmArgs p) {
         }
 
         behind = whole;
+        }
         __syncthreads();                                   // the staged rows have been read back by everyone
         if (q < total) issue_late();
     }
     sched_finish(p.sched, drawer, draw, streams, total);
 }
 
-int launch_wgrad(const GmmArgs &args, hipStream_t stream) {
+// Adds up the pieces of every tile in their order and rounds once: a wavefront per 16 x 64 of the result.
+__global__ __launch_bounds__(256) void wgrad_join_kernel(const GmmArgs p, int kt_n, int nt_n) {
+    constexpr int NW = 8, FM = 8, FN = 4;
+    const long long tiles = (long long)p.E * kt_n * nt_n;
+    const long long id = (long long)blockIdx.x * 4 + threadIdx.x / kWave;
+    const int lane = threadIdx.x & (kWave - 1), l16 = lane & 15, g16 = lane >> 4;
+    const int i = (int)(id % FM), wave = (int)(id / FM % NW);
+    const long long tile = id / (FM * NW);
+    if (tile >= tiles) return;
+    f32x4 acc[FN];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const f32x4 *sums = (const f32x4 *)p.partials + ((size_t)tile * NW + wave) * (FM * FN * kWave) + i * FN * kWave + lane;
+    const size_t piece = (size_t)tiles * NW * FM * FN * kWave;
+#pragma unroll 4
+    for (int k = 0; k < p.split; ++k)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[j] += sums[k * piece + j * kWave];
+    // (the tile order of gmm_wgrad_kernel)
+    const int e = (int)(tile / ((long long)kt_n * nt_n));
+    const int idx = (int)(tile - (long long)e * kt_n * nt_n);
+    int k0, n0;
+    wgrad_tile(idx, kt_n, nt_n, k0, n0);
+    const int row = k0 + (wave / 4) * 128 + i * 16 + l16;
+    if (row >= p.K) return;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        const int col = n0 + (wave % 4) * 64 + j * 16 + g16 * 4;
+        if (col >= p.N) continue;                          // N % 8 == 0: 4 columns at once
+        uint2 pk;
+        pk.x = pack_bf16x2(acc[j][0], acc[j][1]);
+        pk.y = pack_bf16x2(acc[j][2], acc[j][3]);
+        *(uint2 *)((uint16_t *)p.c + ((size_t)e * p.K + row) * p.N + col) = pk;
+    }
+}
+
+// A launch whose tiles fill half of the compute units at most cuts their contractions into pieces that fill them, of 8 stages
+// (256 rows) or more for an expert of average size, as the workspace has room for.  Joining them is a second, short launch:
+// with the pieces counted in and added up by whichever comes last, one compute unit read all pieces of a tile past the caches
+// and that took longer than the whole contraction (2 experts of 4096 rows, 512 x 1024: 89 us, 47 us uncut).
+static int wgrad_split(const GmmArgs &args, long long tiles, long long cus) {
+    if (args.arrive == nullptr || tiles * 2 > cus) return 1;
+    const long long room = args.partial_bytes / (256 * 256 * (long long)sizeof(float)), stages = args.rows / ((long long)args.E * kDK);
+    long long most = cus / tiles;
+    most = most < stages / 8 ? most : stages / 8;
+    most = most < room / tiles ? most : room / tiles;
+    return most < 2 ? 1 : (int)most;
+}
+
+int launch_wgrad(const GmmArgs &given, hipStream_t stream) {
     constexpr int lds = 4 * 2 * 256 * kDK * 2;
     static unsigned long long configured = 0;   // devices on which the kernel's LDS size has been raised
     DMOE_HIP(raise_dynamic_lds((const void *)gmm_wgrad_kernel, lds, &configured));
-    const long long tiles = (long long)args.E * ((args.K + 255) / 256) * ((args.N + 255) / 256);
-    const long long cus = device_cus();
-    const long long grid = ((tiles < cus ? tiles : cus) + kXcds - 1) / kXcds * kXcds;
+    GmmArgs args = given;
+    const int kt_n = (args.K + 255) / 256, nt_n = (args.N + 255) / 256;
+    const long long tiles = (long long)args.E * kt_n * nt_n, cus = device_cus();
+    args.split = wgrad_split(args, tiles, cus);
+    const long long items = tiles * args.split;
+    const long long grid = ((items < cus ? items : cus) + kXcds - 1) / kXcds * kXcds;
     hipLaunchKernelGGL(gmm_wgrad_kernel, dim3((unsigned)grid), dim3(512), lds, stream, args);
     DMOE_LAUNCH_CHECK("gmm_wgrad_kernel");
+    if (args.split > 1) {
+        hipLaunchKernelGGL(wgrad_join_kernel, dim3((unsigned)(tiles * 16)), dim3(256), 0, stream, args, kt_n, nt_n);
+        DMOE_LAUNCH_CHECK("wgrad_join_kernel");
+    }
     return DMOE_OK;
 }
 

@@ -125,6 +125,28 @@ def test_wgrad_many_experts_and_long_contraction():
     _check_wgrad(gg.gmm_wgrad(a, dc, sizes), a, dc, sizes)
 
 
+@pytest.mark.parametrize("sizes", [[1024], [3001], [1700, 0, 900], [4000, 37], [0, 20000, 1, 0]], ids=str)
+@pytest.mark.parametrize("K,N", [(8, 264), (264, 512)])
+def test_wgrad_of_few_tiles(sizes, K, N):
+    announce(test="wgrad_few_tiles", sizes=sizes, K=K, N=N)
+    # contractions that are cut in pieces: pieces of any length, experts without rows, the same bits every time, and a state
+    # block that every launch leaves clean
+    sizes = torch.tensor(sizes)
+    R = int(sizes.sum())
+    a, dc = _rand((R, K), R + 1), _rand((R, N), R + 2)
+    size, ptr = gg.get_arguments(len(sizes), dev())
+    own = dict(arguments_ptr=ptr, workspace=torch.empty(size, dtype=torch.uint8, device=dev()).fill_(255))
+    db = gg.gmm_wgrad(a, dc, sizes, **own)
+    _check_wgrad(db, a, dc, sizes)
+    for _ in range(3):
+        assert torch.equal(db, gg.gmm_wgrad(a, dc, sizes, **own))
+    _check_wgrad(gg.gmm_wgrad(a, dc, sizes, arguments_ptr=ptr), a, dc, sizes)      # no workspace: nothing is cut
+    small = own["workspace"][:3 * 256 * 256 * 4]
+    _check_wgrad(gg.gmm_wgrad(a, dc, sizes, arguments_ptr=ptr, workspace=small), a, dc, sizes)
+    assert not bool(gg._STATE_BLOCKS[ptr].any())
+    gg.release_arguments(ptr)
+
+
 @pytest.mark.parametrize("trans_b", [False, True])
 @pytest.mark.parametrize("E,R,K,I", [(1, 1, 8, 8), (3, 50, 64, 40), (4, 300, 256, 128), (6, 900, 264, 328), (5, 1500, 512, 136),
                                      (64, 500, 128, 96), (2, 700, 1024, 256)])
