@@ -376,14 +376,13 @@ void gmm_tile256_kernel(const GmmArgs p) {
 #pragma unroll
             for (int i2 = 0; i2 < FM / 2; ++i2) {
                 if (kGuard && i2 * 2 >= nfr) break;        // wave-uniform: no valid row from here on
+                if constexpr (KEEP) {
+                    // the sums in whole lines, before the results take the same place: 16 rows of 128 bytes of the gate columns,
+                    // then of the up columns, through the wavefront's 4 KiB, the 16-byte chunk c of row r at c ^ (r & 7)
+                    char *keep = smem + (cur_S % kStages) * kStage + wave * 4096;
 #pragma unroll
-                for (int ii = 0; ii < 2; ++ii) {
-                    const int i = i2 * 2 + ii;
-                    const int row = ii * 16 + l16;
-                    if constexpr (KEEP) {
-                        // the sums in whole lines: 16 rows of 128 bytes of the gate columns, then of the up columns, through
-                        // the wavefront's 4 KiB, the 16-byte chunk c of row r at c ^ (r & 7)
-                        char *keep = smem + (cur_S % kStages) * kStage + wave * 4096;
+                    for (int ii = 0; ii < 2; ++ii) {
+                        const int i = i2 * 2 + ii;
 #pragma unroll
                         for (int j = 0; j < FN; ++j)
                             *(f32x4 *)(keep + (j / FNO) * 2048 + l16 * 128 + ((((j % FNO) * 4 + g16) ^ (l16 & 7)) << 4)) = acc[i][j];
@@ -396,6 +395,11 @@ void gmm_tile256_kernel(const GmmArgs p) {
                                 __builtin_nontemporal_store(val, (f32x4 *)(p.u + (long long)(cur_row0 + r) * p.N + (q >> 1) * n_out + col));
                         }
                     }
+                }
+#pragma unroll
+                for (int ii = 0; ii < 2; ++ii) {
+                    const int i = i2 * 2 + ii;
+                    const int row = ii * 16 + l16;
                     if constexpr (HALF) {
                         // rows and columns outside the tile read a valid neighbour's scale; their results are never stored
                         const int r = wm * TM + i * 16 + l16;

@@ -171,6 +171,42 @@ def test_gated_block(E, R, K, I, trans_b):
     assert torch.equal(fused, y) and not fused.requires_grad     # the same sums, kept or not
 
 
+@pytest.fixture
+def default_tile():
+    yield
+    gg.set_tile_variant(0)
+
+
+@pytest.mark.parametrize("trans_b", [False, True])
+@pytest.mark.parametrize("variant", range(1, 9))
+def test_gated_block_on_every_tile(variant, trans_b, default_tile):
+    announce(test="gated_block_tiles", variant=variant, trans_b=trans_b)
+    # tiles full of rows and tiles with a few, columns that end inside one, more than one k-stage
+    E, K, I = 4, 160, 328
+    sizes = torch.tensor([600, 0, 17, 303])
+    R = 920
+    gg.set_tile_variant(variant)
+    a, b, dh = _rand((R, K), 1), _rand((E, K, 2 * I), 2, 1.0 / K ** 0.5), _rand((R, I), 3)
+    bl = b.transpose(1, 2).contiguous() if trans_b else b
+    h, u = gg.gmm_swiglu_keep(a, bl, sizes, trans_b=trans_b)
+    da, db = gg.gmm_swiglu_backward(dh, u, a, bl, sizes, trans_b=trans_b)
+    _check_block(u, h, da, db.transpose(1, 2) if trans_b else db, a, b, dh, sizes)
+    if not (variant == 8 and not trans_b):                       # (that hook's own kernel keeps nothing: other sums)
+        assert torch.equal(h, gg.gmm_swiglu(a, bl, sizes, trans_b=trans_b))
+
+
+def test_gated_block_that_fills_the_chip():
+    announce(test="gated_block_large")
+    E, K, I, R = 3, 96, 4104, 2300
+    sizes = torch.tensor([1000, 5, 1295])
+    a, b, dh = _rand((R, K), 1), _rand((E, K, 2 * I), 2, 1.0 / K ** 0.5), _rand((R, I), 3)
+    for host in (None, sizes):
+        h, u = gg.gmm_swiglu_keep(a, b, sizes.to(dev()), host_batch_sizes=host)
+        da, db = gg.gmm_swiglu_backward(dh, u, a, b, sizes.to(dev()), host_batch_sizes=host)
+        _check_block(u, h, da, db, a, b, dh, sizes)
+        assert torch.equal(h, gg.gmm_swiglu(a, b, sizes.to(dev()), host_batch_sizes=host))
+
+
 def test_gated_block_where_the_gate_saturates():
     announce(test="gated_block_saturated")
     # gates from -200 to 200: exp(-g) leaves the range of fp32, the sigmoid is 0 or 1 to the last bit
