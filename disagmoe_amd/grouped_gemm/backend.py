@@ -271,15 +271,21 @@ def gmm_swiglu_backward(dh: torch.Tensor, u: torch.Tensor, a: torch.Tensor, b: t
     assert dh.shape == (rows, inter) and u.shape == (rows, 2 * inter), "dh is [rows, I], u is [rows, 2I]"
     assert dh.dtype == torch.bfloat16 and u.dtype == torch.float32 and dh.device == device and u.device == device
     assert dh.is_contiguous() and u.is_contiguous()
-    du = torch.empty((rows, 2 * inter), dtype=torch.bfloat16, device=device)
+    bs = _sizes_on_device(batch_sizes, device)
+    return _swiglu_backward(dh, u, a, b, bs, trans_b, need_da, need_db,
+                            _state_args(device, workspace, arguments_ptr, _stream(device), _host_sizes(batch_sizes, host_batch_sizes)))
+
+
+def _swiglu_backward(dh, u, a, b, bs, trans_b: bool, need_da: bool, need_db: bool, state_args: tuple):
+    """:func:`gmm_swiglu_backward` on operands that have been checked."""
+    (rows, K), two_i = a.shape, u.shape[1]
+    du = torch.empty((rows, two_i), dtype=torch.bfloat16, device=a.device)
     da = torch.empty_like(a) if need_da else None
     db = torch.empty_like(b) if need_db else None
-    bs = _sizes_on_device(batch_sizes, device)
-    with torch.cuda.device(device):
+    with torch.cuda.device(a.device):
         _lib.call("dmoe_gmm_swiglu_backward", dh.data_ptr(), u.data_ptr(), a.data_ptr(), b.data_ptr(), du.data_ptr(),
-                  da.data_ptr() if need_da else None, db.data_ptr() if need_db else None, bs.data_ptr(), rows, E, K, inter,
-                  1 if trans_b else 0, _lib.BF16, *_state_args(device, workspace, arguments_ptr, _stream(device),
-                               _host_sizes(batch_sizes, host_batch_sizes)))
+                  da.data_ptr() if need_da else None, db.data_ptr() if need_db else None, bs.data_ptr(), rows, b.shape[0], K, two_i // 2,
+                  1 if trans_b else 0, _lib.BF16, *state_args)
     return da, db
 
 
@@ -293,13 +299,31 @@ def gmm_wgrad(a: torch.Tensor, dc: torch.Tensor, batch_sizes: torch.Tensor, work
     assert a.dim() == 2 and dc.dim() == 2 and a.shape[0] == dc.shape[0], "a is [rows, K], dc is [rows, N]"
     assert a.dtype == torch.bfloat16 and dc.dtype == torch.bfloat16 and a.device == dc.device
     assert a.is_contiguous() and dc.is_contiguous()
-    E, (rows, K), N, device = batch_sizes.numel(), a.shape, dc.shape[1], a.device
-    db = torch.empty((E, K, N), dtype=a.dtype, device=device)
-    bs = _sizes_on_device(batch_sizes, device)
-    with torch.cuda.device(device):
-        _lib.call("dmoe_gmm_wgrad", a.data_ptr(), dc.data_ptr(), db.data_ptr(), bs.data_ptr(), rows, E, K, N, _lib.BF16,
-                  *_state_args(device, workspace, arguments_ptr, _stream(device), _host_sizes(batch_sizes, host_batch_sizes)))
+    return _wgrad(a, dc, _sizes_on_device(batch_sizes, a.device),
+                  _state_args(a.device, workspace, arguments_ptr, _stream(a.device), _host_sizes(batch_sizes, host_batch_sizes)))
+
+
+def _wgrad(a, dc, bs, state_args: tuple) -> torch.Tensor:
+    """:func:`gmm_wgrad` on operands that have been checked."""
+    E, (rows, K), N = bs.numel(), a.shape, dc.shape[1]
+    db = torch.empty((E, K, N), dtype=a.dtype, device=a.device)
+    with torch.cuda.device(a.device):
+        _lib.call("dmoe_gmm_wgrad", a.data_ptr(), dc.data_ptr(), db.data_ptr(), bs.data_ptr(), rows, E, K, N, _lib.BF16, *state_args)
     return db
+
+
+def _gmm_backward(dc, a, b, bs, trans_b: bool, need_da: bool, need_db: bool, state_args: tuple):
+    """The gradients ``(da, db)`` of :func:`gmm`'s operands; rows of ``da`` past ``sum(batch_sizes)`` are zero."""
+    da = db = None
+    if need_da:
+        da = torch.empty_like(a)
+        with torch.cuda.device(a.device):
+            _lib.call("dmoe_gmm", dc.data_ptr(), b.data_ptr(), da.data_ptr(), bs.data_ptr(), a.shape[0], b.shape[0], dc.shape[1], a.shape[1],
+                      0 if trans_b else 1, _lib.BF16, *state_args)
+        zero_rows_behind(da, bs)
+    if need_db:
+        db = _wgrad(dc, a, bs, state_args) if trans_b else _wgrad(a, dc, bs, state_args)
+    return da, db
 
 
 def zero_rows_behind(c: torch.Tensor, batch_sizes: torch.Tensor) -> torch.Tensor:

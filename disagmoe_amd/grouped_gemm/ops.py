@@ -23,25 +23,35 @@ def _on_device(batch_sizes: torch.Tensor, host_batch_sizes: Optional[torch.Tenso
     return backend._sizes_on_device(batch_sizes, device), backend._host_sizes(batch_sizes, host_batch_sizes)
 
 
+def _remember(ctx, device: torch.device, host: Optional[torch.Tensor], trans_b: bool, state: dict) -> None:
+    """What the backward launches take besides the saved tensors, and what has to live until then: the engine runs them on
+    the forward pass's stream, in a thread of its own where a statement costs several times what it costs here."""
+    ctx.trans_b = trans_b
+    ctx.state_args = backend._state_args(device, state["workspace"], state["arguments_ptr"], backend._stream(device), host)
+    ctx.alive = (host, state["workspace"], backend._STATE_BLOCKS.get(state["arguments_ptr"]))
+
+
+def _check_capture(ctx) -> None:
+    if ctx.alive[2] is None and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("a backward pass recorded into a graph needs a state block of its own: pass the arguments_ptr of "
+                           "get_arguments() (and a workspace) to the forward call")
+
+
 class _Gmm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, a, b, sizes, host, trans_b, state):
         ctx.save_for_backward(a, b, sizes)
-        ctx.host, ctx.trans_b, ctx.state = host, trans_b, state
-        return backend.zero_rows_behind(backend.gmm(a, b, sizes, trans_b=trans_b, host_batch_sizes=host, **state), sizes)
+        c = backend.zero_rows_behind(backend.gmm(a, b, sizes, trans_b=trans_b, host_batch_sizes=host, **state), sizes)
+        _remember(ctx, a.device, host, trans_b, state)
+        return c
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dc):
+        _check_capture(ctx)
         a, b, sizes = ctx.saved_tensors
-        more = dict(ctx.state, host_batch_sizes=ctx.host)
-        dc = dc.contiguous()
-        da = db = None
-        if ctx.needs_input_grad[0]:
-            da = backend.zero_rows_behind(backend.gmm(dc, b, sizes, trans_b=not ctx.trans_b, **more), sizes)
-        if ctx.needs_input_grad[1]:
-            db = backend.gmm_wgrad(dc, a, sizes, **more) if ctx.trans_b else backend.gmm_wgrad(a, dc, sizes, **more)
-        return da, db, None, None, None, None
+        return (*backend._gmm_backward(dc.contiguous(), a, b, sizes, ctx.trans_b, ctx.needs_input_grad[0], ctx.needs_input_grad[1],
+                                       ctx.state_args), None, None, None, None)
 
 
 class _GmmSwiglu(torch.autograd.Function):
@@ -49,16 +59,16 @@ class _GmmSwiglu(torch.autograd.Function):
     def forward(ctx, a, b, sizes, host, trans_b, state):
         h, u = backend.gmm_swiglu_keep(a, b, sizes, trans_b=trans_b, host_batch_sizes=host, **state)
         ctx.save_for_backward(a, b, sizes, u)
-        ctx.host, ctx.trans_b, ctx.state = host, trans_b, state
+        _remember(ctx, a.device, host, trans_b, state)
         return h
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dh):
+        _check_capture(ctx)
         a, b, sizes, u = ctx.saved_tensors
-        da, db = backend.gmm_swiglu_backward(dh.contiguous(), u, a, b, sizes, trans_b=ctx.trans_b, need_da=ctx.needs_input_grad[0],
-                                             need_db=ctx.needs_input_grad[1], host_batch_sizes=ctx.host, **ctx.state)
-        return da, db, None, None, None, None
+        return (*backend._swiglu_backward(dh.contiguous(), u, a, b, sizes, ctx.trans_b, ctx.needs_input_grad[0], ctx.needs_input_grad[1],
+                                          ctx.state_args), None, None, None, None)
 
 
 def gmm(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor, trans_b: bool = False,

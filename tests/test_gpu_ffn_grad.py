@@ -370,6 +370,23 @@ def test_step_in_a_graph_beside_eager_steps():
     gg.release_arguments(ptr)
 
 
+def test_backward_after_the_layer_is_gone():
+    announce(test="layer_gone")
+    # the state block and the sizes that a backward pass needs live as long as its graph
+    sizes = torch.tensor([40, 24])
+    x, dy = _rand((64, 128), 1), _rand((64, 128), 2)
+    layer = MoEExperts(128, 64, 2, init_std=0.1, device=dev()).requires_grad_()
+    want_x = x.clone().requires_grad_()
+    layer.forward_train(64, want_x, sizes).backward(dy)
+    got_x = x.clone().requires_grad_()
+    y = layer.forward_train(64, got_x, sizes.clone(), host_batch_sizes=sizes.clone())
+    ptr = layer.arguments_ptr
+    del layer
+    assert ptr not in gg._STATE_BLOCKS
+    y.backward(dy)
+    assert torch.equal(want_x.grad, got_x.grad)
+
+
 def test_another_stream():
     announce(test="step_stream")
     sizes = torch.tensor([90, 30])
