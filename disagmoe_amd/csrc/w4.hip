@@ -80,10 +80,11 @@ __global__ __launch_bounds__(kWave) void w4_quant_kernel(const uint16_t *__restr
 //   HALF true:  out = fp16((q - z) s / f), col_scale[e, n] = f, the power of two below the column's largest scale: the values
 //               are rounded to 11 bits where the 8 of bf16 would show in the product (relative error of the gated form
 //               2.5e-3 instead of 1.7e-3, the rounding of its results alone), and f keeps them in fp16's range.
+// Rows of `out` are Kp >= K long; what lies behind K is some finite value (it meets zeros there, see w4_half_rows_kernel).
 template <bool HALF>
 __global__ __launch_bounds__(256) void w4_widen_kernel(const char *__restrict__ codes, const uint16_t *__restrict__ scales, const uint8_t *__restrict__ zeros,
                                                       uint16_t *__restrict__ out, float *__restrict__ col_scale, const int64_t *__restrict__ batch_sizes,
-                                                      int K, int N, int nt, int kt, int group) {
+                                                      int K, int Kp, int N, int nt, int kt, int group) {
     __shared__ __attribute__((aligned(16))) char stage[4][4096];
     __shared__ uint16_t largest[kW4Cols][16];
     const int lane = lane_id(), r = lane & 15, g16 = lane >> 4, wave = threadIdx.x / kWave;
@@ -136,14 +137,16 @@ __global__ __launch_bounds__(256) void w4_widen_kernel(const char *__restrict__ 
         for (int i = 0; i < 4; ++i) {
             const int row = i * 4 + g16, n = t * kW4Cols + row, k = c * kW4Chunk + r * 8;
             const u32x4 v = *(const u32x4 *)(mine + row * 256 + ((r ^ row) << 4));
-            if (n < N && k < K) __builtin_nontemporal_store(v, (u32x4 *)(out + ((int64_t)e * N + n) * K + k));
+            if (n < N && k < Kp) __builtin_nontemporal_store(v, (u32x4 *)(out + ((int64_t)e * N + n) * Kp + k));
         }
     }
 }
 
 // out = fp16(x / f), row_scale[r] = f, the power of two below the row's largest magnitude: exact but for values 2^14 times
-// smaller than that, which lose what lies below 2^-24 of it.  One workgroup per row.
-__global__ __launch_bounds__(256) void w4_half_rows_kernel(const u32x4 *__restrict__ x, u32x4 *__restrict__ out, float *__restrict__ row_scale, int vecs) {
+// smaller than that, which lose what lies below 2^-24 of it.  Rows of `out` are out_vecs >= vecs long, zeros behind the
+// values.  One workgroup per row.
+__global__ __launch_bounds__(256) void w4_half_rows_kernel(const u32x4 *__restrict__ x, u32x4 *__restrict__ out, float *__restrict__ row_scale, int vecs,
+                                                          int out_vecs) {
     __shared__ uint32_t part[4];
     const int64_t row = blockIdx.x;
     uint32_t most = 0;
@@ -169,15 +172,16 @@ __global__ __launch_bounds__(256) void w4_half_rows_kernel(const u32x4 *__restri
     exponent = exponent < 1 ? 127 : (exponent > 253 ? 253 : exponent);       // a row of zeros: 1; not finite: it stays so
     const float inv = __uint_as_float((uint32_t)(254 - exponent) << 23);
     if (threadIdx.x == 0) row_scale[row] = __uint_as_float((uint32_t)exponent << 23);
-    for (int i = threadIdx.x; i < vecs; i += 256) {
-        const u32x4 v = x[row * vecs + i];
+    for (int i = threadIdx.x; i < out_vecs; i += 256) {
+        u32x4 v = {0, 0, 0, 0};
+        if (i < vecs) v = x[row * vecs + i];
         u32x4 o;
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
             typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
             o[p] = __builtin_bit_cast(uint32_t, (f16x2{(_Float16)(__uint_as_float(v[p] << 16) * inv), (_Float16)(__uint_as_float(v[p] & 0xffff0000u) * inv)}));
         }
-        out[row * vecs + i] = o;
+        out[row * out_vecs + i] = o;
     }
 }
 
@@ -198,7 +202,9 @@ static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 struct WideLayout {
     size_t weights, col_scales, rows, row_scales, bytes;
 };
-static WideLayout wide_layout(int64_t rows, int E, int64_t K, int64_t N) {
+static int64_t wide_k(int64_t K) { return (K + 31) / 32 * 32; }   // whole stages of the 256-row tile
+static WideLayout wide_layout(int64_t rows, int E, int64_t K_given, int64_t N) {
+    const int64_t K = wide_k(K_given);
     WideLayout w;
     w.weights = 0;
     w.col_scales = up256((size_t)E * N * K * 2);
@@ -228,7 +234,7 @@ static W4Form choose_w4(int64_t rows, int E, int64_t K, int64_t N, int group, co
     if (busy < 1) busy = 1;
     const long long avg = (rows + busy - 1) / busy;
     W4Form f;
-    f.wide = avg > wide_rows(group) && K % 32 == 0 && K * N * 2 < (1ll << 32);   // (what the 256-row tile takes)
+    f.wide = avg > wide_rows(group) && wide_k(K) * N * 2 < (1ll << 32);   // (what the 256-row tile takes)
     f.tile_rows = avg <= 16 ? 16 : (avg <= 32 ? 32 : 64);
     // row tiles: those of the sizes, or at most one short one for every expert with rows
     long long m = rows / f.tile_rows + (E < rows ? E : rows);
@@ -263,16 +269,18 @@ static int gmm_w4(const char *who, const void *a, const void *codes, const void 
     const WideLayout at = wide_layout(rows, E, K, N);
     if (f.wide && wide != nullptr && wide_bytes >= at.bytes) {
         char *w = (char *)wide;
+        const int64_t Kp = wide_k(K);
         const int nt = tiles_of(N, kW4Cols), kt = tiles_of(K, kW4Chunk);
         hipLaunchKernelGGL(w4_widen_kernel<true>, dim3(nt, E), dim3(256), 0, (hipStream_t)stream, (const char *)codes, (const uint16_t *)scales,
-                           (const uint8_t *)zeros, (uint16_t *)(w + at.weights), (float *)(w + at.col_scales), batch_sizes, (int)K, (int)N, nt, kt, group);
+                           (const uint8_t *)zeros, (uint16_t *)(w + at.weights), (float *)(w + at.col_scales), batch_sizes, (int)K, (int)Kp, (int)N, nt, kt,
+                           group);
         DMOE_LAUNCH_CHECK("w4_widen_kernel");
         hipLaunchKernelGGL(w4_half_rows_kernel, dim3((unsigned)rows), dim3(256), 0, (hipStream_t)stream, (const u32x4 *)a, (u32x4 *)(w + at.rows),
-                           (float *)(w + at.row_scales), (int)(K / 8));
+                           (float *)(w + at.row_scales), (int)(K / 8), (int)(Kp / 8));
         DMOE_LAUNCH_CHECK("w4_half_rows_kernel");
         const HostSizes known(host_batch_sizes);
         GmmArgs args{w + at.rows, w + at.weights, (char *)c, batch_sizes, (const float *)(w + at.row_scales), (const float *)(w + at.col_scales), rows, E,
-                     (int)K, (int)N, (int)n_out};
+                     (int)Kp, (int)N, (int)n_out};
         rc = bind_state(args, state, workspace, workspace_bytes, (hipStream_t)stream);
         return rc != DMOE_OK ? rc : launch_tile256_half(args, swiglu, (hipStream_t)stream);
     }
@@ -320,7 +328,7 @@ extern "C" int dmoe_w4_dequant(const void *codes, const void *scales, const void
     DMOE_REQUIRE(aligned(codes, 16) && aligned(scales, 16) && aligned(out, 16), DMOE_ERR_ARG, "dmoe_w4_dequant: a pointer is not 16-byte aligned");
     const int nt = tiles_of(N, kW4Cols), kt = tiles_of(K, kW4Chunk);
     hipLaunchKernelGGL(w4_widen_kernel<false>, dim3(nt, E), dim3(256), 0, (hipStream_t)stream, (const char *)codes, (const uint16_t *)scales,
-                       (const uint8_t *)zeros, (uint16_t *)out, (float *)nullptr, batch_sizes, (int)K, (int)N, nt, kt, group);
+                       (const uint8_t *)zeros, (uint16_t *)out, (float *)nullptr, batch_sizes, (int)K, (int)K, (int)N, nt, kt, group);
     DMOE_LAUNCH_CHECK("w4_widen_kernel");
     return DMOE_OK;
 }

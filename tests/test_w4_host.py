@@ -33,7 +33,7 @@ def test_host_side_argument_errors():
     up = lambda n: -(-n // 256) * 256                             # weights, their scales, rows, their scales
     wide = lambda rows: up(8 * 64 * 64 * 2) + up(8 * 64 * 4) + up(rows * 64 * 2) + up(rows * 4)
     assert lib.dmoe_gmm_w4_wide_bytes(1 << 20, 8, 64, 64, 128, None, ctypes.byref(need)) == 0 and need.value == wide(1 << 20)
-    assert lib.dmoe_gmm_w4_wide_bytes(1 << 20, 8, 72, 64, 128, None, ctypes.byref(need)) == 0 and need.value == 0     # K % 32
+    assert lib.dmoe_gmm_w4_wide_bytes(1 << 20, 8, 40, 64, 128, None, ctypes.byref(need)) == 0 and need.value == wide(1 << 20)  # K up to 32s
     sizes = (ctypes.c_int64 * 8)(*([0] * 7 + [4000]))             # one expert has all the rows
     assert lib.dmoe_gmm_w4_wide_bytes(4000, 8, 64, 64, 128, sizes, ctypes.byref(need)) == 0 and need.value == wide(4000)
     assert lib.dmoe_gmm_w4_wide_bytes(-1, 8, 64, 64, 128, None, ctypes.byref(need)) == _lib.ERR_ARG
