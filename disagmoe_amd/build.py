@@ -15,7 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_PATH = os.path.join(HERE, "libdmoe_hip.so")
 SOURCES = ["gmm_wave128_fp8.hip", "gmm_wave128.hip", "gmm_tile256.hip", "gmm_tile256_fp8.hip", "gmm_direct_bf16.hip", "gmm_direct_bf16_small.hip", "gmm_direct_fp8.hip", "gmm.hip", "route.hip", "topk.hip", "rows.hip",
-           "meta.hip", "grads.hip", "swiglu.hip", "gmm_wgrad.hip", "gmm_keep.hip", "gmm_half.hip", "w4_rows16.hip", "w4_rows32.hip", "w4_rows64.hip", "w4.hip"]
+           "meta.hip", "grads.hip", "swiglu.hip", "gmm_wgrad.hip", "gmm_keep.hip", "gmm_tail.hip", "gmm_half.hip", "w4_rows16.hip", "w4_rows32.hip", "w4_rows64.hip", "w4.hip"]
 ARCH = "gfx950"
 
 FLAGS = [

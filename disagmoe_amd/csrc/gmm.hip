@@ -566,10 +566,21 @@ static int launch_by_rows(const GmmArgs &args, hipStream_t stream) {
     else return launch_direct_bf16(args, L.tile_rows, TRANS_B, SWIGLU, stream);
 }
 
+// Contractions that end inside a stage, in the gated block's training: the 256-row tile with its last stage filled up with
+// zeros, where the experts have 256 rows and more on average and tiles of that height are chosen; below, the register-staged
+// kernel and its smaller tiles.  Forward / backward in us, staged -> this (K, I both no multiple of 32): 8 experts of 2048
+// rows, 4104 x 5000: 1654 / 3386 -> 1369 / 3019; of 512 rows, 4104 x 2056: 323 / 505 -> 284 / 508; of 256 rows, 1000 x 1000
+// (128-row tiles): 40 / 72 against 43 / 106; 64 experts of 32 rows, weights [N, K]: 61 against 83 forward.
+static bool takes_tail(const GmmArgs &args, const GmmLaunch &L) {
+    return L.kernel == kKernelStaged && g_variant == 0 && L.tile_rows == 256 && args.K % 32 != 0 && args.rows >= 256ll * args.E &&
+           (long long)args.K * args.N * 2 < (1ll << 32);
+}
+
 // The gated form that also leaves its fp32 sums in args.u.
 template <bool TRANS_B>
 static int launch_keep(const GmmArgs &args, hipStream_t stream) {
     GmmLaunch L = choose_launch(args, TRANS_B, true, false);
+    if (takes_tail(args, L)) return launch_tile256_tail(args, TRANS_B, true, stream);
     if (L.kernel == kKernelStaged) {
         if (L.tile_rows == 64) return launch_one<64, 256, 1, 4, TRANS_B, true, false, true>(args, stream);
         if (L.tile_rows == 128) return launch_one<128, 256, 1, 4, TRANS_B, true, false, true>(args, stream);
@@ -741,8 +752,15 @@ extern "C" int dmoe_gmm_swiglu_backward(const void *dh, const float *u, const vo
     if (rows > 0) {
         DMOE_REQUIRE(du != (const void *)u && du != dh && da != dh && da != a, DMOE_ERR_ARG, "dmoe_gmm_swiglu_backward: a result overlaps an input");
         rc = launch_swiglu_backward(dh, u, du, batch_sizes, rows, E, I, da, K, (hipStream_t)stream);
-        if (rc == DMOE_OK && da != nullptr)
-            rc = dmoe_gmm(du, b, da, batch_sizes, rows, E, 2 * I, K, !trans_b, dtype, state, workspace, workspace_bytes, host_batch_sizes, stream);
+        if (rc == DMOE_OK && da != nullptr) {
+            const HostSizes known(host_batch_sizes);
+            GmmArgs args{(const char *)du, (const char *)b, (char *)da, batch_sizes, nullptr, nullptr, rows, E, (int)(2 * I), (int)K, (int)K};
+            rc = bind_state(args, state, workspace, workspace_bytes, (hipStream_t)stream);
+            if (rc == DMOE_OK && takes_tail(args, choose_launch(args, !trans_b, false, false)))
+                rc = launch_tile256_tail(args, !trans_b, false, (hipStream_t)stream);
+            else if (rc == DMOE_OK)
+                rc = trans_b ? launch_by_rows<false, false, false>(args, (hipStream_t)stream) : launch_by_rows<true, false, false>(args, (hipStream_t)stream);
+        }
     }
     if (rc != DMOE_OK || db == nullptr) return rc;
     return trans_b ? dmoe_gmm_wgrad(du, a, db, batch_sizes, rows, E, 2 * I, K, dtype, state, workspace, workspace_bytes, host_batch_sizes, stream)

@@ -373,6 +373,7 @@ int launch_wave128(const GmmArgs &args, bool swiglu, hipStream_t stream);
 int launch_wave128_fp8(const GmmArgs &args, bool swiglu, hipStream_t stream);
 int launch_tile256_rows(const GmmArgs &args, hipStream_t stream);
 int launch_wgrad(const GmmArgs &args, hipStream_t stream);
+int launch_tile256_tail(const GmmArgs &args, bool trans_b, bool keep, hipStream_t stream);
 int launch_tile256_half(const GmmArgs &args, bool swiglu, hipStream_t stream);
 int bind_state(GmmArgs &args, void *state, void *workspace, size_t workspace_bytes, hipStream_t stream);
 // The caller's copy of the sizes on the host for the length of one call.

@@ -32,7 +32,9 @@ namespace dmoe {
 // wait would also be one for the epilogue's stores.
 // KEEP (gated form): the fp32 sums also go to p.u, for the activation's gradient.
 // HALF (trans_b): fp16 operands whose rows and columns carry fp32 scales, c = (a @ b[e]^T) a_scale[r] b_scale[e, n] in bf16.
-template <bool TRANS_B, bool SWIGLU, bool GATHER = false, bool KEEP = false, bool HALF = false>
+// TAIL: K is no multiple of 32; the last stage reaches past it.  What lies there (the next row, the next expert, nothing) is not
+// read: such lanes copy the stage's first k again, and write zeros over it once it has landed, in both operands.
+template <bool TRANS_B, bool SWIGLU, bool GATHER = false, bool KEEP = false, bool HALF = false, bool TAIL = false>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void gmm_tile256_kernel(const GmmArgs p) {
     constexpr int kDM = 256, NW = 8, WN = 4;
@@ -48,6 +50,7 @@ void gmm_tile256_kernel(const GmmArgs p) {
     constexpr int kStages = 4;
     constexpr int BNO = SWIGLU ? kDN / 2 : kDN;
     static_assert(!KEEP || SWIGLU, "only the gated form has something to keep");
+    static_assert(!TAIL || (!GATHER && !HALF), "rows fetched by number and fp16 operands have whole stages");
     static_assert(!HALF || (TRANS_B && !KEEP && !GATHER), "fp16 operands are K-contiguous");
     static_assert(CA == 2 && CB == 2 && (kStages - 1) * kLoads <= 63, "copies per stage");
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -66,7 +69,8 @@ void gmm_tile256_kernel(const GmmArgs p) {
 
     const int n_out = SWIGLU ? p.N / 2 : p.N;
     const int n_tiles = (n_out + BNO - 1) / BNO;
-    const int S_all = p.K / kDK;
+    const int S_all = TAIL ? (p.K + kDK - 1) / kDK : p.K / kDK;
+    const int k_tail = TAIL ? p.K - (S_all - 1) * kDK : kDK;   // k of the last stage
     const int G = gridDim.x;
     constexpr long long kPieceBytes = (long long)kDM * kDN * sizeof(float);
     const WorkPlan plan = plan_work((long long)s_tile_start[E] * n_tiles, G, S_all,
@@ -167,9 +171,28 @@ void gmm_tile256_kernel(const GmmArgs p) {
         fetch_rows(it);
         open_item(it);
     };
+    // TAIL: whether this lane's piece of block i of the last stage lies past K
+    auto a_past = [&]() { return kc_chunk * 8 >= k_tail; };
+    auto b_past = [&](int i) { return TRANS_B ? a_past() : i * 2 * NW + kn_k >= k_tail; };
     // the kLoads copies of this wavefront for stage s of the item: its CA blocks of A, then its CB blocks of B
     auto issue_copies = [&](int s) {
         const uint32_t lds = smem_addr + (s % kStages) * kStage + wave * 1024;
+        if constexpr (TAIL) {
+            if (s_lo + s == S_all - 1) {
+                const uint64_t a_stage = a_base + (uint64_t)s * 64;
+                const uint64_t b_stage = b_exp + (TRANS_B ? (uint64_t)s * 64 : (uint64_t)s * kDK * p.N * 2);
+                static_for<0, CA>([&](auto c_tag) {
+                    constexpr int c = decltype(c_tag)::value;
+                    copy_g2lds_16<c * kBlock>(a_past() ? a_off[c] - kc_chunk * 16 : a_off[c], to_scalar(a_stage), lds);
+                });
+                static_for<0, CB>([&](auto i_tag) {
+                    constexpr int i = decltype(i_tag)::value;
+                    const uint32_t back = TRANS_B ? kc_chunk * 16 : (uint32_t)(i * 2 * NW + kn_k) * (uint32_t)p.N * 2;
+                    copy_g2lds_16<kStageA + i * kBlock>(b_past(i) ? b_off[i] - back : b_off[i], to_scalar(b_stage), lds);
+                });
+                return;
+            }
+        }
         // (GATHER: the compiler loses track of these wave-uniform addresses being uniform where the next item is
         // located from inside the tile's code; to_scalar costs nothing where it has not)
         const uint64_t a_stage = GATHER ? to_scalar(a_base + (uint64_t)s * 64) : a_base + (uint64_t)s * 64;
@@ -268,7 +291,7 @@ void gmm_tile256_kernel(const GmmArgs p) {
         WorkItem next_item{};                              // GATHER: the next item, located before this one's epilogue
         const int cur_row0 = row0, cur_rows_e = rows_e, cur_n0 = n0;
         const int cur_part = part, cur_split_tile = split_tile, cur_S = S;
-        const int cur_e = e;
+        const int cur_e = e, cur_s_lo = s_lo;
         // 16-row fragments of this wavefront that hold at least one valid row (a short last tile skips the rest)
         int nfr = ((rows_e < kDM ? rows_e : kDM) - wm * TM + 15) / 16;
         nfr = __builtin_amdgcn_readfirstlane(nfr < 0 ? 0 : (nfr > FM ? FM : nfr));
@@ -284,10 +307,25 @@ void gmm_tile256_kernel(const GmmArgs p) {
             for (int i = 0; i < FM; ++i)
 #pragma unroll
                 for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            // TAIL: zeros over what lies past K of stage s, if that is the last of the tile (this lane's own copies, landed)
+            auto clear_past = [&](int s) {
+                if constexpr (TAIL) {
+                    if (cur_s_lo + s != S_all - 1) return;
+                    __builtin_amdgcn_sched_barrier(0);     // behind the wait
+                    char *mine = smem + (s % kStages) * kStage + wave * 1024 + lane * 16;
+#pragma unroll
+                    for (int i = 0; i < CA; ++i)
+                        if (a_past()) *(u32x4 *)(mine + i * kBlock) = u32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int i = 0; i < CB; ++i)
+                        if (b_past(i)) *(u32x4 *)(mine + kStageA + i * kBlock) = u32x4{0, 0, 0, 0};
+                }
+            };
 
             // stage 0 has landed (the other stages of the prologue and stores of the previous epilogue, issued before
             // them, may still be in flight: waiting for fewer is only stricter)
             wait_ahead(pre - 1);
+            clear_past(0);
             __syncthreads();
             // The slot of stage s - 1 is free once every wavefront has read that stage, i.e. behind the barrier that
             // closes the memory phase of the late half; from then on (memory phases of stage s) it is refilled with
@@ -297,7 +335,10 @@ void gmm_tile256_kernel(const GmmArgs p) {
                 constexpr bool kRefill = decltype(refill_tag)::value;
                 auto landed = [&]() {
                     if constexpr (kRefill) DMOE_WAIT_VMCNT((kStages - 2) * kLoads);
-                    else wait_ahead(ahead);
+                    else {
+                        wait_ahead(ahead);
+                        clear_past(s + 1);
+                    }
                 };
                 load_operands(s, kAlt ? FM : nfr);
                 if constexpr (kRefill) issue_copies(s + kStages - 1);
@@ -460,10 +501,10 @@ void gmm_tile256_kernel(const GmmArgs p) {
     sched_finish(p.sched, drawer, draw, streams, total);
 }
 
-template <bool TRANS_B, bool SWIGLU, bool GATHER = false, bool KEEP = false, bool HALF = false>
+template <bool TRANS_B, bool SWIGLU, bool GATHER = false, bool KEEP = false, bool HALF = false, bool TAIL = false>
 static int launch_tile256_one(const GmmArgs &args, hipStream_t stream) {
     const size_t lds = (size_t)4 * (256 * kDK * 2 + kStageB);
-    auto kern = gmm_tile256_kernel<TRANS_B, SWIGLU, GATHER, KEEP, HALF>;
+    auto kern = gmm_tile256_kernel<TRANS_B, SWIGLU, GATHER, KEEP, HALF, TAIL>;
     static unsigned long long configured = 0;   // devices on which the kernel's LDS size has been raised
     DMOE_HIP(raise_dynamic_lds((const void *)kern, (int)lds, &configured));
     const long long grid = launch_grid(args, 256, SWIGLU, kDK, true, device_cus());

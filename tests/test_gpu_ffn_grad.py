@@ -178,6 +178,33 @@ def default_tile():
 
 
 @pytest.mark.parametrize("trans_b", [False, True])
+@pytest.mark.parametrize("sizes,K,I", [([5], 8, 8), ([300, 0, 17], 24, 4), ([70, 1, 256, 257], 40, 300), ([600, 520], 4104, 132),
+                                       ([33], 8200, 4100), ([2000, 0, 1500], 1000, 516), ([900, 700], 56, 2052),
+                                       ([1600, 4000], 40, 2052), ([3000, 40], 4104, 1500), ([5000], 8, 1800)], ids=str)
+def test_contractions_that_end_inside_a_stage(sizes, K, I, trans_b):
+    announce(test="block_tail", sizes=sizes, K=K, I=I, trans_b=trans_b)
+    # K and 2I of any multiple of 8, long ones of few tiles among them (cut into pieces).  The rows, weights and gradients
+    # stand in front of NaN: a k past the end that got into a product would show, as a zero times it would.
+    if I % 8:
+        I += 4
+    E, R, sizes = len(sizes), sum(sizes), torch.tensor(sizes)
+
+    def guarded(*shape, seed, std=1.0):
+        n = 1
+        for s in shape:
+            n *= s
+        buf = torch.full((n + 4096,), float("nan"), device=dev(), dtype=torch.bfloat16)
+        buf[:n] = _rand((n,), seed, std)
+        return buf[:n].view(shape)
+    a, dh = guarded(R, K, seed=1), guarded(R, I, seed=3)
+    w = (2 * I, K) if trans_b else (K, 2 * I)
+    b = guarded(E, *w, seed=2, std=K ** -0.5)
+    h, u = gg.gmm_swiglu_keep(a, b, sizes, trans_b=trans_b)
+    da, db = gg.gmm_swiglu_backward(dh, u, a, b, sizes, trans_b=trans_b)
+    _check_block(u, h, da, db.transpose(1, 2) if trans_b else db, a, b.transpose(1, 2) if trans_b else b, dh, sizes)
+
+
+@pytest.mark.parametrize("trans_b", [False, True])
 @pytest.mark.parametrize("variant", range(1, 9))
 def test_gated_block_on_every_tile(variant, trans_b, default_tile):
     announce(test="gated_block_tiles", variant=variant, trans_b=trans_b)
