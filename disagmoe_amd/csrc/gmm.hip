@@ -744,6 +744,7 @@ extern "C" int dmoe_gmm_swiglu_backward(const void *dh, const float *u, const vo
     DMOE_REQUIRE(dtype == DMOE_BF16, DMOE_ERR_DTYPE, "dmoe_gmm_swiglu_backward: dtype %d (bf16 only)", dtype);
     int rc = check_shape("dmoe_gmm_swiglu_backward", rows, E, K, I, 8);
     if (rc != DMOE_OK) return rc;
+    DMOE_REQUIRE(2 * I < (1ll << 22), DMOE_ERR_SHAPE, "dmoe_gmm_swiglu_backward: 2I=%lld is a contraction length, below 2^22", (long long)(2 * I));
     DMOE_REQUIRE(batch_sizes != nullptr && (da == nullptr || b != nullptr), DMOE_ERR_ARG, "dmoe_gmm_swiglu_backward: null pointer");
     DMOE_REQUIRE(rows == 0 || (dh != nullptr && u != nullptr && du != nullptr && (db == nullptr || a != nullptr)), DMOE_ERR_ARG,
                  "dmoe_gmm_swiglu_backward: null pointer");

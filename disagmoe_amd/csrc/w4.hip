@@ -6,7 +6,7 @@ namespace dmoe {
 // One wavefront packs one tile: lane 16 g + r holds the 32 weights of column r at k = 32 j + 8 g + i, which a group's
 // lanes (4 per column) share the extremes of.  Without zero points s = max |w| / 7 and q = round(w / s) + 8; with them
 // s = (max(w, 0) - min(w, 0)) / 15 and z = round(-min(w, 0) / s), so that a weight of zero stays one.  s is rounded to
-// bf16 first and the codes follow the rounded one.  Bound by its scattered 2-byte reads; weights are packed once.
+// bf16 first and the codes follow the rounded one; one below the normal numbers is 0.  Bound by its scattered 2-byte reads; weights are packed once.
 __global__ __launch_bounds__(kWave) void w4_quant_kernel(const uint16_t *__restrict__ w, char *__restrict__ codes, uint16_t *__restrict__ scales,
                                                         uint8_t *__restrict__ zeros, int K, int N, int nt, int kt, int group) {
     const int lane = lane_id(), r = lane & 15, g16 = lane >> 4;
@@ -49,6 +49,7 @@ __global__ __launch_bounds__(kWave) void w4_quant_kernel(const uint16_t *__restr
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         float s = zeros != nullptr ? (hi[j] - lo[j]) / 15.f : fmaxf(hi[j], -lo[j]) / 7.f;
+        if (s < 0x1p-126f) s = 0.f;                            // (its inverse would not be finite)
         const uint16_t bits = f32_to_bf16(s);
         s = bf16_to_f32(bits);
         const float inv = s > 0.f ? 1.f / s : 0.f;

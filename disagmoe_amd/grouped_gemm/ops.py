@@ -37,6 +37,17 @@ def _check_capture(ctx) -> None:
                            "get_arguments() (and a workspace) to the forward call")
 
 
+def _check_aligned(a: torch.Tensor, b: torch.Tensor) -> None:
+    if (a.data_ptr() | b.data_ptr()) & 15:
+        raise ValueError("a and b must be 16-byte aligned")
+
+
+def _gradient(dc: torch.Tensor) -> torch.Tensor:
+    """The gradient as the kernels read it, whatever view of other memory it arrived as."""
+    dc = dc.contiguous()
+    return dc.clone() if dc.data_ptr() & 15 else dc
+
+
 class _Gmm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, a, b, sizes, host, trans_b, state):
@@ -50,7 +61,7 @@ class _Gmm(torch.autograd.Function):
     def backward(ctx, dc):
         _check_capture(ctx)
         a, b, sizes = ctx.saved_tensors
-        return (*backend._gmm_backward(dc.contiguous(), a, b, sizes, ctx.trans_b, ctx.needs_input_grad[0], ctx.needs_input_grad[1],
+        return (*backend._gmm_backward(_gradient(dc), a, b, sizes, ctx.trans_b, ctx.needs_input_grad[0], ctx.needs_input_grad[1],
                                        ctx.state_args), None, None, None, None)
 
 
@@ -67,7 +78,7 @@ class _GmmSwiglu(torch.autograd.Function):
     def backward(ctx, dh):
         _check_capture(ctx)
         a, b, sizes, u = ctx.saved_tensors
-        return (*backend._swiglu_backward(dh.contiguous(), u, a, b, sizes, ctx.trans_b, ctx.needs_input_grad[0], ctx.needs_input_grad[1],
+        return (*backend._swiglu_backward(_gradient(dh), u, a, b, sizes, ctx.trans_b, ctx.needs_input_grad[0], ctx.needs_input_grad[1],
                                           ctx.state_args), None, None, None, None)
 
 
@@ -77,6 +88,7 @@ def gmm(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor, trans_b: bo
     """Differentiable ``backend.gmm``: ``c[o_e:o_e+n_e] = a[o_e:o_e+n_e] @ b[e]`` (``b[e].T`` with
     ``trans_b``), bf16 in and out."""
     backend._check_operands(a, b, torch.bfloat16)
+    _check_aligned(a, b)
     sizes, host = _on_device(batch_sizes, host_batch_sizes, a.device)
     return _Gmm.apply(a, b, sizes, host, trans_b, dict(workspace=workspace, arguments_ptr=arguments_ptr))
 
@@ -88,6 +100,7 @@ def gmm_swiglu(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor, tran
     ``b [E, K, 2I]`` (``[E, 2I, K]`` with ``trans_b``).  Keeps ``u`` in fp32 (8 bytes per element of
     the result) for the backward pass; without a gradient to come it is ``backend.gmm_swiglu``."""
     backend._check_operands(a, b, torch.bfloat16)
+    _check_aligned(a, b)
     sizes, host = _on_device(batch_sizes, host_batch_sizes, a.device)
     if not (torch.is_grad_enabled() and (a.requires_grad or b.requires_grad)):
         return backend.zero_rows_behind(backend.gmm_swiglu(a, b, sizes, trans_b=trans_b, workspace=workspace,

@@ -35,7 +35,7 @@ def test_host_side_argument_errors():
         return lib.dmoe_gmm_swiglu_backward(dh, u, a, b, du, da, db, bs, rows, 4, K, I, 0, dtype, None, None, 0, None, None)
 
     assert back(dtype=_lib.FP16) == _lib.ERR_DTYPE
-    assert back(K=60) == _lib.ERR_SHAPE and back(I=12) == _lib.ERR_SHAPE
+    assert back(K=60) == _lib.ERR_SHAPE and back(I=12) == _lib.ERR_SHAPE and back(I=1 << 21) == _lib.ERR_SHAPE
     for bad in (dict(dh=None), dict(u=None), dict(a=None), dict(b=None), dict(du=None), dict(bs=None), dict(du=p), dict(du=p + 0x1000),
                 dict(da=p), dict(da=p + 0x2000), dict(dh=p + 8), dict(db=p + 0x6002)):
         assert back(**bad) == _lib.ERR_ARG, bad

@@ -414,6 +414,22 @@ def test_backward_after_the_layer_is_gone():
     assert torch.equal(want_x.grad, got_x.grad)
 
 
+def test_gradients_that_arrive_unaligned():
+    announce(test="unaligned_gradient")
+    # a gradient may be a view of other memory at any element; the operands may not
+    sizes, K, N = torch.tensor([3, 0, 5]), 64, 48
+    a, b = _rand((8, K), 1).requires_grad_(), _rand((3, K, N), 2, 0.1).requires_grad_()
+    for call, cols in ((ops.gmm, N), (ops.gmm_swiglu, N // 2)):
+        c = call(a, b, sizes)
+        d = _rand((8 * cols + 1,), 3)
+        view, copy = d[1:].view(8, cols), d[1:].clone().view(8, cols)
+        assert view.data_ptr() % 16 != 0
+        for x, y in zip(torch.autograd.grad(c, (a, b), view, retain_graph=True), torch.autograd.grad(c, (a, b), copy)):
+            assert torch.equal(x, y)
+        with pytest.raises(ValueError, match="aligned"):
+            call(_rand((8 * K + 1,), 1)[1:].view(8, K), b, sizes)
+
+
 def test_another_stream():
     announce(test="step_stream")
     sizes = torch.tensor([90, 30])

@@ -189,6 +189,22 @@ def test_rows_keep_apart_and_rows_behind():
     assert torch.equal(guard[23:R], clean[23:]) and bool((guard[R:] == 5).all())
 
 
+@pytest.mark.parametrize("zeros", [False, True])
+def test_quantisation_of_tiny_weights(zeros):
+    announce(test="w4_tiny", zeros=zeros)
+    # down to the smallest numbers of bf16: a weight is off by half a step of its group and what the rounded scale cuts off
+    # (2^-8 of 7.5 steps); a scale below 2^-126 counts as zero, and its weights, of up to 7 or 15 steps, with it
+    K, N, group = 128, 48, 32
+    w = _rand((1, K, N), 1) * (2.0 ** -torch.arange(100, 148, device=dev()).double()).to(torch.float32)
+    w = w.to(torch.bfloat16)
+    got = gg.dequantize_w4(gg.quantize_weight_w4(w, group=group, zeros=zeros))[0].t().double()
+    v = w[0].double().view(K // group, group, N)
+    top = v.abs().amax(1) / 7 if not zeros else (v.amax(1).clamp(min=0) - v.amin(1).clamp(max=0)) / 15
+    allowed = torch.where(top * (1 + 2.0 ** -7) < 2.0 ** -126, 15 * 2.0 ** -126, top * (0.5 + 15 * 2.0 ** -8) + 2.0 ** -126)
+    bad = (got.view_as(v) - v).abs() > allowed.unsqueeze(1)
+    assert not bool(bad.any()), (int(bad.sum()), bad.nonzero()[:3].tolist())
+
+
 def test_many_experts():
     announce(test="w4_many_experts")
     E, K, N = 300, 64, 32
@@ -270,7 +286,7 @@ def test_layer(T, zeros):
     assert torch.equal(ready.forward(T * k, stages["permuted"], sizes), stages["expert_out"])
 
 
-@pytest.mark.parametrize("T", [6, 400])
+@pytest.mark.parametrize("T", [6, 400, 1200])
 def test_graph_replays_and_streams(T):
     announce(test="w4_graph", T=T)
     E, d, I = 4, 256, 136
