@@ -1,4 +1,6 @@
-// Instantiations of the gated bf16 product that also leaves its fp32 sums for the gradient.
+// Instantiations of the gated bf16 product that also leaves its fp32 sums for the gradient.  The sums are 8 bytes for every 2
+// of the result: 8192 rows on 8 experts of 4096 x 28672: 1637 - 1734 us (0.94 GB of sums on top of 3.5 GB of other traffic; the
+// form without them 1540), 64 experts of 768 rows, 2048 x 2816: 637 - 676 us.
 #include "gmm_tile256.h"
 
 namespace dmoe {

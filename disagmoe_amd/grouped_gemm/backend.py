@@ -237,6 +237,16 @@ def gmm_swiglu_rows(x: torch.Tensor, row_token: torch.Tensor, b: torch.Tensor, b
 
 # ---- gradients: no counterpart in the reference ------------------------------
 
+def _call_on(device: torch.device, name: str, *args) -> None:
+    """The call with ``device`` current.  (The autograd engine's threads have it current already, and changing it costs
+    them several microseconds.)"""
+    if torch.cuda.current_device() == device.index:
+        _lib.call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args)
+
+
 def gmm_swiglu_keep(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor, trans_b: bool = False,
                     workspace: Optional[torch.Tensor] = None, arguments_ptr: Optional[int] = None,
                     host_batch_sizes: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -251,10 +261,9 @@ def gmm_swiglu_keep(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor,
     h = torch.empty((rows, N2 // 2), dtype=a.dtype, device=device)
     u = torch.empty((rows, N2), dtype=torch.float32, device=device)
     bs = _sizes_on_device(batch_sizes, device)
-    with torch.cuda.device(device):
-        _lib.call("dmoe_gmm_swiglu_keep", a.data_ptr(), b.data_ptr(), h.data_ptr(), u.data_ptr(), bs.data_ptr(), rows, E, K, N2 // 2,
-                  1 if trans_b else 0, _lib.BF16, *_state_args(device, workspace, arguments_ptr, _stream(device),
-                               _host_sizes(batch_sizes, host_batch_sizes)))
+    _call_on(device, "dmoe_gmm_swiglu_keep", a.data_ptr(), b.data_ptr(), h.data_ptr(), u.data_ptr(), bs.data_ptr(), rows, E, K, N2 // 2,
+             1 if trans_b else 0, _lib.BF16, *_state_args(device, workspace, arguments_ptr, _stream(device),
+                                                          _host_sizes(batch_sizes, host_batch_sizes)))
     return h, u
 
 
@@ -282,10 +291,9 @@ def _swiglu_backward(dh, u, a, b, bs, trans_b: bool, need_da: bool, need_db: boo
     du = torch.empty((rows, two_i), dtype=torch.bfloat16, device=a.device)
     da = torch.empty_like(a) if need_da else None
     db = torch.empty_like(b) if need_db else None
-    with torch.cuda.device(a.device):
-        _lib.call("dmoe_gmm_swiglu_backward", dh.data_ptr(), u.data_ptr(), a.data_ptr(), b.data_ptr(), du.data_ptr(),
-                  da.data_ptr() if need_da else None, db.data_ptr() if need_db else None, bs.data_ptr(), rows, b.shape[0], K, two_i // 2,
-                  1 if trans_b else 0, _lib.BF16, *state_args)
+    _call_on(a.device, "dmoe_gmm_swiglu_backward", dh.data_ptr(), u.data_ptr(), a.data_ptr(), b.data_ptr(), du.data_ptr(),
+             da.data_ptr() if need_da else None, db.data_ptr() if need_db else None, bs.data_ptr(), rows, b.shape[0], K, two_i // 2,
+             1 if trans_b else 0, _lib.BF16, *state_args)
     return da, db
 
 
@@ -307,8 +315,7 @@ def _wgrad(a, dc, bs, state_args: tuple) -> torch.Tensor:
     """:func:`gmm_wgrad` on operands that have been checked."""
     E, (rows, K), N = bs.numel(), a.shape, dc.shape[1]
     db = torch.empty((E, K, N), dtype=a.dtype, device=a.device)
-    with torch.cuda.device(a.device):
-        _lib.call("dmoe_gmm_wgrad", a.data_ptr(), dc.data_ptr(), db.data_ptr(), bs.data_ptr(), rows, E, K, N, _lib.BF16, *state_args)
+    _call_on(a.device, "dmoe_gmm_wgrad", a.data_ptr(), dc.data_ptr(), db.data_ptr(), bs.data_ptr(), rows, E, K, N, _lib.BF16, *state_args)
     return db
 
 
@@ -317,9 +324,8 @@ def _gmm_backward(dc, a, b, bs, trans_b: bool, need_da: bool, need_db: bool, sta
     da = db = None
     if need_da:
         da = torch.empty_like(a)
-        with torch.cuda.device(a.device):
-            _lib.call("dmoe_gmm", dc.data_ptr(), b.data_ptr(), da.data_ptr(), bs.data_ptr(), a.shape[0], b.shape[0], dc.shape[1], a.shape[1],
-                      0 if trans_b else 1, _lib.BF16, *state_args)
+        _call_on(a.device, "dmoe_gmm", dc.data_ptr(), b.data_ptr(), da.data_ptr(), bs.data_ptr(), a.shape[0], b.shape[0], dc.shape[1], a.shape[1],
+                 0 if trans_b else 1, _lib.BF16, *state_args)
         zero_rows_behind(da, bs)
     if need_db:
         db = _wgrad(dc, a, bs, state_args) if trans_b else _wgrad(a, dc, bs, state_args)
@@ -330,9 +336,8 @@ def zero_rows_behind(c: torch.Tensor, batch_sizes: torch.Tensor) -> torch.Tensor
     """Zeros in the rows of ``c [rows, d]`` past ``sum(batch_sizes)``, which the products leave as they are."""
     assert c.is_cuda and c.dim() == 2 and c.is_contiguous() and c.dtype in (torch.bfloat16, torch.float16)
     bs = _sizes_on_device(batch_sizes, c.device)
-    with torch.cuda.device(c.device):
-        _lib.call("dmoe_zero_rows_behind", c.data_ptr(), bs.data_ptr(), c.shape[0], bs.numel(), c.shape[1],
-                  _lib.BF16 if c.dtype == torch.bfloat16 else _lib.FP16, _stream(c.device))
+    _call_on(c.device, "dmoe_zero_rows_behind", c.data_ptr(), bs.data_ptr(), c.shape[0], bs.numel(), c.shape[1],
+             _lib.BF16 if c.dtype == torch.bfloat16 else _lib.FP16, _stream(c.device))
     return c
 
 

@@ -48,6 +48,15 @@ def _gradient(dc: torch.Tensor) -> torch.Tensor:
     return dc.clone() if dc.data_ptr() & 15 else dc
 
 
+def _once(backward):
+    """``once_differentiable``, whose wrapper is left out where no gradient of the gradient can be asked for."""
+    wrapped = once_differentiable(backward)
+
+    def run(ctx, dc):
+        return (wrapped if torch.is_grad_enabled() else backward)(ctx, dc)
+    return run
+
+
 class _Gmm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, a, b, sizes, host, trans_b, state):
@@ -57,7 +66,7 @@ class _Gmm(torch.autograd.Function):
         return c
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dc):
         _check_capture(ctx)
         a, b, sizes = ctx.saved_tensors
@@ -74,7 +83,7 @@ class _GmmSwiglu(torch.autograd.Function):
         return h
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dh):
         _check_capture(ctx)
         a, b, sizes, u = ctx.saved_tensors

@@ -2,8 +2,10 @@
  * dmoe.h -- C ABI of libdmoe_hip.so: the MI355X (gfx950) expert-worker hot path.
  *
  * Routing ids -> expert-sorted row mapping, token permute / gather, ragged
- * grouped GEMM (bf16 and fp8-e4m3, SiLU*mul fused for the gate-up projection)
- * and the gate-weighted combine back to token order.
+ * grouped GEMM (bf16, fp8-e4m3 and 4-bit weights, SiLU*mul fused for the gate-up
+ * projection) and the gate-weighted combine back to token order; and, for training
+ * the experts, the gradients of the grouped products and of the gated block, the
+ * global gradient norm and clipping.
  *
  * Conventions for every entry point
  *   - all data pointers are DEVICE pointers on the current HIP device unless a
