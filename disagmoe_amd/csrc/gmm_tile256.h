@@ -31,7 +31,8 @@ namespace dmoe {
 // the epilogue of the tile before it, when nothing else of the wavefront is in flight: behind the epilogue the same
 // wait would also be one for the epilogue's stores.
 // KEEP (gated form): the fp32 sums also go to p.u, for the activation's gradient.
-// HALF (trans_b): fp16 operands whose rows and columns carry fp32 scales, c = (a @ b[e]^T) a_scale[r] b_scale[e, n] in bf16.
+// HALF (trans_b): fp16 operands whose rows and columns carry scales that are powers of two, in fp32: c = (a @ b[e]^T)
+// a_scale[r] b_scale[e, n] in bf16.
 // TAIL: K is no multiple of 32; the last stage reaches past it.  What lies there (the next row, the next expert, nothing) is not
 // read: such lanes copy the stage's first k again, and write zeros over it once it has landed, in both operands.
 template <bool TRANS_B, bool SWIGLU, bool GATHER = false, bool KEEP = false, bool HALF = false, bool TAIL = false>
@@ -442,14 +443,18 @@ void gmm_tile256_kernel(const GmmArgs p) {
                     const int i = i2 * 2 + ii;
                     const int row = ii * 16 + l16;
                     if constexpr (HALF) {
-                        // rows and columns outside the tile read a valid neighbour's scale; their results are never stored
+                        // rows and columns outside the tile read a valid neighbour's scale; their results are never stored.
+                        // The scales are powers of two and their exponents are added: their product may lie outside fp32
+                        // where the result does not.
+                        auto exponent = [](float f) { return (int)(__float_as_uint(f) >> 23) - 127; };
                         const int r = wm * TM + i * 16 + l16;
-                        const float sa = p.a_scale[cur_row0 + (r < cur_rows_e ? r : 0)];
+                        const int ea = exponent(p.a_scale[cur_row0 + (r < cur_rows_e ? r : 0)]);
 #pragma unroll
                         for (int j = 0; j < FN; ++j) {
                             const int col = col0 + (j % FNO) * 16 + g16 * 4;
                             const f32x4 sb = *(const f32x4 *)(p.b_scale + (long long)cur_e * p.N + (j < FNO ? 0 : n_out) + (col < n_out ? col : cur_n0));
-                            acc[i][j] *= sb * sa;
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) acc[i][j][x] = __builtin_ldexpf(acc[i][j][x], ea + exponent(sb[x]));
                         }
                     }
 #pragma unroll

@@ -358,7 +358,8 @@ int dmoe_gmm_fp8_swiglu(const void *a, const float *a_scale, const void *b, cons
  * the experts that have rows, rounded to the 11 bits of fp16, and the rows are written there with scales that are powers
  * of two and go through the bf16 product's 256-row tile; without it the one kernel serves any number of rows.
  * A row of a with an infinity or NaN has no finite result (NaN where few rows run: the offset of the codes is taken off as
- * a sum of its own, inf - inf); the other rows do not see it.  state, workspace and host_batch_sizes as for dmoe_gmm (the first two serve the form of many
+ * a sum of its own, inf - inf; so are sums past the range of fp32, which magnitudes of a below 2^116 cannot reach); the other
+ * rows do not see it.  state, workspace and host_batch_sizes as for dmoe_gmm (the first two serve the form of many
  * rows only). */
 int dmoe_w4_bytes(int E, int64_t K, int64_t N, int group, size_t *code_bytes, size_t *scale_bytes, size_t *zero_bytes);
 int dmoe_w4_quant(const void *w, int E, int64_t K, int64_t N, int group, void *codes, void *scales, void *zeros,

@@ -204,6 +204,28 @@ def test_contractions_that_end_inside_a_stage(sizes, K, I, trans_b):
     _check_block(u, h, da, db.transpose(1, 2) if trans_b else db, a, b.transpose(1, 2) if trans_b else b, dh, sizes)
 
 
+def test_offsets_past_32_bits():
+    announce(test="ffn_offsets")
+    # sums of 4.5 GB, then weight gradients of 5.4 GB: what lies at the far end
+    K, I, sizes = 64, 16384, torch.tensor([33000, 1000])
+    a, b, dh = _rand((34000, K), 1), _rand((2, K, 2 * I), 2, 0.125), _rand((34000, I), 3)
+    h, u = gg.gmm_swiglu_keep(a, b, sizes)
+    da, db = gg.gmm_swiglu_backward(dh, u, a, b, sizes)
+    _check_block(u[33000:], h[33000:], da[33000:], db[1:], a[33000:], b[1:], dh[33000:], torch.tensor([1000]))
+    del u, h, da, db, dh
+    E, K, N = 40, 8192, 8192
+    sizes = torch.zeros(E, dtype=torch.int64)
+    sizes[0], sizes[E - 1] = 30, 40
+    a, dc = _rand((70, K), 4), _rand((70, N), 5)
+    db = gg.gmm_wgrad(a, dc, sizes)
+    for e, at in ((0, slice(0, 30)), (E - 1, slice(30, 70))):
+        x, d = a[at].double(), dc[at].double()
+        _close(db[e], x.t() @ d, ACC * 44 * (x.abs().t() @ d.abs()))
+    assert not bool(db[1:E - 1].any())
+    del db
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("trans_b", [False, True])
 @pytest.mark.parametrize("variant", range(1, 9))
 def test_gated_block_on_every_tile(variant, trans_b, default_tile):
@@ -412,6 +434,19 @@ def test_backward_after_the_layer_is_gone():
     assert ptr not in gg._STATE_BLOCKS
     y.backward(dy)
     assert torch.equal(want_x.grad, got_x.grad)
+
+
+def test_a_layer_without_rows():
+    announce(test="no_rows")
+    layer = MoEExperts(64, 48, 3, device=dev()).requires_grad_()
+    sizes = torch.zeros(3, dtype=torch.int64)
+    for rows in (0, 700):                                 # none at all, and a padded batch that belongs to nobody
+        x = torch.full((rows, 64), float("nan"), dtype=torch.bfloat16, device=dev(), requires_grad=True)
+        y = layer.forward_train(rows, x, sizes)
+        assert y.shape == (rows, 64) and not bool(y.any())
+        for g in torch.autograd.grad(y, (x, *layer.parameters()), torch.ones_like(y)):
+            assert not bool(g.any())
+        assert float(grads.global_norm(torch.autograd.grad(layer.forward_train(rows, x, sizes).sum(), list(layer.parameters())))) == 0
 
 
 def test_gradients_that_arrive_unaligned():

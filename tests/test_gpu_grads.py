@@ -157,3 +157,17 @@ def test_graph_replays_and_streams():
         torch.cuda.synchronize()
         for (g, n, ts), (m, eager) in zip(graphs, want):
             assert torch.equal(n, m) and all(torch.equal(x, y) for x, y in zip(ts, eager))
+
+
+def test_a_tensor_past_32_bits():
+    announce(test="clip_large")
+    n = (1 << 31) + 4099                                  # bf16: more than 4 GiB
+    g = torch.full((n,), 0.5, dtype=torch.bfloat16, device=dev())
+    g[n - 1] = 40000.0
+    want = (0.25 * (n - 1) + float(g[n - 1]) ** 2) ** 0.5
+    assert abs(float(grads.global_norm(g)) - want) <= 2.0 ** -23 * want
+    last = float(g[n - 1])
+    grads.clip_by_global_norm_(g, want / 4)
+    assert bool((g[:n - 1] == 0.125).all()) and abs(float(g[n - 1]) - last / 4) <= 2.0 ** -8 * last
+    del g
+    torch.cuda.empty_cache()

@@ -189,6 +189,46 @@ def test_rows_keep_apart_and_rows_behind():
     assert torch.equal(guard[23:R], clean[23:]) and bool((guard[R:] == 5).all())
 
 
+@pytest.mark.parametrize("rows", [40, 600])
+def test_scales_whose_product_leaves_the_range(rows):
+    announce(test="w4_scales_range", rows=rows)
+    # rows and columns whose scales multiplied lie outside fp32 while every result is zero or of ordinary size
+    K, N, group = 256, 48, 128
+    x = torch.zeros(rows, K, dtype=torch.bfloat16, device=dev())
+    x[:, 7] = 2.0 ** 110
+    x[1::2, 7] = 2.0 ** -100
+    x[:, 200] = 1.0
+    q = torch.full((1, N, K), 8, device=dev(), dtype=torch.uint8)
+    q[0, :, 200] = 9
+    s = torch.ones(1, N, K // group, device=dev(), dtype=torch.bfloat16)
+    s[0, :, 0] = 2.0 ** 40                                # of weights that are zero
+    s[0, 16:, 0] = 2.0 ** -60
+    s[0, 32:, 1] = 0
+    out = gg.gmm_w4(x, gg.pack_w4(q, s, None, group), torch.tensor([rows]))
+    assert bool((out[:, 32:] == 0).all())
+    # (many rows: a 1 beside 2^110 in its row, or a scale of 1 beside 2^40 in its column, is below what fp16 has left)
+    near = out[1::2, 16:32] if rows > 512 else out[:, :32]
+    assert bool((near == 1).all()) and bool(out.isfinite().all())
+
+
+def test_offsets_past_32_bits():
+    announce(test="w4_offsets")
+    # codes of 5 GiB, 16-bit weights of 20 GiB: the last expert's rows, few and many
+    E, N, K, group = 80, 16384, 8192, 128
+    codes, groups = gg._w4_shapes(E, K, N, group)
+    w = gg.W4Weight(torch.zeros(codes, dtype=torch.uint8, device=dev()), torch.zeros(groups, dtype=torch.bfloat16, device=dev()), None, K, N, group)
+    one, ref, s = _weight(1, N, K, group, False, 3)
+    w.codes[E - 1], w.scales[E - 1] = one.codes[0], one.scales[0]
+    for rows in (5, 100, 600):
+        sizes = torch.zeros(E, dtype=torch.int64)
+        sizes[E - 1] = rows
+        x = _rand((rows, K), rows)
+        got = gg.gmm_w4(x, w, sizes)
+        assert torch.equal(got, gg.gmm_w4(x, one, torch.tensor([rows])))
+        _check(got[:8, -64:], x[:8], ref[:, -64:], s[:, -64:], torch.tensor([min(rows, 8)]), group, False, rows > 512)
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("zeros", [False, True])
 def test_quantisation_of_tiny_weights(zeros):
     announce(test="w4_tiny", zeros=zeros)
