@@ -507,6 +507,7 @@ static GmmLaunch choose_launch(const GmmArgs &args, bool trans_b, bool swiglu, b
             if (busy < 1) busy = 1;
         }
         const long long avg = args.rows / busy;
+        L.avg_rows = avg;
         const long long n_tiles = ((swiglu ? args.N / 2 : args.N) + (swiglu ? 127 : 255)) / (swiglu ? 128 : 256);
         const bool exact = t_host_sizes != nullptr;
         const long long est256 = (exact ? m_tiles_of(args, 256) : args.rows / 256 + (args.E + 1) / 2) * n_tiles;
@@ -566,21 +567,29 @@ static int launch_by_rows(const GmmArgs &args, hipStream_t stream) {
     else return launch_direct_bf16(args, L.tile_rows, TRANS_B, SWIGLU, stream);
 }
 
-// Contractions that end inside a stage, in the gated block's training: the 256-row tile with its last stage filled up with
-// zeros, where the experts have 256 rows and more on average and tiles of that height are chosen; below, the register-staged
-// kernel and its smaller tiles.  Forward / backward in us, staged -> this (K, I both no multiple of 32): 8 experts of 2048
-// rows, 4104 x 5000: 1654 / 3386 -> 1369 / 3019; of 512 rows, 4104 x 2056: 323 / 505 -> 284 / 508; of 256 rows, 1000 x 1000
-// (128-row tiles): 40 / 72 against 43 / 106; 64 experts of 32 rows, weights [N, K]: 61 against 83 forward.
-static bool takes_tail(const GmmArgs &args, const GmmLaunch &L) {
-    return L.kernel == kKernelStaged && g_variant == 0 && L.tile_rows == 256 && args.K % 32 != 0 && args.rows >= 256ll * args.E &&
-           (long long)args.K * args.N * 2 < (1ll << 32);
+// Contractions that end inside a stage, in the gated block's training: the tile rows of the kernels that fill the last stage up
+// with zeros, 0 where the register-staged kernel has to run (one expert's weights past 4 GiB).  The rows are those of any
+// other launch, but 256-row tiles are left to experts of more rows: a tile's loop runs at the pace of its copies, and those of
+// K-contiguous weights, 64 bytes of rows that begin anywhere, fetch their lines twice.  Measured, us, register-staged / rule of
+// other launches / this rule; forward on [K, N] weights, backward (without db) on them, forward on [N, K]:
+//   1 expert,  210 rows, 2392 x 2 x 15288: 76 / 60 / 60      599 / 110 / 110     76 / 67 / 67
+//   8 experts,   8 rows, 3520 x 2 x 4120:  46 / 46 / 46      146 / 52 / 52       52 / 51 / 51
+//   8 experts,  32 rows, 5552 x 2 x 9768:  460 / 329 / 312   480 / 432 / 432     521 / 553 / 437
+//  64 experts, 1548 rows, 520 x 2 x 1832:  110 / 69 / 56     103 / 87 / 87       81 / 104 / 68
+//  31 experts, 3440 rows, 648 x 2 x 6616:  269 / 200 / 200   395 / 402 / 374     258 / 294 / 241
+//  64 experts, 8192 rows, 1000 x 2 x 712:  99 / 86 / 86      76 / 109 / 86       82 / 114 / 88
+//   5 experts, 12680 rows, 1112 x 2 x 8008: 834 / 665 / 665  1579 / 1020 / 1020  804 / 710 / 710
+static int tail_rows(const GmmArgs &args, const GmmLaunch &L, bool trans_b) {
+    if (L.kernel != kKernelStaged || (g_variant >= 1 && g_variant <= 4) || args.K % 32 == 0 || (long long)args.K * args.N * 2 >= (1ll << 32)) return 0;
+    if (g_variant != 0 || L.tile_rows != 256) return L.tile_rows;
+    return L.avg_rows <= 64 ? 64 : (trans_b && L.avg_rows <= 160 ? 128 : 256);
 }
 
 // The gated form that also leaves its fp32 sums in args.u.
 template <bool TRANS_B>
 static int launch_keep(const GmmArgs &args, hipStream_t stream) {
     GmmLaunch L = choose_launch(args, TRANS_B, true, false);
-    if (takes_tail(args, L)) return launch_tile256_tail(args, TRANS_B, true, stream);
+    if (const int rows = tail_rows(args, L, TRANS_B)) return launch_tail(args, rows, TRANS_B, true, stream);
     if (L.kernel == kKernelStaged) {
         if (L.tile_rows == 64) return launch_one<64, 256, 1, 4, TRANS_B, true, false, true>(args, stream);
         if (L.tile_rows == 128) return launch_one<128, 256, 1, 4, TRANS_B, true, false, true>(args, stream);
@@ -757,8 +766,9 @@ extern "C" int dmoe_gmm_swiglu_backward(const void *dh, const float *u, const vo
             const HostSizes known(host_batch_sizes);
             GmmArgs args{(const char *)du, (const char *)b, (char *)da, batch_sizes, nullptr, nullptr, rows, E, (int)(2 * I), (int)K, (int)K};
             rc = bind_state(args, state, workspace, workspace_bytes, (hipStream_t)stream);
-            if (rc == DMOE_OK && takes_tail(args, choose_launch(args, !trans_b, false, false)))
-                rc = launch_tile256_tail(args, !trans_b, false, (hipStream_t)stream);
+            const int tail = tail_rows(args, choose_launch(args, !trans_b, false, false), !trans_b);
+            if (rc == DMOE_OK && tail != 0)
+                rc = launch_tail(args, tail, !trans_b, false, (hipStream_t)stream);
             else if (rc == DMOE_OK)
                 rc = trans_b ? launch_by_rows<false, false, false>(args, (hipStream_t)stream) : launch_by_rows<true, false, false>(args, (hipStream_t)stream);
         }

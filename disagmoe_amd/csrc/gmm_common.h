@@ -335,6 +335,7 @@ struct GmmLaunch {
     int stage_k;       // k per unit of plan_work's lengths (bf16: 32; fp8: 64)
     bool may_cut;      // the kernel cuts tiles along K when the launch has a workspace
     long long grid;    // workgroups
+    long long avg_rows;   // rows per expert that has any (as far as the host knows)
 };
 // The caller's copy of batch_sizes in host memory for the call that this thread is in, or nullptr: the reference keeps
 // the sizes on the host wherever it does not run its CUTLASS path (disagmoe/frontend/engine.py:377-380, 690-701).
@@ -373,7 +374,7 @@ int launch_wave128(const GmmArgs &args, bool swiglu, hipStream_t stream);
 int launch_wave128_fp8(const GmmArgs &args, bool swiglu, hipStream_t stream);
 int launch_tile256_rows(const GmmArgs &args, hipStream_t stream);
 int launch_wgrad(const GmmArgs &args, hipStream_t stream);
-int launch_tile256_tail(const GmmArgs &args, bool trans_b, bool keep, hipStream_t stream);
+int launch_tail(const GmmArgs &args, int tile_rows, bool trans_b, bool keep, hipStream_t stream);
 int launch_tile256_half(const GmmArgs &args, bool swiglu, hipStream_t stream);
 int bind_state(GmmArgs &args, void *state, void *workspace, size_t workspace_bytes, hipStream_t stream);
 // The caller's copy of the sizes on the host for the length of one call.

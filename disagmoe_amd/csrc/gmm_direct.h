@@ -80,7 +80,9 @@ constexpr int kStageB = kDN * kDK * 2;     // 16 KiB of B per stage
 // (and draw the work items), the first NW only compute: a copy that waits for room in the memory pipeline then holds
 // up no MFMA, which is what small tiles on weights streamed from HBM need.
 // KEEP (bf16, gated form): the fp32 sums also go to p.u, for the activation's gradient.
-template <int kDM, int NW, int WM, bool TRANS_B, bool SWIGLU, bool FP8, int NP = 0, bool KEEP = false>
+// TAIL (bf16): K is no multiple of 32; the last stage reaches past it, and what lies there is not read: such lanes copy the
+// stage's first k again and write zeros over it once it has landed, in both operands.
+template <int kDM, int NW, int WM, bool TRANS_B, bool SWIGLU, bool FP8, int NP = 0, bool KEEP = false, bool TAIL = false>
 __global__ __launch_bounds__((NW + NP) * 64) __attribute__((amdgpu_waves_per_eu((NW + NP + 3) / 4, (NW + NP + 3) / 4)))
 void gmm_direct_kernel(const GmmArgs p) {
     constexpr int kStageK = FP8 ? 64 : kDK;               // k per stage: 64 bytes per row either way
@@ -100,6 +102,7 @@ void gmm_direct_kernel(const GmmArgs p) {
     constexpr int kStages = kDM == 256 ? 4 : (kDM == 128 ? 5 : 6);
     constexpr int BNO = SWIGLU ? kDN / 2 : kDN;
     static_assert(!KEEP || (SWIGLU && !FP8), "only the gated form has something to keep");
+    static_assert(!TAIL || !FP8, "fp8 operands have whole stages");
     static_assert(kDM == 64 || kDM == 128 || kDM == 256, "tile rows");
     static_assert((NW == 4 || NW == 8) && WM * WN == NW && CA >= 1 && FM >= 1 && FN >= 2 && NR <= NM, "wave layout");
     static_assert(NP == 0 || (NP == 2 && NW == 4 && !FP8), "copying wavefronts: two, beside four computing ones");
@@ -120,7 +123,8 @@ void gmm_direct_kernel(const GmmArgs p) {
 
     const int n_out = SWIGLU ? p.N / 2 : p.N;
     const int n_tiles = (n_out + BNO - 1) / BNO;
-    const int S_all = p.K / kStageK;               // stages of a whole tile (whole stages only)
+    const int S_all = TAIL ? (p.K + kStageK - 1) / kStageK : p.K / kStageK;   // stages of a whole tile
+    const int k_tail = TAIL ? p.K - (S_all - 1) * kStageK : kStageK;          // k of the last one
     const int G = gridDim.x;
     // tiles of the last, partly filled round are cut along K (plan_work) when the launch has a workspace for their sums
     constexpr long long kPieceBytes = (long long)kDM * kDN * sizeof(float);
@@ -190,16 +194,33 @@ void gmm_direct_kernel(const GmmArgs p) {
         }
     };
 
+    // TAIL: whether this lane's piece of copy c lies past K in the last stage
+    auto past = [&](int c) { return (c < CA || TRANS_B ? kc_chunk * 8 : (c - CA) * 2 * NC + kn_k) >= k_tail; };
     // copy number c (0 .. kLoads-1) of this wavefront for stage s: first its CA blocks of A, then its CB blocks of B
     auto issue_copy = [&](int s, auto c_tag) {
         constexpr int c = decltype(c_tag)::value;
         const uint32_t lds = smem_addr + (s % kStages) * kStage + cw * 1024;
+        const bool back = TAIL && s_lo + s == S_all - 1 && past(c);
         if constexpr (c < CA) {
-            copy_g2lds_16<c * kBlock>(a_off[c], a_base + (uint64_t)s * 64, lds);
+            copy_g2lds_16<c * kBlock>(back ? a_off[c] - kc_chunk * 16 : a_off[c], a_base + (uint64_t)s * 64, lds);
         } else {
             constexpr int i = c - CA;
-            if constexpr (TRANS_B) copy_g2lds_16<kStageA + i * kBlock>(b_off[i], b_exp + (uint64_t)s * 64, lds);
-            else copy_g2lds_16<kStageA + i * kBlock>(b_off[i], b_exp + (uint64_t)s * kDK * p.N * 2, lds);
+            const uint32_t first = TRANS_B ? (uint32_t)kc_chunk * 16 : (uint32_t)(i * 2 * NC + kn_k) * (uint32_t)p.N * 2;
+            const uint32_t off = back ? b_off[i] - first : b_off[i];
+            if constexpr (TRANS_B) copy_g2lds_16<kStageA + i * kBlock>(off, b_exp + (uint64_t)s * 64, lds);
+            else copy_g2lds_16<kStageA + i * kBlock>(off, b_exp + (uint64_t)s * kDK * p.N * 2, lds);
+        }
+    };
+    // TAIL: zeros over what lies past K of stage s, if that is the last of the tile whose first stage is `lo` (this lane's
+    // own copies, which have landed)
+    auto clear_past = [&](int s, int lo) {
+        if constexpr (TAIL) {
+            if (lo + s != S_all - 1) return;
+            __builtin_amdgcn_sched_barrier(0);                 // behind the wait
+            char *mine = smem + (s % kStages) * kStage + cw * 1024 + lane * 16;
+#pragma unroll
+            for (int c = 0; c < kLoads; ++c)
+                if (past(c)) *(u32x4 *)(mine + (c < CA ? c * kBlock : kStageA + (c - CA) * kBlock)) = u32x4{0, 0, 0, 0};
         }
     };
     auto issue_prologue = [&]() {
@@ -290,10 +311,12 @@ void gmm_direct_kernel(const GmmArgs p) {
             // ---- a copying wavefront: the same barriers as the computing ones, tile by tile ----
             while (q < total) {
                 wait_ahead(pre - 1);
+                clear_past(0, s_lo);
                 __syncthreads();                   // stage 0 has landed
                 for (int s = 0; s + 1 < S; ++s) {
                     const int left = S - 1 - s;    // stages after s; s + 1 has to land, the ones behind it may be in flight
                     wait_ahead(left - 1 < kStages - 2 ? left - 1 : kStages - 2);
+                    clear_past(s + 1, s_lo);
                     __syncthreads();               // hand-over: stage s + 1 is there, stage s has been read
                     if (s + kStages < S) static_for<0, kLoads>([&](auto c) { issue_copy(s + kStages, c); });
                 }
@@ -314,7 +337,7 @@ void gmm_direct_kernel(const GmmArgs p) {
     while (q < total) {
         // results of this tile go here after the next tile's copies have been issued
         const int cur_row0 = row0, cur_rows_e = rows_e, cur_n0 = n0, cur_e = e;
-        const int cur_part = part, cur_split_tile = split_tile;
+        const int cur_part = part, cur_split_tile = split_tile, cur_s_lo = s_lo;
         // row fragments of this wavefront that hold at least one valid row (a short last tile skips the rest)
         int nfr = ((rows_e < kDM ? rows_e : kDM) - wm * TM + 31) / 32;
         nfr = __builtin_amdgcn_readfirstlane(nfr < 0 ? 0 : (nfr > FM ? FM : nfr));
@@ -346,7 +369,10 @@ void gmm_direct_kernel(const GmmArgs p) {
 
         // stage 0 of this tile has landed (its other prologue stages, and stores of the previous tile's
         // epilogue that were issued after them, may still be in flight: waiting for fewer is only stricter)
-        if constexpr (NP == 0) wait_ahead(pre - 1);
+        if constexpr (NP == 0) {
+            wait_ahead(pre - 1);
+            clear_past(0, cur_s_lo);
+        }
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < NR; ++r) load_frag(0, 0, 0, r);
@@ -387,7 +413,10 @@ void gmm_direct_kernel(const GmmArgs p) {
             if (kSteady || next) {
                 if constexpr (NP > 0) {}   // the copying wavefronts wait for the data
                 else if constexpr (kSteady) DMOE_WAIT_VMCNT((kStages - 2) * kLoads);
-                else wait_ahead(ahead);
+                else {
+                    wait_ahead(ahead);
+                    clear_past(s + 1, cur_s_lo);
+                }
                 __syncthreads();
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -622,11 +651,11 @@ void gmm_direct_kernel(const GmmArgs p) {
     sched_finish(p.sched, drawer, draw, streams, total);
 }
 
-template <int kDM, int NW, int WM, bool TRANS_B, bool SWIGLU, bool FP8, int NP = 0, bool KEEP = false>
+template <int kDM, int NW, int WM, bool TRANS_B, bool SWIGLU, bool FP8, int NP = 0, bool KEEP = false, bool TAIL = false>
 static int launch_direct_one(const GmmArgs &args, hipStream_t stream) {
     constexpr int kStages = kDM == 256 ? 4 : (kDM == 128 ? 5 : 6);
     const size_t lds = (size_t)kStages * (kDM * kDK * 2 + kStageB);
-    auto kern = gmm_direct_kernel<kDM, NW, WM, TRANS_B, SWIGLU, FP8, NP, KEEP>;
+    auto kern = gmm_direct_kernel<kDM, NW, WM, TRANS_B, SWIGLU, FP8, NP, KEEP, TAIL>;
     static unsigned long long configured = 0;   // devices on which the kernel's LDS size has been raised
     DMOE_HIP(raise_dynamic_lds((const void *)kern, (int)lds, &configured));
     const long long grid = launch_grid(args, kDM, SWIGLU, FP8 ? 64 : kDK, true, device_cus());

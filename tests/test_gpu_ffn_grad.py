@@ -177,17 +177,19 @@ def default_tile():
     gg.set_tile_variant(0)
 
 
+@pytest.mark.parametrize("variant", [0, 5, 6, 7])
 @pytest.mark.parametrize("trans_b", [False, True])
 @pytest.mark.parametrize("sizes,K,I", [([5], 8, 8), ([300, 0, 17], 24, 4), ([70, 1, 256, 257], 40, 300), ([600, 520], 4104, 132),
-                                       ([33], 8200, 4100), ([2000, 0, 1500], 1000, 516), ([900, 700], 56, 2052),
+                                       ([33], 8200, 4100), ([2000, 0, 1500], 1000, 516), ([900, 700], 56, 2052), ([3] * 40, 1000, 72),
                                        ([1600, 4000], 40, 2052), ([3000, 40], 4104, 1500), ([5000], 8, 1800)], ids=str)
-def test_contractions_that_end_inside_a_stage(sizes, K, I, trans_b):
-    announce(test="block_tail", sizes=sizes, K=K, I=I, trans_b=trans_b)
+def test_contractions_that_end_inside_a_stage(sizes, K, I, trans_b, variant, default_tile):
+    announce(test="block_tail", sizes=sizes, K=K, I=I, trans_b=trans_b, variant=variant)
     # K and 2I of any multiple of 8, long ones of few tiles among them (cut into pieces).  The rows, weights and gradients
     # stand in front of NaN: a k past the end that got into a product would show, as a zero times it would.
     if I % 8:
         I += 4
     E, R, sizes = len(sizes), sum(sizes), torch.tensor(sizes)
+    gg.set_tile_variant(variant)                          # (5, 6, 7: tiles of 64, 128 and 256 rows)
 
     def guarded(*shape, seed, std=1.0):
         n = 1
