@@ -579,9 +579,17 @@ static int launch_by_rows(const GmmArgs &args, hipStream_t stream) {
 //  31 experts, 3440 rows, 648 x 2 x 6616:  269 / 200 / 200   395 / 402 / 374     258 / 294 / 241
 //  64 experts, 8192 rows, 1000 x 2 x 712:  99 / 86 / 86      76 / 109 / 86       82 / 114 / 88
 //   5 experts, 12680 rows, 1112 x 2 x 8008: 834 / 665 / 665  1579 / 1020 / 1020  804 / 710 / 710
-static int tail_rows(const GmmArgs &args, const GmmLaunch &L, bool trans_b) {
+// And 256-row tiles are taken instead of 128-row ones where (nearly) a third of the compute units get one and their contractions are
+// long enough to be cut in two (backward without db on [K, N] and [N, K] weights, 128 / 256-row tiles): 126 tiles of 574 stages:
+// 535 / 408 and 413 / 381; 84 of 574: 436 / 349 and 368 / 296; 96 of 312: 219 / 193 and 207 / 167; but 64 of 187: 119 / 142, 60
+// of 173: 138 / 161.
+static int tail_rows(const GmmArgs &args, const GmmLaunch &L, bool trans_b, bool swiglu) {
     if (L.kernel != kKernelStaged || (g_variant >= 1 && g_variant <= 4) || args.K % 32 == 0 || (long long)args.K * args.N * 2 >= (1ll << 32)) return 0;
-    if (g_variant != 0 || L.tile_rows != 256) return L.tile_rows;
+    if (g_variant != 0 || L.tile_rows == 64) return L.tile_rows;
+    if (L.tile_rows == 128) {
+        const long long tiles = m_tiles_of(args, 256) * (swiglu ? (args.N / 2 + 127) / 128 : (args.N + 255) / 256);
+        return L.avg_rows > 160 && args.arrive != nullptr && 3 * tiles + 16 >= device_cus() && args.K / 32 >= 2 * kMinPieceStages ? 256 : 128;
+    }
     return L.avg_rows <= 64 ? 64 : (trans_b && L.avg_rows <= 160 ? 128 : 256);
 }
 
@@ -589,7 +597,7 @@ static int tail_rows(const GmmArgs &args, const GmmLaunch &L, bool trans_b) {
 template <bool TRANS_B>
 static int launch_keep(const GmmArgs &args, hipStream_t stream) {
     GmmLaunch L = choose_launch(args, TRANS_B, true, false);
-    if (const int rows = tail_rows(args, L, TRANS_B)) return launch_tail(args, rows, TRANS_B, true, stream);
+    if (const int rows = tail_rows(args, L, TRANS_B, true)) return launch_tail(args, rows, TRANS_B, true, stream);
     if (L.kernel == kKernelStaged) {
         if (L.tile_rows == 64) return launch_one<64, 256, 1, 4, TRANS_B, true, false, true>(args, stream);
         if (L.tile_rows == 128) return launch_one<128, 256, 1, 4, TRANS_B, true, false, true>(args, stream);
@@ -766,7 +774,7 @@ extern "C" int dmoe_gmm_swiglu_backward(const void *dh, const float *u, const vo
             const HostSizes known(host_batch_sizes);
             GmmArgs args{(const char *)du, (const char *)b, (char *)da, batch_sizes, nullptr, nullptr, rows, E, (int)(2 * I), (int)K, (int)K};
             rc = bind_state(args, state, workspace, workspace_bytes, (hipStream_t)stream);
-            const int tail = tail_rows(args, choose_launch(args, !trans_b, false, false), !trans_b);
+            const int tail = tail_rows(args, choose_launch(args, !trans_b, false, false), !trans_b, false);
             if (rc == DMOE_OK && tail != 0)
                 rc = launch_tail(args, tail, !trans_b, false, (hipStream_t)stream);
             else if (rc == DMOE_OK)
