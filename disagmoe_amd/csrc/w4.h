@@ -321,8 +321,10 @@ __device__ __forceinline__ void w4_finish(const W4Args &p, float *red, const f32
     __syncthreads();                                          // read: the LDS may be written again
 }
 
-// Wavefronts to a SIMD: as many as the registers of the form allow without spills.
-constexpr int w4_waves(int FM) { return FM == 1 ? 4 : (FM == 2 ? 3 : 2); }
+// Wavefronts to a SIMD: as many as the registers of the form allow without (many) spills.
+constexpr int w4_waves(int FM, int NF) {
+    return FM == 1 ? 4 : (FM == 2 && NF <= 4 ? 3 : 2);
+}
 
 // FM row fragments of 16, FG column fragments of 16 per wavefront (SWIGLU: of the result, with as many of the gate and of
 // the up columns; SHIFT: the up columns begin in the middle of a tile, one more), WN wavefronts along the columns, WK
@@ -330,7 +332,7 @@ constexpr int w4_waves(int FM) { return FM == 1 ? 4 : (FM == 2 ? 3 : 2); }
 // wavefronts to a SIMD keep loads in flight.  64 rows (FM 4): the sums leave room for two, so weights and rows are fetched a
 // round ahead, and all wavefronts bring the WK chunks of a round into LDS, once for the WN wavefronts that read each.
 template <int FM, int FG, int WN, int WK, int G, bool ZERO, bool SWIGLU, bool SHIFT>
-__global__ __launch_bounds__(WN *WK *kWave) __attribute__((amdgpu_waves_per_eu(w4_waves(FM))))
+__global__ __launch_bounds__(WN *WK *kWave) __attribute__((amdgpu_waves_per_eu(w4_waves(FM, SWIGLU ? 2 * FG + (SHIFT ? 1 : 0) : FG))))
 void gmm_w4_kernel(const W4Args p) {
     constexpr int BM = 16 * FM;
     constexpr int NF = SWIGLU ? 2 * FG + (SHIFT ? 1 : 0) : FG;
@@ -479,7 +481,13 @@ template <int FM, int FG, int WN, int WK, int G, bool ZERO>
 static int launch_w4_form(const W4Args &args, bool swiglu, hipStream_t stream) {
     if (!swiglu) return launch_w4_one<FM, 2 * FG, WN, WK, G, ZERO, false, false>(args, stream);
     if (args.n_out % 16 == 0) return launch_w4_one<FM, FG, WN, WK, G, ZERO, true, false>(args, stream);
-    return launch_w4_one<FM, (FG > 1 ? FG / 2 : 1), WN, WK, G, ZERO, true, true>(args, stream);
+    // Up columns that begin in the middle of a tile cost one fragment more, which is half a wavefront's work again where it
+    // holds one column fragment and a quarter where it holds two; two where they leave the registers for as many wavefronts.
+    // Measured, one fragment / two, in us: 8 experts of 4096 x 28688, groups of 128: 3 rows 130 / 103, 32 rows 259 / 166; with
+    // zero points and groups of 32 (three wavefronts to a SIMD instead of four), 64 experts of 2048 x 2832, 3 rows: 71 / 75;
+    // 64 rows (spills), groups of 128: 118 / 151.
+    constexpr bool kNarrow = FM == 4 || (FM == 1 && (G == 32 || (G == 64 && ZERO)));
+    return launch_w4_one<FM, (kNarrow && FG > 1 ? FG / 2 : FG), WN, WK, G, ZERO, true, true>(args, stream);
 }
 
 template <int FM, int FG, int WN, int WK>
