@@ -245,6 +245,20 @@ def test_quantisation_of_tiny_weights(zeros):
     assert not bool(bad.any()), (int(bad.sum()), bad.nonzero()[:3].tolist())
 
 
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("rows_e,N", [(5, 528), (5, 1040), (5, 4112), (5, 4128), (20, 528), (20, 2064), (20, 2080), (45, 528), (45, 1040), (45, 1056)])
+def test_forms_for_more_and_less_work(rows_e, N, group, zeros):
+    announce(test="w4_forms", rows_e=rows_e, N=N, group=group, zeros=zeros)
+    # columns x row tiles on either side of every threshold between the forms; halves of N that are and are not whole tiles
+    E, K = 40, 272
+    sizes = ragged_sizes(E, E * rows_e, seed=N) if rows_e != 45 else torch.full((E,), rows_e, dtype=torch.int64)
+    w, ref, s = _weight(E, N, K, group, zeros, seed=N + rows_e)
+    x = _rand((int(sizes.sum()), K), N)
+    _check(gg.gmm_w4(x, w, sizes), x, ref, s, sizes, group, False, False)
+    _check(gg.gmm_w4_swiglu(x, w, sizes), x, ref, s, sizes, group, True, False)
+
+
 def test_many_experts():
     announce(test="w4_many_experts")
     E, K, N = 300, 64, 32
