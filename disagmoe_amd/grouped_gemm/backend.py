@@ -252,18 +252,31 @@ def gmm_swiglu_keep(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor,
                     host_batch_sizes: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """:func:`gmm_swiglu` for a step whose gradient will be asked for: ``(h [rows, I], u [rows, 2I])``
     with ``u = gmm(a, b)`` in fp32.  Rows of ``h`` past ``sum(batch_sizes)`` are zero."""
+    device = _check_block(a, b, batch_sizes, trans_b)
+    return _swiglu_keep(a, b, _sizes_on_device(batch_sizes, device), trans_b,
+                        _state_args(device, workspace, arguments_ptr, _stream(device), _host_sizes(batch_sizes, host_batch_sizes)))
+
+
+def _check_product(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor, trans_b: bool) -> torch.device:
     device = _check_operands(a, b, torch.bfloat16)
+    assert (b.shape[2] if trans_b else b.shape[1]) == a.shape[1], "contraction length mismatch"
+    assert batch_sizes.numel() == b.shape[0]
+    return device
+
+
+def _check_block(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor, trans_b: bool) -> torch.device:
+    assert b.dim() == 3 and (b.shape[1] if trans_b else b.shape[2]) % 2 == 0, "b holds as many gate as up columns"
+    return _check_product(a, b, batch_sizes, trans_b)
+
+
+def _swiglu_keep(a, b, bs, trans_b: bool, state_args: tuple):
+    """:func:`gmm_swiglu_keep` on operands that have been checked."""
     rows, K = a.shape
-    E = b.shape[0]
     N2 = b.shape[1] if trans_b else b.shape[2]
-    assert (b.shape[2] if trans_b else b.shape[1]) == K, "contraction length mismatch"
-    assert N2 % 2 == 0 and batch_sizes.numel() == E
-    h = torch.empty((rows, N2 // 2), dtype=a.dtype, device=device)
-    u = torch.empty((rows, N2), dtype=torch.float32, device=device)
-    bs = _sizes_on_device(batch_sizes, device)
-    _call_on(device, "dmoe_gmm_swiglu_keep", a.data_ptr(), b.data_ptr(), h.data_ptr(), u.data_ptr(), bs.data_ptr(), rows, E, K, N2 // 2,
-             1 if trans_b else 0, _lib.BF16, *_state_args(device, workspace, arguments_ptr, _stream(device),
-                                                          _host_sizes(batch_sizes, host_batch_sizes)))
+    h = torch.empty((rows, N2 // 2), dtype=torch.bfloat16, device=a.device)
+    u = torch.empty((rows, N2), dtype=torch.float32, device=a.device)
+    _call_on(a.device, "dmoe_gmm_swiglu_keep", a.data_ptr(), b.data_ptr(), h.data_ptr(), u.data_ptr(), bs.data_ptr(), rows, b.shape[0], K,
+             N2 // 2, 1 if trans_b else 0, _lib.BF16, *state_args)
     return h, u
 
 
@@ -317,6 +330,15 @@ def _wgrad(a, dc, bs, state_args: tuple) -> torch.Tensor:
     db = torch.empty((E, K, N), dtype=a.dtype, device=a.device)
     _call_on(a.device, "dmoe_gmm_wgrad", a.data_ptr(), dc.data_ptr(), db.data_ptr(), bs.data_ptr(), rows, E, K, N, _lib.BF16, *state_args)
     return db
+
+
+def _gmm_zeroed(a, b, bs, trans_b: bool, state_args: tuple) -> torch.Tensor:
+    """:func:`gmm` on operands that have been checked; rows past ``sum(batch_sizes)`` are zero."""
+    (rows, K), N = a.shape, b.shape[1] if trans_b else b.shape[2]
+    c = torch.empty((rows, N), dtype=torch.bfloat16, device=a.device)
+    _call_on(a.device, "dmoe_gmm", a.data_ptr(), b.data_ptr(), c.data_ptr(), bs.data_ptr(), rows, b.shape[0], K, N, 1 if trans_b else 0,
+             _lib.BF16, *state_args)
+    return zero_rows_behind(c, bs)
 
 
 def _gmm_backward(dc, a, b, bs, trans_b: bool, need_da: bool, need_db: bool, state_args: tuple):

@@ -18,17 +18,13 @@ from torch.autograd.function import once_differentiable
 from . import backend
 
 
-def _on_device(batch_sizes: torch.Tensor, host_batch_sizes: Optional[torch.Tensor], device: torch.device):
-    """(sizes on the device, sizes on the host or None), for the forward and the backward launches alike."""
-    return backend._sizes_on_device(batch_sizes, device), backend._host_sizes(batch_sizes, host_batch_sizes)
-
-
-def _remember(ctx, device: torch.device, host: Optional[torch.Tensor], trans_b: bool, state: dict) -> None:
-    """What the backward launches take besides the saved tensors, and what has to live until then: the engine runs them on
-    the forward pass's stream, in a thread of its own where a statement costs several times what it costs here."""
-    ctx.trans_b = trans_b
-    ctx.state_args = backend._state_args(device, state["workspace"], state["arguments_ptr"], backend._stream(device), host)
-    ctx.alive = (host, state["workspace"], backend._STATE_BLOCKS.get(state["arguments_ptr"]))
+def _prepare(a: torch.Tensor, batch_sizes: torch.Tensor, host_batch_sizes: Optional[torch.Tensor], workspace, arguments_ptr):
+    """(sizes on the device, the trailing arguments of the forward and the backward launches, what those need alive): made
+    once, because the engine runs the backward pass in a thread of its own where a statement costs several times what it
+    costs here."""
+    host = backend._host_sizes(batch_sizes, host_batch_sizes)
+    state_args = backend._state_args(a.device, workspace, arguments_ptr, backend._stream(a.device), host)
+    return backend._sizes_on_device(batch_sizes, a.device), state_args, (host, workspace, backend._STATE_BLOCKS.get(arguments_ptr))
 
 
 def _check_capture(ctx) -> None:
@@ -59,11 +55,10 @@ def _once(backward):
 
 class _Gmm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, a, b, sizes, host, trans_b, state):
+    def forward(ctx, a, b, sizes, trans_b, state_args, alive):
         ctx.save_for_backward(a, b, sizes)
-        c = backend.zero_rows_behind(backend.gmm(a, b, sizes, trans_b=trans_b, host_batch_sizes=host, **state), sizes)
-        _remember(ctx, a.device, host, trans_b, state)
-        return c
+        ctx.trans_b, ctx.state_args, ctx.alive = trans_b, state_args, alive
+        return backend._gmm_zeroed(a, b, sizes, trans_b, state_args)
 
     @staticmethod
     @_once
@@ -76,10 +71,10 @@ class _Gmm(torch.autograd.Function):
 
 class _GmmSwiglu(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, a, b, sizes, host, trans_b, state):
-        h, u = backend.gmm_swiglu_keep(a, b, sizes, trans_b=trans_b, host_batch_sizes=host, **state)
+    def forward(ctx, a, b, sizes, trans_b, state_args, alive):
+        h, u = backend._swiglu_keep(a, b, sizes, trans_b, state_args)
         ctx.save_for_backward(a, b, sizes, u)
-        _remember(ctx, a.device, host, trans_b, state)
+        ctx.trans_b, ctx.state_args, ctx.alive = trans_b, state_args, alive
         return h
 
     @staticmethod
@@ -96,10 +91,10 @@ def gmm(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor, trans_b: bo
         host_batch_sizes: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Differentiable ``backend.gmm``: ``c[o_e:o_e+n_e] = a[o_e:o_e+n_e] @ b[e]`` (``b[e].T`` with
     ``trans_b``), bf16 in and out."""
-    backend._check_operands(a, b, torch.bfloat16)
+    backend._check_product(a, b, batch_sizes, trans_b)
     _check_aligned(a, b)
-    sizes, host = _on_device(batch_sizes, host_batch_sizes, a.device)
-    return _Gmm.apply(a, b, sizes, host, trans_b, dict(workspace=workspace, arguments_ptr=arguments_ptr))
+    sizes, state_args, alive = _prepare(a, batch_sizes, host_batch_sizes, workspace, arguments_ptr)
+    return _Gmm.apply(a, b, sizes, trans_b, state_args, alive)
 
 
 def gmm_swiglu(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor, trans_b: bool = False,
@@ -108,10 +103,11 @@ def gmm_swiglu(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor, tran
     """Differentiable ``backend.gmm_swiglu``: ``silu(u[:, :I]) * u[:, I:]`` for ``u = gmm(a, b)``,
     ``b [E, K, 2I]`` (``[E, 2I, K]`` with ``trans_b``).  Keeps ``u`` in fp32 (8 bytes per element of
     the result) for the backward pass; without a gradient to come it is ``backend.gmm_swiglu``."""
-    backend._check_operands(a, b, torch.bfloat16)
+    backend._check_block(a, b, batch_sizes, trans_b)
     _check_aligned(a, b)
-    sizes, host = _on_device(batch_sizes, host_batch_sizes, a.device)
     if not (torch.is_grad_enabled() and (a.requires_grad or b.requires_grad)):
+        sizes, host = backend._sizes_on_device(batch_sizes, a.device), backend._host_sizes(batch_sizes, host_batch_sizes)
         return backend.zero_rows_behind(backend.gmm_swiglu(a, b, sizes, trans_b=trans_b, workspace=workspace,
                                                            arguments_ptr=arguments_ptr, host_batch_sizes=host), sizes)
-    return _GmmSwiglu.apply(a, b, sizes, host, trans_b, dict(workspace=workspace, arguments_ptr=arguments_ptr))
+    sizes, state_args, alive = _prepare(a, batch_sizes, host_batch_sizes, workspace, arguments_ptr)
+    return _GmmSwiglu.apply(a, b, sizes, trans_b, state_args, alive)
