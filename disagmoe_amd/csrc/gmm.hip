@@ -481,6 +481,19 @@ int bind_state(GmmArgs &args, void *state, void *workspace, size_t workspace_byt
     return DMOE_OK;
 }
 
+// One mutex for every workspace but for those that share a place of the table, which wait for each other needlessly.
+static std::mutex *turn_of(const void *workspace) {
+    static std::mutex table[64];
+    const uintptr_t at = (uintptr_t)workspace >> 8;
+    return table + (at ^ at >> 6 ^ at >> 12 ^ at >> 18) % 64;
+}
+WorkspaceTurn::WorkspaceTurn(const GmmArgs &args) : held_(args.partials != nullptr ? turn_of(args.partials) : nullptr) {
+    if (held_ != nullptr) held_->lock();
+}
+WorkspaceTurn::~WorkspaceTurn() {
+    if (held_ != nullptr) held_->unlock();
+}
+
 // Kernel, tile rows and grid of a launch, from what the host knows (the shapes, not how the rows split over the experts).
 // The one place where that is decided: launch_by_rows dispatches on the result and dmoe_gmm_plan reports it.
 static GmmLaunch choose_launch(const GmmArgs &args, bool trans_b, bool swiglu, bool fp8) {
@@ -698,6 +711,7 @@ extern "C" int dmoe_gmm(const void *a, const void *b, void *c, const int64_t *ba
     GmmArgs args{(const char *)a, (const char *)b, (char *)c, batch_sizes, nullptr, nullptr, rows, E, (int)K, (int)N, (int)N};
     rc = bind_state(args, state, workspace, workspace_bytes, (hipStream_t)stream);
     if (rc != DMOE_OK) return rc;
+    const WorkspaceTurn turn(args);
     return trans_b ? launch_by_rows<true, false, false>(args, (hipStream_t)stream)
                    : launch_by_rows<false, false, false>(args, (hipStream_t)stream);
 }
@@ -713,6 +727,7 @@ extern "C" int dmoe_gmm_swiglu(const void *a, const void *b, void *h, const int6
     GmmArgs args{(const char *)a, (const char *)b, (char *)h, batch_sizes, nullptr, nullptr, rows, E, (int)K, (int)(2 * I), (int)I};
     rc = bind_state(args, state, workspace, workspace_bytes, (hipStream_t)stream);
     if (rc != DMOE_OK) return rc;
+    const WorkspaceTurn turn(args);
     return trans_b ? launch_by_rows<true, true, false>(args, (hipStream_t)stream)
                    : launch_by_rows<false, true, false>(args, (hipStream_t)stream);
 }
@@ -731,6 +746,7 @@ extern "C" int dmoe_gmm_swiglu_keep(const void *a, const void *b, void *h, float
     GmmArgs args{(const char *)a, (const char *)b, (char *)h, batch_sizes, nullptr, nullptr, rows, E, (int)K, (int)(2 * I), (int)I};
     rc = bind_state(args, state, workspace, workspace_bytes, (hipStream_t)stream);
     if (rc != DMOE_OK) return rc;
+    const WorkspaceTurn turn(args);
     args.u = u;
     rc = trans_b ? launch_keep<true>(args, (hipStream_t)stream) : launch_keep<false>(args, (hipStream_t)stream);
     if (rc != DMOE_OK) return rc;
@@ -751,6 +767,7 @@ extern "C" int dmoe_gmm_wgrad(const void *a, const void *dc, void *db, const int
     GmmArgs args{(const char *)a, (const char *)dc, (char *)db, batch_sizes, nullptr, nullptr, rows, E, (int)K, (int)N, (int)N};
     rc = bind_state(args, state, workspace, workspace_bytes, (hipStream_t)stream);
     if (rc != DMOE_OK) return rc;
+    const WorkspaceTurn turn(args);
     return launch_wgrad(args, (hipStream_t)stream);
 }
 
@@ -774,6 +791,7 @@ extern "C" int dmoe_gmm_swiglu_backward(const void *dh, const float *u, const vo
             const HostSizes known(host_batch_sizes);
             GmmArgs args{(const char *)du, (const char *)b, (char *)da, batch_sizes, nullptr, nullptr, rows, E, (int)(2 * I), (int)K, (int)K};
             rc = bind_state(args, state, workspace, workspace_bytes, (hipStream_t)stream);
+            const WorkspaceTurn turn(args);
             const int tail = tail_rows(args, choose_launch(args, !trans_b, false, false), !trans_b, false);
             if (rc == DMOE_OK && tail != 0)
                 rc = launch_tail(args, tail, !trans_b, false, (hipStream_t)stream);
@@ -803,6 +821,7 @@ extern "C" int dmoe_gmm_swiglu_rows(const void *x, const int32_t *row_token, int
     GmmArgs args{(const char *)x, (const char *)b, (char *)h, batch_sizes, nullptr, nullptr, rows, E, (int)K, (int)(2 * I), (int)I};
     rc = bind_state(args, state, workspace, workspace_bytes, (hipStream_t)stream);
     if (rc != DMOE_OK) return rc;
+    const WorkspaceTurn turn(args);
     args.a_rows = row_token;
     args.a_src_rows = T;
     return launch_tile256_rows(args, (hipStream_t)stream);
@@ -819,6 +838,7 @@ extern "C" int dmoe_gmm_fp8(const void *a, const float *a_scale, const void *b, 
     GmmArgs args{(const char *)a, (const char *)b, (char *)c, batch_sizes, a_scale, b_scale, rows, E, (int)K, (int)N, (int)N};
     rc = bind_state(args, state, workspace, workspace_bytes, (hipStream_t)stream);
     if (rc != DMOE_OK) return rc;
+    const WorkspaceTurn turn(args);
     return launch_by_rows<true, false, true>(args, (hipStream_t)stream);
 }
 
@@ -834,5 +854,6 @@ extern "C" int dmoe_gmm_fp8_swiglu(const void *a, const float *a_scale, const vo
     GmmArgs args{(const char *)a, (const char *)b, (char *)h, batch_sizes, a_scale, b_scale, rows, E, (int)K, (int)(2 * I), (int)I};
     rc = bind_state(args, state, workspace, workspace_bytes, (hipStream_t)stream);
     if (rc != DMOE_OK) return rc;
+    const WorkspaceTurn turn(args);
     return launch_by_rows<true, true, true>(args, (hipStream_t)stream);
 }

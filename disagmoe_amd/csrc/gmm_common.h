@@ -2,6 +2,7 @@
 // device-side work list (expert, m-tile, n-tile) derived from batch_sizes.
 #pragma once
 
+#include <mutex>
 #include <type_traits>
 
 #include "common.h"
@@ -377,6 +378,20 @@ int launch_wgrad(const GmmArgs &args, hipStream_t stream);
 int launch_tail(const GmmArgs &args, int tile_rows, bool trans_b, bool keep, hipStream_t stream);
 int launch_tile256_half(const GmmArgs &args, bool swiglu, hipStream_t stream);
 int bind_state(GmmArgs &args, void *state, void *workspace, size_t workspace_bytes, hipStream_t stream);
+// Held from bind_state until the launches of a call are on their stream.  A weight gradient whose contraction is cut takes two
+// launches, and the workspace holds its pieces between them; autograd runs backward passes in a thread of its own, on the
+// stream and with the workspace that the caller's thread launches on as well.  A launch with partial sums in that workspace must
+// not come between the two.  (Without a workspace nothing is held.)
+class WorkspaceTurn {
+public:
+    explicit WorkspaceTurn(const GmmArgs &args);
+    ~WorkspaceTurn();
+    WorkspaceTurn(const WorkspaceTurn &) = delete;
+    WorkspaceTurn &operator=(const WorkspaceTurn &) = delete;
+
+private:
+    std::mutex *held_;
+};
 // The caller's copy of the sizes on the host for the length of one call.
 struct HostSizes {
     explicit HostSizes(const int64_t *p) { t_host_sizes = p; }

@@ -285,6 +285,7 @@ static int gmm_w4(const char *who, const void *a, const void *codes, const void 
         GmmArgs args{w + at.rows, w + at.weights, (char *)c, batch_sizes, (const float *)(w + at.row_scales), (const float *)(w + at.col_scales), rows, E,
                      (int)Kp, (int)N, (int)n_out};
         rc = bind_state(args, state, workspace, workspace_bytes, (hipStream_t)stream);
+        const WorkspaceTurn turn(args);
         return rc != DMOE_OK ? rc : launch_tile256_half(args, swiglu, (hipStream_t)stream);
     }
     W4Args args{(const char *)a, (const char *)codes, (const char *)scales, (const char *)zeros, (char *)c, batch_sizes, rows, E, (int)K, (int)N,

@@ -34,9 +34,10 @@ def _sizes_on_device(batch_sizes: torch.Tensor, device: torch.device) -> torch.T
 # Footprint: a state block is 33 KB; a workspace of the size ``get_arguments``
 # states is 2 x (compute units) x 256 KiB = 128 MiB on a 256-CU device.  Launches
 # that follow each other on one stream can share one workspace (it carries nothing
-# from one launch to the next), so layers should take ``shared_workspace`` rather
-# than allocate one each; only launches that may overlap in time (graphs replayed
-# on different streams) need workspaces of their own.
+# from one call to the next; a weight gradient's two launches are kept together by
+# the library, whichever threads launch on the stream), so layers should take
+# ``shared_workspace`` rather than allocate one each; only launches that may overlap
+# in time (graphs replayed on different streams) need workspaces of their own.
 
 _STATE_BLOCKS = {}     # address -> the zeroed uint8 tensor behind an arguments_ptr
 _DEFAULTS = {}         # (device index, stream handle) -> (state block, workspace)

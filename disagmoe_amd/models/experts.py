@@ -19,7 +19,7 @@ class _GemmState:
 
     The 33 KB state block (work counters) is the layer's own: a recorded graph of the layer then shares
     its scheduler state with no other launch.  The workspace (fp32 partial sums of tiles cut along K,
-    128 MiB on a 256-CU device) carries nothing from one launch to the next, so eager launches use the
+    128 MiB on a 256-CU device) carries nothing from one call to the next, so eager launches use the
     one the backend keeps for the stream they run on, shared by every layer that runs there.  A layer
     gets a workspace of its own when one is passed in (``workspace=``; the caller may hand the same
     tensor to layers whose launches never overlap in time), with ``own_workspace=True``, or when it

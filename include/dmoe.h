@@ -247,6 +247,9 @@ int dmoe_combine(const void *y, const void *mappings, int map_type, const float 
  *              dmoe_gmm_workspace_bytes() is the size at which no launch is short
  *              of room for that; a smaller one (or NULL) cuts less (or nothing).
  * Launches that may overlap in time must not share a state block or a workspace.
+ * Host threads that launch on one stream may share both: the launches of a call that
+ * keeps sums in the workspace from one to the next (dmoe_gmm_wgrad) go onto the stream
+ * with no other launch of that workspace between them.
  * state == NULL: counters of the library's own, one set per stream (at most 64
  * streams per device), nothing is cut; refused with DMOE_ERR_WORKSPACE while
  * `stream` is being captured into a graph, whose replays may run beside anything.
