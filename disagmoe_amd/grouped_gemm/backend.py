@@ -65,8 +65,7 @@ def _default_pair(device: torch.device, stream: int):
                                "get_arguments() (and a workspace), as MoEExperts does")
         with torch.cuda.device(device):
             state, ws = _new_state_block(device), torch.empty(workspace_bytes(), dtype=torch.uint8, device=device)
-        pair = (state, ws)
-        _DEFAULTS[key] = pair
+        pair = _DEFAULTS.setdefault(key, (state, ws))   # (another thread may have been first: its pair is in use already)
     return pair
 
 
