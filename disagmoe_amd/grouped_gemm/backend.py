@@ -80,7 +80,8 @@ def shared_workspace(device: torch.device, stream: Optional[int] = None) -> torc
 def _state_args(device: torch.device, workspace: Optional[torch.Tensor], arguments_ptr: Optional[int], stream: int,
                 host_sizes: Optional[torch.Tensor] = None):
     """The trailing arguments of a dmoe_gmm* call: state block, workspace and its size, the host copy of the sizes
-    (or NULL), the stream."""
+    (or NULL), the stream.  They are addresses: the caller keeps ``host_sizes``, which may be a converted copy of its own,
+    until the library has read it."""
     return (*_state_triple(device, workspace, arguments_ptr, stream),
             None if host_sizes is None else host_sizes.data_ptr(), stream)
 
@@ -176,11 +177,10 @@ def gmm(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor, trans_b: bo
     else:
         assert c.is_contiguous() and c.dtype == a.dtype and c.device == device
         assert c.dim() == 2 and c.shape[1] == N and c.shape[0] >= rows
-    bs = _sizes_on_device(batch_sizes, device)
+    bs, host = _sizes_on_device(batch_sizes, device), _host_sizes(batch_sizes, host_batch_sizes)
     with torch.cuda.device(device):
         _lib.call("dmoe_gmm", a.data_ptr(), b.data_ptr(), c.data_ptr(), bs.data_ptr(), rows, E, K, N,
-                  1 if trans_b else 0, _lib.BF16, *_state_args(device, workspace, arguments_ptr, _stream(device),
-                               _host_sizes(batch_sizes, host_batch_sizes)))
+                  1 if trans_b else 0, _lib.BF16, *_state_args(device, workspace, arguments_ptr, _stream(device), host))
     return c
 
 
@@ -202,11 +202,10 @@ def gmm_swiglu(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor, tran
         c = torch.empty((rows, inter), dtype=a.dtype, device=device)
     else:
         assert c.is_contiguous() and c.dtype == a.dtype and c.shape[1] == inter and c.shape[0] >= rows
-    bs = _sizes_on_device(batch_sizes, device)
+    bs, host = _sizes_on_device(batch_sizes, device), _host_sizes(batch_sizes, host_batch_sizes)
     with torch.cuda.device(device):
         _lib.call("dmoe_gmm_swiglu", a.data_ptr(), b.data_ptr(), c.data_ptr(), bs.data_ptr(), rows, E, K, inter,
-                  1 if trans_b else 0, _lib.BF16, *_state_args(device, workspace, arguments_ptr, _stream(device),
-                               _host_sizes(batch_sizes, host_batch_sizes)))
+                  1 if trans_b else 0, _lib.BF16, *_state_args(device, workspace, arguments_ptr, _stream(device), host))
     return c
 
 
@@ -227,11 +226,10 @@ def gmm_swiglu_rows(x: torch.Tensor, row_token: torch.Tensor, b: torch.Tensor, b
         c = torch.empty((rows, inter), dtype=x.dtype, device=device)
     else:
         assert c.is_contiguous() and c.dtype == x.dtype and c.shape[1] == inter and c.shape[0] >= rows
-    bs = _sizes_on_device(batch_sizes, device)
+    bs, host = _sizes_on_device(batch_sizes, device), _host_sizes(batch_sizes, host_batch_sizes)
     with torch.cuda.device(device):
         _lib.call("dmoe_gmm_swiglu_rows", x.data_ptr(), row_token.data_ptr(), T, b.data_ptr(), c.data_ptr(), bs.data_ptr(),
-                  rows, E, K, inter, _lib.BF16, *_state_args(device, workspace, arguments_ptr, _stream(device),
-                               _host_sizes(batch_sizes, host_batch_sizes)))
+                  rows, E, K, inter, _lib.BF16, *_state_args(device, workspace, arguments_ptr, _stream(device), host))
     return c
 
 
@@ -253,8 +251,9 @@ def gmm_swiglu_keep(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor,
     """:func:`gmm_swiglu` for a step whose gradient will be asked for: ``(h [rows, I], u [rows, 2I])``
     with ``u = gmm(a, b)`` in fp32.  Rows of ``h`` past ``sum(batch_sizes)`` are zero."""
     device = _check_block(a, b, batch_sizes, trans_b)
+    host = _host_sizes(batch_sizes, host_batch_sizes)
     return _swiglu_keep(a, b, _sizes_on_device(batch_sizes, device), trans_b,
-                        _state_args(device, workspace, arguments_ptr, _stream(device), _host_sizes(batch_sizes, host_batch_sizes)))
+                        _state_args(device, workspace, arguments_ptr, _stream(device), host))
 
 
 def _check_product(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor, trans_b: bool) -> torch.device:
@@ -293,9 +292,9 @@ def gmm_swiglu_backward(dh: torch.Tensor, u: torch.Tensor, a: torch.Tensor, b: t
     assert dh.shape == (rows, inter) and u.shape == (rows, 2 * inter), "dh is [rows, I], u is [rows, 2I]"
     assert dh.dtype == torch.bfloat16 and u.dtype == torch.float32 and dh.device == device and u.device == device
     assert dh.is_contiguous() and u.is_contiguous()
-    bs = _sizes_on_device(batch_sizes, device)
+    bs, host = _sizes_on_device(batch_sizes, device), _host_sizes(batch_sizes, host_batch_sizes)
     return _swiglu_backward(dh, u, a, b, bs, trans_b, need_da, need_db,
-                            _state_args(device, workspace, arguments_ptr, _stream(device), _host_sizes(batch_sizes, host_batch_sizes)))
+                            _state_args(device, workspace, arguments_ptr, _stream(device), host))
 
 
 def _swiglu_backward(dh, u, a, b, bs, trans_b: bool, need_da: bool, need_db: bool, state_args: tuple):
@@ -320,8 +319,9 @@ def gmm_wgrad(a: torch.Tensor, dc: torch.Tensor, batch_sizes: torch.Tensor, work
     assert a.dim() == 2 and dc.dim() == 2 and a.shape[0] == dc.shape[0], "a is [rows, K], dc is [rows, N]"
     assert a.dtype == torch.bfloat16 and dc.dtype == torch.bfloat16 and a.device == dc.device
     assert a.is_contiguous() and dc.is_contiguous()
+    host = _host_sizes(batch_sizes, host_batch_sizes)
     return _wgrad(a, dc, _sizes_on_device(batch_sizes, a.device),
-                  _state_args(a.device, workspace, arguments_ptr, _stream(a.device), _host_sizes(batch_sizes, host_batch_sizes)))
+                  _state_args(a.device, workspace, arguments_ptr, _stream(a.device), host))
 
 
 def _wgrad(a, dc, bs, state_args: tuple) -> torch.Tensor:
@@ -457,12 +457,11 @@ def gmm_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: to
     rows, K, E, N = _fp8_common(a, a_scale, b, b_scale)
     if c is None:
         c = torch.empty((rows, N), dtype=torch.bfloat16, device=a.device)
-    bs = _sizes_on_device(batch_sizes, a.device)
+    bs, host = _sizes_on_device(batch_sizes, a.device), _host_sizes(batch_sizes, host_batch_sizes)
     with torch.cuda.device(a.device):
         _lib.call("dmoe_gmm_fp8", a.data_ptr(), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(), c.data_ptr(),
                   bs.data_ptr(), rows, E, K, N,
-                  *_state_args(a.device, workspace, arguments_ptr, _stream(a.device),
-                               _host_sizes(batch_sizes, host_batch_sizes)))
+                  *_state_args(a.device, workspace, arguments_ptr, _stream(a.device), host))
     return c
 
 
@@ -475,12 +474,11 @@ def gmm_fp8_swiglu(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_sc
     assert N2 % 2 == 0
     if c is None:
         c = torch.empty((rows, N2 // 2), dtype=torch.bfloat16, device=a.device)
-    bs = _sizes_on_device(batch_sizes, a.device)
+    bs, host = _sizes_on_device(batch_sizes, a.device), _host_sizes(batch_sizes, host_batch_sizes)
     with torch.cuda.device(a.device):
         _lib.call("dmoe_gmm_fp8_swiglu", a.data_ptr(), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(),
                   c.data_ptr(), bs.data_ptr(), rows, E, K, N2 // 2,
-                  *_state_args(a.device, workspace, arguments_ptr, _stream(a.device),
-                               _host_sizes(batch_sizes, host_batch_sizes)))
+                  *_state_args(a.device, workspace, arguments_ptr, _stream(a.device), host))
     return c
 
 
