@@ -6,13 +6,15 @@ Gradients are bf16 like the operands, each sum taken in fp32 and rounded once.  
 an expert without rows has a zero gradient.  ``workspace`` and ``arguments_ptr``
 (``backend.get_arguments``) serve the forward and the backward launches, which follow each other
 on the stream the forward ran on; a step that is captured into a graph has to bring them, as
-``backend.gmm`` does.  The gradients themselves are not differentiable.
+``backend.gmm`` does.  The gradients themselves are not differentiable, and there is no
+forward-mode derivative: both are refused.
 """
 from __future__ import annotations
 
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import backend
@@ -36,6 +38,11 @@ def _check_capture(ctx) -> None:
 def _check_aligned(a: torch.Tensor, b: torch.Tensor) -> None:
     if (a.data_ptr() | b.data_ptr()) & 15:
         raise ValueError("a and b must be 16-byte aligned")
+
+
+def _has_tangent(x: torch.Tensor) -> bool:
+    """Whether ``x`` carries a forward-mode derivative (which torch refuses of the functions below)."""
+    return forward_ad.unpack_dual(x).tangent is not None
 
 
 def _gradient(dc: torch.Tensor) -> torch.Tensor:
@@ -105,7 +112,7 @@ def gmm_swiglu(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor, tran
     the result) for the backward pass; without a gradient to come it is ``backend.gmm_swiglu``."""
     backend._check_block(a, b, batch_sizes, trans_b)
     _check_aligned(a, b)
-    if not (torch.is_grad_enabled() and (a.requires_grad or b.requires_grad)):
+    if not (torch.is_grad_enabled() and (a.requires_grad or b.requires_grad) or _has_tangent(a) or _has_tangent(b)):
         sizes, host = backend._sizes_on_device(batch_sizes, a.device), backend._host_sizes(batch_sizes, host_batch_sizes)
         return backend.zero_rows_behind(backend.gmm_swiglu(a, b, sizes, trans_b=trans_b, workspace=workspace,
                                                            arguments_ptr=arguments_ptr, host_batch_sizes=host), sizes)

@@ -5,8 +5,10 @@ import weakref
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from disagmoe_amd.grouped_gemm import backend as gg
+from disagmoe_amd.grouped_gemm import ops
 
 
 def test_threads_that_first_launch_on_one_stream_share_its_pair(monkeypatch):
@@ -94,3 +96,20 @@ def test_host_sizes_live_until_the_call_has_read_them(monkeypatch, name, kind):
     _fake_device(monkeypatch, called)
     _products()[name](sizes)
     assert reads == [True]
+
+
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(monkeypatch, which, grad):
+    """The products have no forward-mode derivative: an operand with a tangent is refused, not taken without it."""
+    _fake_device(monkeypatch, lambda name, args: None)
+    monkeypatch.setattr(gg, "_check_operands", lambda a, b, dtype: a.device)
+    monkeypatch.setattr(gg, "zero_rows_behind", lambda c, sizes: c)
+    operands = [torch.zeros(8, 32, dtype=torch.bfloat16), torch.zeros(3, 32, 64, dtype=torch.bfloat16)]
+    n = torch.tensor(SIZES)
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        assert ops.gmm_swiglu(*operands, n).shape == (8, 32)          # nothing has a tangent
+        operands[which] = forward_ad.make_dual(operands[which], torch.ones_like(operands[which]))
+        for product in (ops.gmm, ops.gmm_swiglu):
+            with pytest.raises(NotImplementedError):
+                product(*operands, n)
