@@ -55,8 +55,7 @@ def _table(grads: List[torch.Tensor]):
     return device, table
 
 
-def _run(name: str, grads: Union[torch.Tensor, Iterable[torch.Tensor]], *limit) -> torch.Tensor:
-    grads = [grads] if torch.is_tensor(grads) else list(grads)
+def _run(name: str, grads: List[torch.Tensor], *limit) -> torch.Tensor:
     if not grads:
         return torch.zeros(())
     device, table = _table(grads)
@@ -74,19 +73,24 @@ def global_norm(grads: Union[torch.Tensor, Iterable[torch.Tensor]]) -> torch.Ten
     """``sqrt(sum of g^2)`` over every element of all gradients (fp32, bf16, fp16, mixed;
     any sizes; dense, on one device), summed in 64 bits in a fixed order.  A 0-dimensional
     fp32 device tensor; an empty list has norm 0 (on the host)."""
-    return _run("dmoe_grad_norm", grads)
+    return _run("dmoe_grad_norm", [grads] if torch.is_tensor(grads) else list(grads))
 
 
 @torch.no_grad()
 def clip_by_global_norm_(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float) -> torch.Tensor:
     """Scales all gradients in place by ``min(1, max_norm / (norm + 1e-6))`` and returns
     their :func:`global_norm` before that.  Gradients whose norm is below the limit are not
-    written.  A norm that is infinite or NaN is treated as torch.nn.utils.clip_grad_norm_ treats it:
+    written (to autograd they are modified in place all the same: the host does not wait for the
+    norm).  A norm that is infinite or NaN is treated as torch.nn.utils.clip_grad_norm_ treats it:
     a factor of zero, or NaN.  No two gradients may share memory."""
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
-    return _run("dmoe_clip_grads", grads, max_norm)
+    grads = [grads] if torch.is_tensor(grads) else list(grads)
+    norm = _run("dmoe_clip_grads", grads, max_norm)
+    # written through their addresses, which autograd does not see: what saved one of them has to notice
+    torch.autograd.graph.increment_version(grads)
+    return norm
 
 
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float) -> torch.Tensor:
