@@ -147,6 +147,12 @@ def launch_plan(rows: int, num_experts: int, K: int, N: int, swiglu: bool = Fals
     return plan
 
 
+def _modified(c: torch.Tensor) -> torch.Tensor:
+    """``c``, which a call has written through its address: autograd, which did not see that, is told."""
+    torch.autograd.graph.increment_version(c)
+    return c
+
+
 def _check_operands(a: torch.Tensor, b: torch.Tensor, dtype: torch.dtype) -> torch.device:
     if not a.is_cuda:
         raise RuntimeError("gmm needs device tensors; disagmoe_amd has no CPU fallback")
@@ -172,7 +178,8 @@ def gmm(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor, trans_b: bo
     N = b.shape[1] if trans_b else b.shape[2]
     assert (b.shape[2] if trans_b else b.shape[1]) == K, "contraction length mismatch"
     assert batch_sizes.numel() == E
-    if c is None:
+    given = c is not None
+    if not given:
         c = torch.empty((rows, N), dtype=a.dtype, device=device)
     else:
         assert c.is_contiguous() and c.dtype == a.dtype and c.device == device
@@ -181,7 +188,7 @@ def gmm(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor, trans_b: bo
     with torch.cuda.device(device):
         _lib.call("dmoe_gmm", a.data_ptr(), b.data_ptr(), c.data_ptr(), bs.data_ptr(), rows, E, K, N,
                   1 if trans_b else 0, _lib.BF16, *_state_args(device, workspace, arguments_ptr, _stream(device), host))
-    return c
+    return _modified(c) if given else c
 
 
 def gmm_swiglu(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor, trans_b: bool = False,
@@ -198,7 +205,8 @@ def gmm_swiglu(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor, tran
     assert (b.shape[2] if trans_b else b.shape[1]) == K, "contraction length mismatch"
     assert N2 % 2 == 0 and batch_sizes.numel() == E
     inter = N2 // 2
-    if c is None:
+    given = c is not None
+    if not given:
         c = torch.empty((rows, inter), dtype=a.dtype, device=device)
     else:
         assert c.is_contiguous() and c.dtype == a.dtype and c.shape[1] == inter and c.shape[0] >= rows
@@ -206,7 +214,7 @@ def gmm_swiglu(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor, tran
     with torch.cuda.device(device):
         _lib.call("dmoe_gmm_swiglu", a.data_ptr(), b.data_ptr(), c.data_ptr(), bs.data_ptr(), rows, E, K, inter,
                   1 if trans_b else 0, _lib.BF16, *_state_args(device, workspace, arguments_ptr, _stream(device), host))
-    return c
+    return _modified(c) if given else c
 
 
 def gmm_swiglu_rows(x: torch.Tensor, row_token: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor,
@@ -222,7 +230,8 @@ def gmm_swiglu_rows(x: torch.Tensor, row_token: torch.Tensor, b: torch.Tensor, b
     assert Kb == K and N2 % 2 == 0 and batch_sizes.numel() == E
     assert row_token.dtype == torch.int32 and row_token.is_contiguous() and row_token.device == device
     rows, inter = row_token.numel(), N2 // 2
-    if c is None:
+    given = c is not None
+    if not given:
         c = torch.empty((rows, inter), dtype=x.dtype, device=device)
     else:
         assert c.is_contiguous() and c.dtype == x.dtype and c.shape[1] == inter and c.shape[0] >= rows
@@ -230,7 +239,7 @@ def gmm_swiglu_rows(x: torch.Tensor, row_token: torch.Tensor, b: torch.Tensor, b
     with torch.cuda.device(device):
         _lib.call("dmoe_gmm_swiglu_rows", x.data_ptr(), row_token.data_ptr(), T, b.data_ptr(), c.data_ptr(), bs.data_ptr(),
                   rows, E, K, inter, _lib.BF16, *_state_args(device, workspace, arguments_ptr, _stream(device), host))
-    return c
+    return _modified(c) if given else c
 
 
 # ---- gradients: no counterpart in the reference ------------------------------
@@ -338,7 +347,7 @@ def _gmm_zeroed(a, b, bs, trans_b: bool, state_args: tuple) -> torch.Tensor:
     c = torch.empty((rows, N), dtype=torch.bfloat16, device=a.device)
     _call_on(a.device, "dmoe_gmm", a.data_ptr(), b.data_ptr(), c.data_ptr(), bs.data_ptr(), rows, b.shape[0], K, N, 1 if trans_b else 0,
              _lib.BF16, *state_args)
-    return zero_rows_behind(c, bs)
+    return _zero_rows_behind(c, bs)
 
 
 def _gmm_backward(dc, a, b, bs, trans_b: bool, need_da: bool, need_db: bool, state_args: tuple):
@@ -348,7 +357,7 @@ def _gmm_backward(dc, a, b, bs, trans_b: bool, need_da: bool, need_db: bool, sta
         da = torch.empty_like(a)
         _call_on(a.device, "dmoe_gmm", dc.data_ptr(), b.data_ptr(), da.data_ptr(), bs.data_ptr(), a.shape[0], b.shape[0], dc.shape[1], a.shape[1],
                  0 if trans_b else 1, _lib.BF16, *state_args)
-        zero_rows_behind(da, bs)
+        _zero_rows_behind(da, bs)
     if need_db:
         db = _wgrad(dc, a, bs, state_args) if trans_b else _wgrad(a, dc, bs, state_args)
     return da, db
@@ -357,7 +366,11 @@ def _gmm_backward(dc, a, b, bs, trans_b: bool, need_da: bool, need_db: bool, sta
 def zero_rows_behind(c: torch.Tensor, batch_sizes: torch.Tensor) -> torch.Tensor:
     """Zeros in the rows of ``c [rows, d]`` past ``sum(batch_sizes)``, which the products leave as they are."""
     assert c.is_cuda and c.dim() == 2 and c.is_contiguous() and c.dtype in (torch.bfloat16, torch.float16)
-    bs = _sizes_on_device(batch_sizes, c.device)
+    return _modified(_zero_rows_behind(c, _sizes_on_device(batch_sizes, c.device)))
+
+
+def _zero_rows_behind(c: torch.Tensor, bs: torch.Tensor) -> torch.Tensor:
+    """:func:`zero_rows_behind` on a result that nobody has seen yet."""
     _call_on(c.device, "dmoe_zero_rows_behind", c.data_ptr(), bs.data_ptr(), c.shape[0], bs.numel(), c.shape[1],
              _lib.BF16 if c.dtype == torch.bfloat16 else _lib.FP16, _stream(c.device))
     return c
@@ -455,14 +468,15 @@ def gmm_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: to
     """``c = (a @ b[e].T) * a_scale[:, None] * b_scale[e][None, :]`` in bf16; ``a``
     fp8 ``[rows, K]``, ``b`` fp8 ``[E, N, K]``."""
     rows, K, E, N = _fp8_common(a, a_scale, b, b_scale)
-    if c is None:
+    given = c is not None
+    if not given:
         c = torch.empty((rows, N), dtype=torch.bfloat16, device=a.device)
     bs, host = _sizes_on_device(batch_sizes, a.device), _host_sizes(batch_sizes, host_batch_sizes)
     with torch.cuda.device(a.device):
         _lib.call("dmoe_gmm_fp8", a.data_ptr(), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(), c.data_ptr(),
                   bs.data_ptr(), rows, E, K, N,
                   *_state_args(a.device, workspace, arguments_ptr, _stream(a.device), host))
-    return c
+    return _modified(c) if given else c
 
 
 def gmm_fp8_swiglu(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
@@ -472,14 +486,15 @@ def gmm_fp8_swiglu(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_sc
     K]``; returns bf16 ``[rows, I]``."""
     rows, K, E, N2 = _fp8_common(a, a_scale, b, b_scale)
     assert N2 % 2 == 0
-    if c is None:
+    given = c is not None
+    if not given:
         c = torch.empty((rows, N2 // 2), dtype=torch.bfloat16, device=a.device)
     bs, host = _sizes_on_device(batch_sizes, a.device), _host_sizes(batch_sizes, host_batch_sizes)
     with torch.cuda.device(a.device):
         _lib.call("dmoe_gmm_fp8_swiglu", a.data_ptr(), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(),
                   c.data_ptr(), bs.data_ptr(), rows, E, K, N2 // 2,
                   *_state_args(a.device, workspace, arguments_ptr, _stream(a.device), host))
-    return c
+    return _modified(c) if given else c
 
 
 # ---- 4-bit weights with group scales: no counterpart in the reference --------
@@ -583,7 +598,8 @@ def _gmm_w4(name: str, a: torch.Tensor, w: W4Weight, n_out: int, batch_sizes: to
     rows = a.shape[0]
     assert a.shape[1] == w.K, "contraction length mismatch"
     assert batch_sizes.numel() == E
-    if c is None:
+    given = c is not None
+    if not given:
         c = torch.empty((rows, n_out), dtype=a.dtype, device=device)
     else:
         assert c.is_contiguous() and c.dtype == a.dtype and c.device == device
@@ -601,7 +617,7 @@ def _gmm_w4(name: str, a: torch.Tensor, w: W4Weight, n_out: int, batch_sizes: to
             more = (None, 0, None, None, 0)
         _lib.call(name, a.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), _zeros_ptr(w), w.group, c.data_ptr(), bs.data_ptr(),
                   rows, E, w.K, n_out, *more, host_ptr, stream)
-    return c
+    return _modified(c) if given else c
 
 
 def gmm_w4(a: torch.Tensor, w: W4Weight, batch_sizes: torch.Tensor, c: Optional[torch.Tensor] = None,

@@ -114,7 +114,7 @@ def gmm_swiglu(a: torch.Tensor, b: torch.Tensor, batch_sizes: torch.Tensor, tran
     _check_aligned(a, b)
     if not (torch.is_grad_enabled() and (a.requires_grad or b.requires_grad) or _has_tangent(a) or _has_tangent(b)):
         sizes, host = backend._sizes_on_device(batch_sizes, a.device), backend._host_sizes(batch_sizes, host_batch_sizes)
-        return backend.zero_rows_behind(backend.gmm_swiglu(a, b, sizes, trans_b=trans_b, workspace=workspace,
-                                                           arguments_ptr=arguments_ptr, host_batch_sizes=host), sizes)
+        return backend._zero_rows_behind(backend.gmm_swiglu(a, b, sizes, trans_b=trans_b, workspace=workspace,
+                                                            arguments_ptr=arguments_ptr, host_batch_sizes=host), sizes)
     sizes, state_args, alive = _prepare(a, batch_sizes, host_batch_sizes, workspace, arguments_ptr)
     return _GmmSwiglu.apply(a, b, sizes, trans_b, state_args, alive)

@@ -210,12 +210,15 @@ def gather_row_ptrs(row_ptrs: torch.Tensor, hidden_size: int, dtype: torch.dtype
     assert row_ptrs.is_cuda and row_ptrs.dtype in (torch.int64, torch.uint64)
     device = row_ptrs.device
     n = row_ptrs.numel()
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty((n, hidden_size), dtype=dtype, device=device)
     assert out.is_contiguous() and out.shape == (n, hidden_size) and out.dtype == dtype
     with torch.cuda.device(device):
         _lib.call("dmoe_gather_ptrs", row_ptrs.data_ptr(), out.data_ptr(), n, hidden_size, _row_dtype(out),
                   _stream(device))
+    if given:
+        torch.autograd.graph.increment_version(out)   # written through its address
     return out
 
 

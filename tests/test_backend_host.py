@@ -9,6 +9,7 @@ from torch.autograd import forward_ad
 
 from disagmoe_amd.grouped_gemm import backend as gg
 from disagmoe_amd.grouped_gemm import ops
+from disagmoe_amd.ops import memory
 
 
 def test_threads_that_first_launch_on_one_stream_share_its_pair(monkeypatch):
@@ -104,7 +105,6 @@ def test_forward_mode_is_refused(monkeypatch, which, grad):
     """The products have no forward-mode derivative: an operand with a tangent is refused, not taken without it."""
     _fake_device(monkeypatch, lambda name, args: None)
     monkeypatch.setattr(gg, "_check_operands", lambda a, b, dtype: a.device)
-    monkeypatch.setattr(gg, "zero_rows_behind", lambda c, sizes: c)
     operands = [torch.zeros(8, 32, dtype=torch.bfloat16), torch.zeros(3, 32, 64, dtype=torch.bfloat16)]
     n = torch.tensor(SIZES)
     with forward_ad.dual_level(), torch.set_grad_enabled(grad):
@@ -113,3 +113,41 @@ def test_forward_mode_is_refused(monkeypatch, which, grad):
         for product in (ops.gmm, ops.gmm_swiglu):
             with pytest.raises(NotImplementedError):
                 product(*operands, n)
+
+
+def _written():
+    """The calls that write into a tensor of the caller's, by the tensor."""
+    a, b = _on_device(8, 32), _on_device(3, 32, 64)
+    q, bq = _on_device(8, 32, dtype=torch.float8_e4m3fn), _on_device(3, 64, 32, dtype=torch.float8_e4m3fn)
+    sa, sb = _on_device(8, dtype=torch.float32), _on_device(3, 64, dtype=torch.float32)
+    rows, ptrs, n = _on_device(8, dtype=torch.int32), _on_device(8, dtype=torch.int64), torch.tensor(SIZES)
+    w = gg.pack_w4(torch.zeros(3, 64, 32, dtype=torch.uint8), torch.ones(3, 64, 1), None, 32)
+    return {
+        "gmm": (64, lambda c: gg.gmm(a, b, n, c=c)),
+        "gmm_swiglu": (32, lambda c: gg.gmm_swiglu(a, b, n, c=c)),
+        "gmm_swiglu_rows": (32, lambda c: gg.gmm_swiglu_rows(a, rows, b, n, c=c)),
+        "gmm_fp8": (64, lambda c: gg.gmm_fp8(q, sa, bq, sb, n, c=c)),
+        "gmm_fp8_swiglu": (32, lambda c: gg.gmm_fp8_swiglu(q, sa, bq, sb, n, c=c)),
+        "gmm_w4": (64, lambda c: gg.gmm_w4(a, w, n, c=c)),
+        "gmm_w4_swiglu": (32, lambda c: gg.gmm_w4_swiglu(a, w, n, c=c)),
+        "zero_rows_behind": (64, lambda c: gg.zero_rows_behind(c, n)),
+        "gather_row_ptrs": (64, lambda c: memory.gather_row_ptrs(ptrs, 64, torch.bfloat16, out=c)),
+    }
+
+
+@pytest.mark.parametrize("name", list(_written()))
+def test_a_result_in_the_callers_tensor_modifies_it(monkeypatch, name):
+    """What autograd has saved of that tensor is not used as if it still held the old values."""
+    _fake_device(monkeypatch, lambda name, args: None)
+    monkeypatch.setattr(gg, "_check_w4", lambda w: w.codes.shape[0])
+    monkeypatch.setattr(memory, "_stream", lambda device: 0)
+    columns, call = _written()[name]
+    c = _on_device(8, columns)
+    x = torch.ones(8, columns, dtype=torch.bfloat16, requires_grad=True)
+    y = x * c                                          # saves c
+    assert call(c) is c
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with torch.inference_mode():                       # a tensor without a version, and one with
+        call(_on_device(8, columns))
+        call(c)
