@@ -68,6 +68,7 @@ SIGNATURES = {
     "dmoe_w4_quant": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
     "dmoe_w4_dequant": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p]),
     "dmoe_gmm_w4_wide_bytes": (c_int, [c_int64, c_int, c_int64, c_int64, c_int, c_void_p, POINTER(c_size_t)]),
+    "dmoe_gmm_w4_wide_bytes_of": (c_int, [c_int64, c_int, c_int64, c_int64, POINTER(c_size_t)]),
     "dmoe_gmm_w4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int, c_int64, c_int64,
                             c_void_p, c_size_t, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
     "dmoe_gmm_w4_swiglu": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int, c_int64,

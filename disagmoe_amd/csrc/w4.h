@@ -46,6 +46,7 @@ struct W4Args {
     int n_out;                                // columns of c
     int nt, kt;                               // tiles of an expert along its columns and along k
     int m_tiles;                              // row tiles of the grid
+    const int64_t *first;                     // the experts before *first are left out (nullptr: none)
 };
 
 // 16 + q of nibbles p and p + 4 as two bf16.  The mask sits in a scalar and the 16s in a vector register: an instruction
@@ -64,13 +65,14 @@ __device__ __forceinline__ W4Constants w4_constants() {
     return k;
 }
 
-// Row tile number `m` of all experts' row tiles of BM rows: its expert, first row and rows, and how many row tiles there are
-// (without one of that number the other results are left as they are).
+// Row tile number `m` of all experts' row tiles of BM rows (of the experts that are not left out): its expert, first row and
+// rows, and how many row tiles there are (without one of that number the other results are left as they are).
 template <int BM>
 __device__ __forceinline__ int w4_locate(const W4Args &p, int m, int &expert, int &row0, int &rows) {
     const int lane = lane_id();
     long long row_carry = 0;
     int tile_carry = 0;
+    const int first = p.first != nullptr ? (int)*p.first : 0;
     for (int e0 = 0; e0 < p.E; e0 += kWave) {
         const int e = e0 + lane;
         long long n = e < p.E ? (long long)p.batch_sizes[e] : 0;
@@ -84,7 +86,7 @@ __device__ __forceinline__ int w4_locate(const W4Args &p, int m, int &expert, in
         long long start = row_carry + incl - n, end = row_carry + incl;
         start = start > p.rows ? p.rows : start;
         end = end > p.rows ? p.rows : end;
-        const int mt = (int)((end - start + BM - 1) / BM);
+        const int mt = e < first ? 0 : (int)((end - start + BM - 1) / BM);
         int tincl = mt;
 #pragma unroll
         for (int s = 1; s < kWave; s <<= 1) {

@@ -84,15 +84,36 @@ __global__ __launch_bounds__(kWave) void w4_quant_kernel(const uint16_t *__restr
 //               are rounded to 11 bits where the 8 of bf16 would show in the product (relative error of the gated form
 //               2.5e-3 instead of 1.7e-3, the rounding of its results alone), and f keeps them in fp16's range.
 // Rows of `out` are Kp >= K long; what lies behind K is some finite value (it meets zeros there, see w4_half_rows_kernel).
+// With slot_sizes, gridDim.y is the number of experts that `out` has room for: its part s takes expert number s of those that have
+// rows, and slot_sizes[s] that expert's rows (0 without one), so that a product on the parts finds its rows where they are;
+// slot_sizes[gridDim.y] is the first expert that got no part.
 template <bool HALF>
 __global__ __launch_bounds__(256) void w4_widen_kernel(const char *__restrict__ codes, const uint16_t *__restrict__ scales, const uint8_t *__restrict__ zeros,
                                                       uint16_t *__restrict__ out, float *__restrict__ col_scale, const int64_t *__restrict__ batch_sizes,
-                                                      int K, int Kp, int N, int nt, int kt, int group) {
+                                                      int K, int Kp, int N, int nt, int kt, int group, int E, int64_t *__restrict__ slot_sizes) {
     __shared__ __attribute__((aligned(16))) char stage[4][4096];
     __shared__ uint16_t largest[kW4Cols][16];
     const int lane = lane_id(), r = lane & 15, g16 = lane >> 4, wave = threadIdx.x / kWave;
-    const int e = blockIdx.y, t = blockIdx.x;
-    if (batch_sizes != nullptr && batch_sizes[e] <= 0) return;
+    const int slot = blockIdx.y, t = blockIdx.x;
+    int e = slot;
+    if (slot_sizes != nullptr) {
+        e = -1;
+        int before = 0;
+        for (int e0 = 0; e0 < E && e < 0; e0 += kWave) {
+            const bool busy = e0 + lane < E && batch_sizes[e0 + lane] > 0;
+            const unsigned long long all = __ballot(busy);
+            const unsigned long long at = __ballot(busy && before + __popcll(all & ((1ull << lane) - 1)) == slot);
+            if (at != 0) e = e0 + __ffsll(at) - 1;
+            before += __popcll(all);
+        }
+        if (t == 0 && threadIdx.x == 0) {
+            slot_sizes[slot] = e < 0 ? 0 : batch_sizes[e];
+            if (slot + 1 == (int)gridDim.y) slot_sizes[slot + 1] = e < 0 ? E : e + 1;
+        }
+        if (e < 0) return;
+    } else if (batch_sizes != nullptr && batch_sizes[e] <= 0) {
+        return;
+    }
     const int ng = kW4Chunk / group;
     const int64_t first = ((int64_t)e * nt + t) * kt;          // tile (t, 0) of the expert
     float inv = 1.f;
@@ -112,7 +133,7 @@ __global__ __launch_bounds__(256) void w4_widen_kernel(const char *__restrict__ 
         int exponent = (int)(top >> 7);
         exponent = exponent < 1 ? 127 : (exponent > 253 ? 253 : exponent);   // all zero: 1; infinite: whatever, it stays so
         inv = __uint_as_float((uint32_t)(254 - exponent) << 23);
-        if (wave == 0 && g16 == 0 && t * kW4Cols + r < N) col_scale[(int64_t)e * N + t * kW4Cols + r] = __uint_as_float((uint32_t)exponent << 23);
+        if (wave == 0 && g16 == 0 && t * kW4Cols + r < N) col_scale[(int64_t)slot * N + t * kW4Cols + r] = __uint_as_float((uint32_t)exponent << 23);
     }
     char *mine = stage[wave];
     for (int c = wave; c < kt; c += 4) {
@@ -140,7 +161,7 @@ __global__ __launch_bounds__(256) void w4_widen_kernel(const char *__restrict__ 
         for (int i = 0; i < 4; ++i) {
             const int row = i * 4 + g16, n = t * kW4Cols + row, k = c * kW4Chunk + r * 8;
             const u32x4 v = *(const u32x4 *)(mine + row * 256 + ((r ^ row) << 4));
-            if (n < N && k < Kp) __builtin_nontemporal_store(v, (u32x4 *)(out + ((int64_t)e * N + n) * Kp + k));
+            if (n < N && k < Kp) __builtin_nontemporal_store(v, (u32x4 *)(out + ((int64_t)slot * N + n) * Kp + k));
         }
     }
 }
@@ -204,6 +225,7 @@ static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 // Where the form for many rows keeps what it writes: fp16 weights and rows, and their scales.
 struct WideLayout {
     size_t weights, col_scales, rows, row_scales, bytes;
+    size_t slot_sizes;                                        // behind the others, where not every expert has room
 };
 static int64_t wide_k(int64_t K) { return (K + 31) / 32 * 32; }   // whole stages of the 256-row tile
 static WideLayout wide_layout(int64_t rows, int E, int64_t K_given, int64_t N) {
@@ -213,14 +235,26 @@ static WideLayout wide_layout(int64_t rows, int E, int64_t K_given, int64_t N) {
     w.col_scales = up256((size_t)E * N * K * 2);
     w.rows = w.col_scales + up256((size_t)E * N * 4);
     w.row_scales = w.rows + up256((size_t)rows * K * 2);
-    w.bytes = w.row_scales + up256((size_t)rows * 4);
+    w.bytes = w.slot_sizes = w.row_scales + up256((size_t)rows * 4);
     return w;
+}
+static size_t wide_part_bytes(int64_t rows, int experts, int64_t K, int64_t N) {
+    return wide_layout(rows, experts, K, N).bytes + up256(((size_t)experts + 1) * sizeof(int64_t));
+}
+// Experts that `bytes` have room for: E of them, or some (the experts that have rows take the room in turn).
+static int wide_experts(int64_t rows, int E, int64_t K, int64_t N, size_t bytes) {
+    if (bytes >= wide_layout(rows, E, K, N).bytes) return E;
+    int least = 0, most = E;                                  // room for `least`, none for `most`
+    while (most - least > 1) {
+        const int mid = (least + most) / 2;
+        if (bytes >= wide_part_bytes(rows, mid, K, N)) least = mid; else most = mid;
+    }
+    return least;
 }
 
 struct W4Form {
     bool wide;        // through fp16 weights
     int tile_rows;
-    int m_tiles;
 };
 // Rows per expert decide.  The one kernel unpacks the codes again for every 64 rows and folds every group; from some number of
 // rows on the product on weights that are written out first is the faster one, the sooner the shorter the groups.  Measured,
@@ -228,6 +262,23 @@ struct W4Form {
 // 1024 2280 / 1973; groups of 32: 256 rows 774 / 1219, 512 1524 / 1262; K 2048, N 2816, 64 experts, groups of 128: 256 rows
 // 381 / 548, 512 748 / 602; groups of 32: 256 rows 480 / 553, 512 951 / 611.
 static long long wide_rows(int group) { return group == 128 ? 512 : (group == 64 ? 448 : 384); }
+// Row tiles of the one kernel for the experts that have rows but the first `left_out` of them: those of the sizes, or at most one
+// short one for every expert with rows.
+static int row_tiles_w4(int64_t rows, int E, int tile_rows, int left_out, const int64_t *host_sizes) {
+    long long m = rows / tile_rows + (E < rows ? E : rows);
+    if (host_sizes != nullptr) {
+        long long left = rows;
+        m = 0;
+        for (int e = 0; e < E; ++e) {
+            long long n = host_sizes[e] < 0 ? 0 : host_sizes[e];
+            if (n > 0 && left_out-- > 0) { left -= n < left ? n : left; continue; }
+            if (n > left) n = left;
+            left -= n;
+            m += (n + tile_rows - 1) / tile_rows;
+        }
+    }
+    return (int)(m > 0 ? m : 1);
+}
 static W4Form choose_w4(int64_t rows, int E, int64_t K, int64_t N, int group, const int64_t *host_sizes) {
     long long busy = E < rows ? E : rows;
     if (host_sizes != nullptr) {
@@ -239,19 +290,6 @@ static W4Form choose_w4(int64_t rows, int E, int64_t K, int64_t N, int group, co
     W4Form f;
     f.wide = avg > wide_rows(group) && wide_k(K) * N * 2 < (1ll << 32);   // (what the 256-row tile takes)
     f.tile_rows = avg <= 16 ? 16 : (avg <= 32 ? 32 : 64);
-    // row tiles: those of the sizes, or at most one short one for every expert with rows
-    long long m = rows / f.tile_rows + (E < rows ? E : rows);
-    if (host_sizes != nullptr) {
-        long long left = rows;
-        m = 0;
-        for (int e = 0; e < E; ++e) {
-            long long n = host_sizes[e] < 0 ? 0 : host_sizes[e];
-            if (n > left) n = left;
-            left -= n;
-            m += (n + f.tile_rows - 1) / f.tile_rows;
-        }
-    }
-    f.m_tiles = (int)(m > 0 ? m : 1);
     return f;
 }
 
@@ -269,27 +307,41 @@ static int gmm_w4(const char *who, const void *a, const void *codes, const void 
                  DMOE_ERR_ARG, "%s: a pointer is not 16-byte aligned", who);
     if (rows == 0) return DMOE_OK;
     const W4Form f = choose_w4(rows, E, K, N, group, host_batch_sizes);
-    const WideLayout at = wide_layout(rows, E, K, N);
-    if (f.wide && wide != nullptr && wide_bytes >= at.bytes) {
+    const int nt = tiles_of(N, kW4Cols), kt = tiles_of(K, kW4Chunk);
+    const int64_t *left = nullptr;                            // the first expert that had no room
+    const int experts = f.wide && wide != nullptr ? wide_experts(rows, E, K, N, wide_bytes) : 0;   // that `wide` has room for
+    if (experts > 0) {
+        const WideLayout at = wide_layout(rows, experts, K, N);
         char *w = (char *)wide;
+        int64_t *slot_sizes = experts < E ? (int64_t *)(w + at.slot_sizes) : nullptr;
         const int64_t Kp = wide_k(K);
-        const int nt = tiles_of(N, kW4Cols), kt = tiles_of(K, kW4Chunk);
-        hipLaunchKernelGGL(w4_widen_kernel<true>, dim3(nt, E), dim3(256), 0, (hipStream_t)stream, (const char *)codes, (const uint16_t *)scales,
+        hipLaunchKernelGGL(w4_widen_kernel<true>, dim3(nt, experts), dim3(256), 0, (hipStream_t)stream, (const char *)codes, (const uint16_t *)scales,
                            (const uint8_t *)zeros, (uint16_t *)(w + at.weights), (float *)(w + at.col_scales), batch_sizes, (int)K, (int)Kp, (int)N, nt, kt,
-                           group);
+                           group, E, slot_sizes);
         DMOE_LAUNCH_CHECK("w4_widen_kernel");
         hipLaunchKernelGGL(w4_half_rows_kernel, dim3((unsigned)rows), dim3(256), 0, (hipStream_t)stream, (const u32x4 *)a, (u32x4 *)(w + at.rows),
                            (float *)(w + at.row_scales), (int)(K / 8), (int)(Kp / 8));
         DMOE_LAUNCH_CHECK("w4_half_rows_kernel");
-        const HostSizes known(host_batch_sizes);
-        GmmArgs args{w + at.rows, w + at.weights, (char *)c, batch_sizes, (const float *)(w + at.row_scales), (const float *)(w + at.col_scales), rows, E,
-                     (int)Kp, (int)N, (int)n_out};
+        // the sizes of the experts that have room, on the host too
+        int64_t host_slots[kMaxGroups];
+        if (host_batch_sizes != nullptr && slot_sizes != nullptr) {
+            int s = 0;
+            for (int e = 0; e < E && s < experts; ++e)
+                if (host_batch_sizes[e] > 0) host_slots[s++] = host_batch_sizes[e];
+            while (s < experts) host_slots[s++] = 0;
+        }
+        const HostSizes known(host_batch_sizes != nullptr && slot_sizes != nullptr ? host_slots : host_batch_sizes);
+        GmmArgs args{w + at.rows, w + at.weights, (char *)c, slot_sizes != nullptr ? slot_sizes : batch_sizes, (const float *)(w + at.row_scales),
+                     (const float *)(w + at.col_scales), rows, experts, (int)Kp, (int)N, (int)n_out};
         rc = bind_state(args, state, workspace, workspace_bytes, (hipStream_t)stream);
         const WorkspaceTurn turn(args);
-        return rc != DMOE_OK ? rc : launch_tile256_half(args, swiglu, (hipStream_t)stream);
+        if (rc == DMOE_OK) rc = launch_tile256_half(args, swiglu, (hipStream_t)stream);
+        if (rc != DMOE_OK || experts >= (E < rows ? E : rows)) return rc;
+        left = slot_sizes + experts;
+        // (where the host's sizes have nobody left, the launch finds out by itself in a few microseconds)
     }
     W4Args args{(const char *)a, (const char *)codes, (const char *)scales, (const char *)zeros, (char *)c, batch_sizes, rows, E, (int)K, (int)N,
-                (int)n_out, tiles_of(N, kW4Cols), tiles_of(K, kW4Chunk), f.m_tiles};
+                (int)n_out, nt, kt, row_tiles_w4(rows, E, f.tile_rows, experts, host_batch_sizes), left};
     if (f.tile_rows == 16) return launch_w4_16(args, group, swiglu, (hipStream_t)stream);
     if (f.tile_rows == 32) return launch_w4_32(args, group, swiglu, (hipStream_t)stream);
     return launch_w4_64(args, group, swiglu, (hipStream_t)stream);
@@ -332,7 +384,7 @@ extern "C" int dmoe_w4_dequant(const void *codes, const void *scales, const void
     DMOE_REQUIRE(aligned(codes, 16) && aligned(scales, 16) && aligned(out, 16), DMOE_ERR_ARG, "dmoe_w4_dequant: a pointer is not 16-byte aligned");
     const int nt = tiles_of(N, kW4Cols), kt = tiles_of(K, kW4Chunk);
     hipLaunchKernelGGL(w4_widen_kernel<false>, dim3(nt, E), dim3(256), 0, (hipStream_t)stream, (const char *)codes, (const uint16_t *)scales,
-                       (const uint8_t *)zeros, (uint16_t *)out, (float *)nullptr, batch_sizes, (int)K, (int)K, (int)N, nt, kt, group);
+                       (const uint8_t *)zeros, (uint16_t *)out, (float *)nullptr, batch_sizes, (int)K, (int)K, (int)N, nt, kt, group, E, (int64_t *)nullptr);
     DMOE_LAUNCH_CHECK("w4_widen_kernel");
     return DMOE_OK;
 }
@@ -342,6 +394,14 @@ extern "C" int dmoe_gmm_w4_wide_bytes(int64_t rows, int E, int64_t K, int64_t N,
     if (rc != DMOE_OK) return rc;
     DMOE_REQUIRE(bytes != nullptr && rows >= 0 && rows < (1ll << 31), DMOE_ERR_ARG, "dmoe_gmm_w4_wide_bytes: bad rows or null output");
     *bytes = choose_w4(rows, E, K, N, group, host_batch_sizes).wide ? wide_layout(rows, E, K, N).bytes : 0;
+    return DMOE_OK;
+}
+
+extern "C" int dmoe_gmm_w4_wide_bytes_of(int64_t rows, int experts, int64_t K, int64_t N, size_t *bytes) {
+    const int rc = check_w4("dmoe_gmm_w4_wide_bytes_of", experts, K, N, 128);
+    if (rc != DMOE_OK) return rc;
+    DMOE_REQUIRE(bytes != nullptr && rows >= 0 && rows < (1ll << 31), DMOE_ERR_ARG, "dmoe_gmm_w4_wide_bytes_of: bad rows or null output");
+    *bytes = wide_part_bytes(rows, experts, K, N);
     return DMOE_OK;
 }
 

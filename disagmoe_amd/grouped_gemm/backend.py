@@ -591,6 +591,14 @@ def dequantize_w4(w: W4Weight) -> torch.Tensor:
     return out
 
 
+def _wide_scratch(nbytes: int, device: torch.device) -> Optional[torch.Tensor]:
+    """Room for the 16-bit weights and rows of one call, ``None`` if the device has none left."""
+    try:
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    except torch.OutOfMemoryError:
+        return None
+
+
 def _gmm_w4(name: str, a: torch.Tensor, w: W4Weight, n_out: int, batch_sizes: torch.Tensor, c: Optional[torch.Tensor],
             workspace: Optional[torch.Tensor], arguments_ptr: Optional[int], host_batch_sizes: Optional[torch.Tensor]) -> torch.Tensor:
     E, device = _check_w4(w), w.codes.device
@@ -610,11 +618,14 @@ def _gmm_w4(name: str, a: torch.Tensor, w: W4Weight, n_out: int, batch_sizes: to
     with torch.cuda.device(device):
         stream = _stream(device)
         _lib.call("dmoe_gmm_w4_wide_bytes", rows, E, w.K, w.N, w.group, host_ptr, _lib.ctypes.byref(need))
+        wide, more = None, (None, 0, None, None, 0)
         if need.value:   # 16-bit weights and rows of this call, and the state of the product on them
-            wide = torch.empty(need.value, dtype=torch.uint8, device=device)
+            busy = E if host is None else max(1, int((host > 0).sum()))
+            if busy < min(E, rows):
+                _lib.call("dmoe_gmm_w4_wide_bytes_of", rows, busy, w.K, w.N, _lib.ctypes.byref(need))
+            wide = _wide_scratch(need.value, device)
+        if wide is not None:
             more = (wide.data_ptr(), need.value, *_state_triple(device, workspace, arguments_ptr, stream))
-        else:
-            more = (None, 0, None, None, 0)
         _lib.call(name, a.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), _zeros_ptr(w), w.group, c.data_ptr(), bs.data_ptr(),
                   rows, E, w.K, n_out, *more, host_ptr, stream)
     return _modified(c) if given else c
@@ -624,8 +635,10 @@ def gmm_w4(a: torch.Tensor, w: W4Weight, batch_sizes: torch.Tensor, c: Optional[
            workspace: Optional[torch.Tensor] = None, arguments_ptr: Optional[int] = None,
            host_batch_sizes: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``c[o_e:o_e+n_e] = a[o_e:o_e+n_e] @ w[e].T`` on 4-bit weights, bf16 ``[rows, N]``.  From one row to
-    a prompt; many rows per expert go through 16-bit weights that the call allocates and writes
-    (``E * N * K * 2`` bytes and a little, for its own length).  The other arguments as :func:`gmm`'s."""
+    a prompt; many rows per expert go through 16-bit weights that the call allocates and writes, for its
+    own length: ``N * K * 2`` bytes and a little for every expert, or with the sizes on the host for every
+    expert that has rows.  Where the device has no room for them, a slower form runs that needs none (and
+    rounds the weights to nothing).  The other arguments as :func:`gmm`'s."""
     return _gmm_w4("dmoe_gmm_w4", a, w, w.N, batch_sizes, c, workspace, arguments_ptr, host_batch_sizes)
 
 

@@ -359,7 +359,9 @@ int dmoe_gmm_fp8_swiglu(const void *a, const float *a_scale, const void *b, cons
  * h [rows, I], as dmoe_gmm_swiglu.  Few rows per expert: one kernel that reads the codes, 32-bit sums of unrounded weights.
  * Many: where `wide` (any contents) has dmoe_gmm_w4_wide_bytes(..) bytes (0: not needed), the weights of
  * the experts that have rows, rounded to the 11 bits of fp16, and the rows are written there with scales that are powers
- * of two and go through the bf16 product's 256-row tile; without it the one kernel serves any number of rows.
+ * of two and go through the bf16 product's 256-row tile; without it the one kernel serves any number of rows.  A `wide` of
+ * dmoe_gmm_w4_wide_bytes_of(.., experts, ..) bytes has room for that many of the experts that have rows: the first ones go
+ * through it, the others through the one kernel.
  * A row of a with an infinity or NaN has no finite result (NaN where few rows run: the offset of the codes is taken off as
  * a sum of its own, inf - inf; so are sums past the range of fp32, which magnitudes of a below 2^116 cannot reach); the other
  * rows do not see it.  state, workspace and host_batch_sizes as for dmoe_gmm (the first two serve the form of many
@@ -371,6 +373,7 @@ int dmoe_w4_dequant(const void *codes, const void *scales, const void *zeros, in
                     const int64_t *batch_sizes, int E, int64_t K, int64_t N, void *stream);
 int dmoe_gmm_w4_wide_bytes(int64_t rows, int E, int64_t K, int64_t N, int group, const int64_t *host_batch_sizes,
                            size_t *bytes);
+int dmoe_gmm_w4_wide_bytes_of(int64_t rows, int experts, int64_t K, int64_t N, size_t *bytes);
 int dmoe_gmm_w4(const void *a, const void *codes, const void *scales, const void *zeros, int group, void *c,
                 const int64_t *batch_sizes, int64_t rows, int E, int64_t K, int64_t N, void *wide, size_t wide_bytes,
                 void *state, void *workspace, size_t workspace_bytes, const int64_t *host_batch_sizes, void *stream);

@@ -90,3 +90,16 @@ def test_python_refusals():
     w = gg.pack_w4(torch.zeros(1, 8, 8, dtype=torch.uint8), torch.zeros(1, 8, 1), None, 32)
     with pytest.raises(RuntimeError):
         gg.gmm_w4(torch.zeros(1, 8, dtype=torch.bfloat16), w, torch.tensor([1]))
+
+
+def test_room_for_some_experts():
+    lib, need, all_of_them = _lib.load(), ctypes.c_size_t(), ctypes.c_size_t()
+    up = lambda n: -(-n // 256) * 256                             # weights, their scales, rows, their scales, sizes
+    for experts in (1, 3, 8):
+        assert lib.dmoe_gmm_w4_wide_bytes_of(5000, experts, 40, 24, ctypes.byref(need)) == 0
+        assert need.value == up(experts * 24 * 64 * 2) + up(experts * 24 * 4) + up(5000 * 64 * 2) + up(5000 * 4) + up(experts * 8 + 8)
+    assert lib.dmoe_gmm_w4_wide_bytes(5000, 8, 40, 24, 128, None, ctypes.byref(all_of_them)) == 0 and all_of_them.value <= need.value
+    assert lib.dmoe_gmm_w4_wide_bytes_of(5000, 0, 40, 24, ctypes.byref(need)) == _lib.ERR_SHAPE
+    assert lib.dmoe_gmm_w4_wide_bytes_of(5000, 2, 44, 24, ctypes.byref(need)) == _lib.ERR_SHAPE
+    assert lib.dmoe_gmm_w4_wide_bytes_of(-1, 2, 40, 24, ctypes.byref(need)) == _lib.ERR_ARG
+    assert lib.dmoe_gmm_w4_wide_bytes_of(1, 2, 40, 24, None) == _lib.ERR_ARG
