@@ -131,7 +131,8 @@ __global__ __launch_bounds__(256) void w4_widen_kernel(const char *__restrict__ 
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = largest[r][i] > top ? largest[r][i] : top;
         int exponent = (int)(top >> 7);
-        exponent = exponent < 1 ? 127 : (exponent > 253 ? 253 : exponent);   // all zero: 1; infinite: whatever, it stays so
+        // (scales below the normal numbers: 2^-126; all zero: 1; infinite: whatever, it stays so)
+        exponent = top == 0 ? 127 : (exponent < 1 ? 1 : (exponent > 253 ? 253 : exponent));
         inv = __uint_as_float((uint32_t)(254 - exponent) << 23);
         if (wave == 0 && g16 == 0 && t * kW4Cols + r < N) col_scale[(int64_t)slot * N + t * kW4Cols + r] = __uint_as_float((uint32_t)exponent << 23);
     }
@@ -193,7 +194,8 @@ __global__ __launch_bounds__(256) void w4_half_rows_kernel(const u32x4 *__restri
 #pragma unroll
     for (int i = 0; i < 4; ++i) most = part[i] > most ? part[i] : most;
     int exponent = (int)(most >> 7);
-    exponent = exponent < 1 ? 127 : (exponent > 253 ? 253 : exponent);       // a row of zeros: 1; not finite: it stays so
+    // (values below the normal numbers: 2^-126; a row of zeros: 1; not finite: it stays so)
+    exponent = most == 0 ? 127 : (exponent < 1 ? 1 : (exponent > 253 ? 253 : exponent));
     const float inv = __uint_as_float((uint32_t)(254 - exponent) << 23);
     if (threadIdx.x == 0) row_scale[row] = __uint_as_float((uint32_t)exponent << 23);
     for (int i = threadIdx.x; i < out_vecs; i += 256) {

@@ -89,3 +89,21 @@ def _off(a, w, s):
     many = (2.0 ** -11 + ACC * (a.shape[1] + 4)) * mag
     many = many + 2.0 ** -24 * (a.abs().sum(1, keepdim=True) * 16 * s.max(1).values + a.abs().max(1, keepdim=True).values * w.abs().sum(1))
     return torch.maximum(one, many)
+
+
+@pytest.mark.parametrize("rows", [3, 30, 60, 700])
+def test_rows_and_scales_below_the_normal_numbers(rows):
+    """bf16 has numbers down to 2^-133: rows that hold no larger one, and columns whose scales are no larger, count."""
+    announce(test="w4_subnormal", rows=rows)
+    K, N, group = 256, 48, 128
+    g = torch.Generator(device=dev()).manual_seed(rows)
+    x = (torch.randint(-100, 101, (rows, K), generator=g, device=dev()).double() * 2.0 ** -133).to(torch.bfloat16)
+    q = torch.randint(0, 16, (1, N, K), generator=g, device=dev(), dtype=torch.uint8)
+    spread = lambda v: v.double().repeat_interleave(group, 2)[:, :, :K]
+    s = (torch.rand(1, N, K // group, generator=g, device=dev()).double() * 2.0 ** 120).to(torch.bfloat16)
+    out = gg.gmm_w4(x, gg.pack_w4(q, s, None, group), torch.tensor([rows]))
+    _check(out, x, (q.double() - 8) * spread(s), spread(s), torch.tensor([rows]), group, False, rows > 512)
+    x = (torch.randn(rows, K, generator=g, device=dev()).double() * 2.0 ** 110).to(torch.bfloat16)
+    s = (torch.randint(1, 128, s.shape, generator=g, device=dev()).double() * 2.0 ** -133).to(torch.bfloat16)
+    out = gg.gmm_w4(x, gg.pack_w4(q, s, None, group), torch.tensor([rows]))
+    _check(out, x, (q.double() - 8) * spread(s), spread(s), torch.tensor([rows]), group, False, rows > 512)
