@@ -6,7 +6,8 @@ namespace dmoe {
 // One wavefront packs one tile: lane 16 g + r holds the 32 weights of column r at k = 32 j + 8 g + i, which a group's
 // lanes (4 per column) share the extremes of.  Without zero points s = max |w| / 7 and q = round(w / s) + 8; with them
 // s = (max(w, 0) - min(w, 0)) / 15 and z = round(-min(w, 0) / s), so that a weight of zero stays one.  s is rounded to
-// bf16 first and the codes follow the rounded one; one below the normal numbers is 0.  Bound by its scattered 2-byte reads
+// bf16 first and the codes follow the rounded one; one below the normal numbers is 0.  A group with a weight that is not finite
+// has NaN for its scale: codes have no place for such a weight.  Bound by its scattered 2-byte reads
 // (8 x 4096 x 28672: 1.1 ms, 2.2 TB/s); weights are packed once.
 __global__ __launch_bounds__(kWave) void w4_quant_kernel(const uint16_t *__restrict__ w, char *__restrict__ codes, uint16_t *__restrict__ scales,
                                                         uint8_t *__restrict__ zeros, int K, int N, int nt, int kt, int group) {
@@ -17,20 +18,24 @@ __global__ __launch_bounds__(kWave) void w4_quant_kernel(const uint16_t *__restr
     const int n = (int)(et % nt) * kW4Cols + r;
     const uint16_t *we = w + (et / nt) * K * N;
     float v[4][8], lo[4], hi[4];
+    int odd[4];                                                // a weight of these is not finite
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         lo[j] = hi[j] = 0.f;
+        odd[j] = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int k = c * kW4Chunk + j * 32 + g16 * 8 + i;
             v[j][i] = n < N && k < K ? bf16_to_f32(we[(int64_t)k * N + n]) : 0.f;
             lo[j] = fminf(lo[j], v[j][i]);
             hi[j] = fmaxf(hi[j], v[j][i]);
+            odd[j] |= !isfinite(v[j][i]);
         }
 #pragma unroll
         for (int s = 16; s < kWave; s <<= 1) {                 // the 4 lanes of a column
             lo[j] = fminf(lo[j], __shfl_xor(lo[j], s, kWave));
             hi[j] = fmaxf(hi[j], __shfl_xor(hi[j], s, kWave));
+            odd[j] |= __shfl_xor(odd[j], s, kWave);
         }
     }
     const int steps = group / 32;                              // k-steps that share a scale
@@ -39,17 +44,20 @@ __global__ __launch_bounds__(kWave) void w4_quant_kernel(const uint16_t *__restr
         for (int s = 1; s < 4; s <<= 1) {
             if (s >= steps) continue;
             float l2[4], h2[4];
+            int o2[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { l2[j] = fminf(lo[j], lo[j ^ s]); h2[j] = fmaxf(hi[j], hi[j ^ s]); }
+            for (int j = 0; j < 4; ++j) { l2[j] = fminf(lo[j], lo[j ^ s]); h2[j] = fmaxf(hi[j], hi[j ^ s]); o2[j] = odd[j] | odd[j ^ s]; }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { lo[j] = l2[j]; hi[j] = h2[j]; }
+            for (int j = 0; j < 4; ++j) { lo[j] = l2[j]; hi[j] = h2[j]; odd[j] = o2[j]; }
         }
     }
     uint32_t words[4];
     const int ng = kW4Chunk / group;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        float s = zeros != nullptr ? (hi[j] - lo[j]) / 15.f : fmaxf(hi[j], -lo[j]) / 7.f;
+        // (a range past fp32 is divided before it is taken)
+        const float range = hi[j] - lo[j];
+        float s = zeros != nullptr ? (isfinite(range) ? range / 15.f : hi[j] / 15.f - lo[j] / 15.f) : fmaxf(hi[j], -lo[j]) / 7.f;
         if (s < 0x1p-126f) s = 0.f;                            // (its inverse would not be finite)
         const uint16_t bits = f32_to_bf16(s);
         s = bf16_to_f32(bits);
@@ -64,7 +72,7 @@ __global__ __launch_bounds__(kWave) void w4_quant_kernel(const uint16_t *__restr
         if (j % steps == 0 && g16 == 0) {
             const int64_t at = tile * (kW4Cols * ng) + (r >> 2) * (ng * 4) + (j / steps) * 4 + (r & 3);
             const bool there = n < N && c * kW4Chunk + j * 32 < K;
-            scales[at] = there ? bits : 0;
+            scales[at] = there ? (odd[j] ? 0x7fc0 : bits) : 0;
             if (zeros != nullptr) zeros[at] = there ? (uint8_t)z : 0;
         }
     }

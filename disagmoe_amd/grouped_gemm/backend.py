@@ -548,7 +548,8 @@ def _zeros_ptr(w: W4Weight):
 def quantize_weight_w4(w: torch.Tensor, group: int = 128, zeros: bool = False) -> W4Weight:
     """Offline quantisation of ``w [E, K, N]`` bf16 to 4 bits: symmetric, ``s = absmax / 7`` over every
     ``group`` k of a column, or with ``zeros`` from the smallest to the largest weight of the group
-    (``s = range / 15``; a weight of zero stays zero)."""
+    (``s = range / 15``; a weight of zero stays zero).  A group with a weight that is not finite comes
+    out as NaN."""
     if not w.is_cuda:
         raise RuntimeError("quantize_weight_w4 needs a device tensor; disagmoe_amd has no CPU fallback")
     assert w.dim() == 3 and w.dtype == torch.bfloat16 and w.is_contiguous()

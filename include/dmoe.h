@@ -352,8 +352,8 @@ int dmoe_gmm_fp8_swiglu(const void *a, const float *a_scale, const void *b, cons
  *
  * dmoe_w4_bytes: the sizes of the three.  dmoe_w4_quant packs bf16 weights w [E, K, N] (the layout of dmoe_gmm): with
  * `zeros` it spreads the 16 codes from the smallest to the largest weight of a group (zero included), without it
- * symmetrically over +-7 steps.  dmoe_w4_dequant writes [E, N, K] bf16, rounded once; with batch_sizes only the experts
- * that have rows.
+ * symmetrically over +-7 steps; a group with a weight that is not finite gets NaN weights.  dmoe_w4_dequant writes
+ * [E, N, K] bf16, rounded once; with batch_sizes only the experts that have rows.
  *
  * dmoe_gmm_w4 is c = a @ w[e]^T for a bf16 [rows, K], c bf16 [rows, N]; dmoe_gmm_w4_swiglu the gated form on w [E, 2I, K],
  * h [rows, I], as dmoe_gmm_swiglu.  Few rows per expert: one kernel that reads the codes, 32-bit sums of unrounded weights.

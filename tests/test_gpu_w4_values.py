@@ -107,3 +107,31 @@ def test_rows_and_scales_below_the_normal_numbers(rows):
     s = (torch.randint(1, 128, s.shape, generator=g, device=dev()).double() * 2.0 ** -133).to(torch.bfloat16)
     out = gg.gmm_w4(x, gg.pack_w4(q, s, None, group), torch.tensor([rows]))
     _check(out, x, (q.double() - 8) * spread(s), spread(s), torch.tensor([rows]), group, False, rows > 512)
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_quantisation_of_what_is_not_finite(group, zeros):
+    """A group with an infinity or NaN has NaN weights, and no other group has; ones that finite weights of the largest
+    magnitudes fill are finite."""
+    announce(test="w4_not_finite", group=group, zeros=zeros)
+    K, N = 264, 32
+    w = _rand((1, K, N), group)
+    top = 2.0 ** 127      # (not the largest bf16: seven steps, rounded up by 2^-8 of them, would lie past it)
+    w[0, :, 4], w[0, 1, 4], w[0, 2, 4] = 0, top, -top
+    clean = gg.dequantize_w4(gg.quantize_weight_w4(w, group, zeros))
+    assert bool(clean.isfinite().all())
+    # within half a step (a whole one with zero points, off by half a step too) and what the step's rounding moves its ends by
+    step = 2 * top / 15 if zeros else top / 7
+    assert bool(((clean[0, 4, 1:3].double() - torch.tensor([top, -top], device=dev())).abs() <= (1.5 + 15 * HALF) * step).all())
+    bad = [(0, 3, float("nan")), (130, 7, float("inf")), (263, 9, float("-inf")), (40, 31, float("nan"))]
+    for k, n, v in bad:
+        w[0, k, n] = v
+    q = gg.quantize_weight_w4(w, group, zeros)
+    got, want = gg.dequantize_w4(q), clean.clone()
+    for k, n, _ in bad:
+        want[0, n, k // group * group:(k // group + 1) * group] = float("nan")
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0))
+    for rows in (3, 700):
+        out = gg.gmm_w4(_rand((rows, K), rows), q, torch.tensor([rows]))
+        assert torch.equal(out.isnan().all(0), want[0].isnan().any(1)) and torch.equal(out.isnan().any(0), want[0].isnan().any(1))
