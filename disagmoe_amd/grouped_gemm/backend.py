@@ -562,10 +562,15 @@ def quantize_weight_w4(w: torch.Tensor, group: int = 128, zeros: bool = False) -
 
 
 def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor], group: int) -> W4Weight:
-    """Lays out weights that are quantised already: ``codes [E, N, K]`` uint8 in 0..15, ``scales [E, N,
-    ceil(K / group)]``, ``zeros`` likewise in uint8 or ``None``.  Once per weight; any device."""
+    """Lays out weights that are quantised already: ``codes [E, N, K]`` whole numbers in 0..15, ``scales
+    [E, N, ceil(K / group)]`` (rounded to bf16), ``zeros`` like the scales with values like the codes, or
+    ``None``.  Once per weight (it waits for the check of the values); any device."""
     E, N, K = codes.shape
     assert K % 8 == 0 and N % 8 == 0 and scales.shape == (E, N, -(-K // group)), "codes [E, N, K], scales [E, N, ceil(K / group)]"
+    assert zeros is None or zeros.shape == scales.shape, "zeros have the scales' shape"
+    for what, v in (("codes", codes), ("zeros", zeros)):
+        if v is not None and (v.is_floating_point() or v.numel() and (int(v.min()) < 0 or int(v.max()) > 15)):
+            raise ValueError(f"{what} are whole numbers from 0 to 15")
     out = _w4_empty(E, K, N, group, zeros is not None, codes.device)
     (_, nt, kt, _), per = out.codes.shape, 128 // group
     for e in range(E):

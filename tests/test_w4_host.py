@@ -103,3 +103,23 @@ def test_room_for_some_experts():
     assert lib.dmoe_gmm_w4_wide_bytes_of(5000, 2, 44, 24, ctypes.byref(need)) == _lib.ERR_SHAPE
     assert lib.dmoe_gmm_w4_wide_bytes_of(-1, 2, 40, 24, ctypes.byref(need)) == _lib.ERR_ARG
     assert lib.dmoe_gmm_w4_wide_bytes_of(1, 2, 40, 24, None) == _lib.ERR_ARG
+
+
+def test_values_that_four_bits_do_not_hold():
+    """A code above 15 would run into its neighbour."""
+    codes, scales, zeros = torch.full((1, 8, 32), 15, dtype=torch.uint8), torch.ones(1, 8, 1), torch.full((1, 8, 1), 15, dtype=torch.uint8)
+    gg.pack_w4(codes, scales, zeros, 32)
+    for bad in (16, 255):
+        c, z = codes.clone(), zeros.clone()
+        c[0, 3, 5] = z[0, 2, 0] = bad
+        with pytest.raises(ValueError, match="codes"):
+            gg.pack_w4(c, scales, zeros, 32)
+        with pytest.raises(ValueError, match="zeros"):
+            gg.pack_w4(codes, scales, z, 32)
+    with pytest.raises(ValueError, match="codes"):
+        gg.pack_w4(codes.to(torch.int8) - 20, scales, None, 32)
+    with pytest.raises(ValueError, match="codes"):
+        gg.pack_w4(codes.float(), scales, None, 32)
+    assert torch.equal(gg.pack_w4(codes.long(), scales, zeros.int(), 32).codes, gg.pack_w4(codes, scales, zeros, 32).codes)
+    with pytest.raises(AssertionError):                          # one zero point for all groups is not taken for the first one's
+        gg.pack_w4(torch.zeros(1, 8, 64, dtype=torch.uint8), torch.ones(1, 8, 2), torch.zeros(1, 8, 1, dtype=torch.uint8), 32)
