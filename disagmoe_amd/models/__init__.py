@@ -1,3 +1,3 @@
-from .experts import MoEExperts, MoEExpertsFP8, MoEExpertsSerial
+from .experts import MoEExperts, MoEExpertsFP8, MoEExpertsSerial, MoEExpertsW4
 
-__all__ = ["MoEExperts", "MoEExpertsSerial", "MoEExpertsFP8"]
+__all__ = ["MoEExperts", "MoEExpertsSerial", "MoEExpertsFP8", "MoEExpertsW4"]
