@@ -27,7 +27,8 @@ def expert_layer_forward(experts: torch.nn.Module, x: torch.Tensor, topk_ids: to
     kernels run.  ``fetch_rows``: whether the gate-up kernel fetches the tokens' rows by their
     place in the expert-sorted order (no permute launch, no ``[R, d]`` copy of the rows; same
     result bit for bit) instead of reading a permuted copy; ``None`` takes it where the experts
-    say it is the faster form (``MoEExperts.takes_rows``)."""
+    say it is the faster form (``MoEExperts.takes_rows``).  A step of inference: none of its
+    stages has a gradient (``MoEExperts.forward_train`` is the experts' differentiable form)."""
     T, k = topk_ids.shape
     num_experts = experts.num_experts
     if hasattr(experts, "forward_quantized"):

@@ -4,6 +4,7 @@ reference's ``disagmoe/models/experts.py`` (MoEExperts :9-96, MoEExpertsSerial
 """
 from __future__ import annotations
 
+import warnings
 from typing import Optional
 
 import torch
@@ -98,6 +99,11 @@ class MoEExperts(_GemmState, torch.nn.Module):
         # state block of this layer's launches and where their workspace comes from (experts.py:69-77)
         self._init_gemm_state(dev, getattr(self, "_workspace_arg", None), getattr(self, "_own_workspace_arg", False))
 
+    def _warn_without_gradient(self, rows: torch.Tensor) -> None:
+        """Says that a gradient somebody may be waiting for will not come."""
+        if torch.is_grad_enabled() and (rows.requires_grad or self.w13_weight.requires_grad or self.w2_weight.requires_grad):
+            warnings.warn("this form of MoEExperts has no gradient: forward_train has", stacklevel=3)
+
     def forward(self, bs: int, hiddens: torch.Tensor, batch_sizes: torch.Tensor,
                 host_batch_sizes: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``gmm(silu(u[:, :I]) * u[:, I:], w2)`` with ``u = gmm(hiddens, w13)``
@@ -105,7 +111,9 @@ class MoEExperts(_GemmState, torch.nn.Module):
         ``max_batch_size`` rows the static buffers are used (the reference's
         cached branch, :83-90).  ``batch_sizes`` on the host (what the reference passes
         off its CUTLASS path) or ``host_batch_sizes`` beside a device tensor let the
-        library count the launch's tiles instead of estimating them."""
+        library count the launch's tiles instead of estimating them.  The result has no
+        gradient (a warning says so where something requires one): :meth:`forward_train`."""
+        self._warn_without_gradient(hiddens)
         ws = dict(self._gemm_state(), host_batch_sizes=host_batch_sizes)
         if self.enable_cache and bs <= self.gmm_cache_max_batch_size and hiddens.shape[0] <= self.cache_up.shape[0]:
             h = gg.gmm_swiglu(hiddens, self.w13_weight, batch_sizes, c=self.cache_up, **ws)[:hiddens.shape[0]]
@@ -119,6 +127,7 @@ class MoEExperts(_GemmState, torch.nn.Module):
         and ``row_token [R]`` (``ops.memory.route_tokens_with_sources``) instead of the
         expert-sorted copy ``hiddens [R, d]``: the gate-up kernel reads row ``row_token[r]`` of
         ``x``, and the permute in front of the FFN (engine.py:671-680) is never launched."""
+        self._warn_without_gradient(x)
         ws = dict(self._gemm_state(), host_batch_sizes=host_batch_sizes)
         h = gg.gmm_swiglu_rows(x, row_token, self.w13_weight, batch_sizes, **ws)
         return gg.gmm(h, self.w2_weight, batch_sizes, **ws)
