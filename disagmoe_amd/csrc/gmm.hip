@@ -592,16 +592,21 @@ static int launch_by_rows(const GmmArgs &args, hipStream_t stream) {
 //  31 experts, 3440 rows, 648 x 2 x 6616:  269 / 200 / 200   395 / 402 / 374     258 / 294 / 241
 //  64 experts, 8192 rows, 1000 x 2 x 712:  99 / 86 / 86      76 / 109 / 86       82 / 114 / 88
 //   5 experts, 12680 rows, 1112 x 2 x 8008: 834 / 665 / 665  1579 / 1020 / 1020  804 / 710 / 710
-// And 256-row tiles are taken instead of 128-row ones where (nearly) a third of the compute units get one and their contractions are
-// long enough to be cut in two (backward without db on [K, N] and [N, K] weights, 128 / 256-row tiles): 126 tiles of 574 stages:
-// 535 / 408 and 413 / 381; 84 of 574: 436 / 349 and 368 / 296; 96 of 312: 219 / 193 and 207 / 167; but 64 of 187: 119 / 142, 60
-// of 173: 138 / 161.
+// And 256-row tiles are taken instead of 128-row ones where more than a quarter of the compute units get one (twice as many 128-row
+// tiles cannot be cut in two within a round then, and these can) and their contractions make pieces of 120 stages.  Measured, the
+// gradient of the rows alone (1000 rows on each of 2 experts), 128 / 256-row tiles on [K, N] and [N, K] weights, 256 compute units:
+//   64 tiles of 176 stages: 106 / 124, 92 / 116   240: 118 / 135, 109 / 129   312: 138 / 148, 127 / 142   574: 245 / 243, 199 / 212
+//   72                      107 / 111, 90 / 104        141 / 126, 117 / 119        184 / 143, 166 / 135        406 / 276, 340 / 230
+//   80                      105 / 114, 89 / 107        140 / 131, 115 / 124        188 / 149, 170 / 140        376 / 279, 301 / 235
+//   96                      105 / 116, 88 / 103        141 / 135, 117 / 122        177 / 159, 152 / 144        466 / 392, 384 / 344
+//   112                     109 / 116, 95 / 109        147 / 141, 127 / 131        186 / 167, 161 / 157        469 / 362, 351 / 294
+//   120                     115 / 121, 103 / 113       153 / 147, 133 / 135        195 / 224, 169 / 175        469 / 363, 354 / 301
 static int tail_rows(const GmmArgs &args, const GmmLaunch &L, bool trans_b, bool swiglu) {
     if (L.kernel != kKernelStaged || (g_variant >= 1 && g_variant <= 4) || args.K % 32 == 0 || (long long)args.K * args.N * 2 >= (1ll << 32)) return 0;
     if (g_variant != 0 || L.tile_rows == 64) return L.tile_rows;
     if (L.tile_rows == 128) {
         const long long tiles = m_tiles_of(args, 256) * (swiglu ? (args.N / 2 + 127) / 128 : (args.N + 255) / 256);
-        return L.avg_rows > 160 && args.arrive != nullptr && 3 * tiles + 16 >= device_cus() && args.K / 32 >= 2 * kMinPieceStages ? 256 : 128;
+        return L.avg_rows > 160 && args.arrive != nullptr && 4 * tiles > device_cus() && args.K / 32 >= 240 ? 256 : 128;
     }
     return L.avg_rows <= 64 ? 64 : (trans_b && L.avg_rows <= 160 ? 128 : 256);
 }
