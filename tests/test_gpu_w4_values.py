@@ -135,3 +135,19 @@ def test_quantisation_of_what_is_not_finite(group, zeros):
     for rows in (3, 700):
         out = gg.gmm_w4(_rand((rows, K), rows), q, torch.tensor([rows]))
         assert torch.equal(out.isnan().all(0), want[0].isnan().any(1)) and torch.equal(out.isnan().any(0), want[0].isnan().any(1))
+
+
+@pytest.mark.parametrize("swiglu", [False, True])
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True), (128, False)])
+def test_one_round_of_workgroups_and_more(group, zeros, swiglu):
+    """64-row tiles on either side of where one round of workgroups ends: 32 and 36 workgroups of 128 columns to an XCD."""
+    K = 200
+    for E, N in ((8, 4096), (9, 3584)):
+        announce(test="w4_rounds", E=E, N=N, group=group, zeros=zeros, swiglu=swiglu)
+        sizes = torch.tensor([64, 33, 0, 64, 1, 50] + [64] * (E - 6))
+        sizes[2] = 64 * E - int(sizes.sum())
+        w, ref, s = _weight(E, N, K, group, zeros, seed=N)
+        x = _rand((64 * E, K), E)
+        _check((gg.gmm_w4_swiglu if swiglu else gg.gmm_w4)(x, w, sizes), x, ref, s, sizes, group, swiglu, False)
+        even = torch.full((E,), 64)
+        _check((gg.gmm_w4_swiglu if swiglu else gg.gmm_w4)(x, w, even), x, ref, s, even, group, swiglu, False)
