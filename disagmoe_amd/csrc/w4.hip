@@ -270,7 +270,11 @@ struct W4Form {
 // rows on the product on weights that are written out first is the faster one, the sooner the shorter the groups.  Measured,
 // us of the one kernel / through 16-bit weights: K 4096, N 28672, 8 experts, groups of 128: 256 rows 596 / 1203, 512 1144 / 1244,
 // 1024 2280 / 1973; groups of 32: 256 rows 774 / 1219, 512 1524 / 1262; K 2048, N 2816, 64 experts, groups of 128: 256 rows
-// 381 / 548, 512 748 / 602; groups of 32: 256 rows 480 / 553, 512 951 / 611.
+// 381 / 548, 512 748 / 602; groups of 32: 256 rows 480 / 553, 512 951 / 611.  These are many columns, of all experts together.
+// Where there are few, the written-out form pays for launches that do not fill the chip and the rule is wrong: plain product, K 4096,
+// groups of 128, 1024 / 4096 rows an expert: 1 expert, N 256 33 / 130 and 70 / 138, N 2816 44 / 136 and 158 / 119; 8 experts, N 256
+// 130 / 154 and 611 / 243, N 1024 159 / 152 and 620 / 369; K 14336, 1 expert, N 256 95 / 228 and 191 / 280.  (A caller who has such
+// a matrix gives no room: 0 wide_bytes.)  And it is one decision for the launch: the experts of a skewed batch share it.
 static long long wide_rows(int group) { return group == 128 ? 512 : (group == 64 ? 448 : 384); }
 // Row tiles of the one kernel for the experts that have rows but the first `left_out` of them: those of the sizes, or at most one
 // short one for every expert with rows.
