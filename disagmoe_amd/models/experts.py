@@ -15,6 +15,12 @@ from ..grouped_gemm import ops as gops
 MAX_BATCH_SIZE = 256  # disagmoe/utils/constants.py:20-22
 
 
+def _warn_without_gradient(what: str, *operands: torch.Tensor) -> None:
+    """Says in the name of the caller's caller that a gradient somebody may be waiting for will not come."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in operands):
+        warnings.warn(what, stacklevel=3)
+
+
 class _GemmState:
     """State of a layer's grouped-GEMM launches (experts.py:69-77: ``get_arguments`` and the workspace).
 
@@ -99,11 +105,6 @@ class MoEExperts(_GemmState, torch.nn.Module):
         # state block of this layer's launches and where their workspace comes from (experts.py:69-77)
         self._init_gemm_state(dev, getattr(self, "_workspace_arg", None), getattr(self, "_own_workspace_arg", False))
 
-    def _warn_without_gradient(self, rows: torch.Tensor) -> None:
-        """Says that a gradient somebody may be waiting for will not come."""
-        if torch.is_grad_enabled() and (rows.requires_grad or self.w13_weight.requires_grad or self.w2_weight.requires_grad):
-            warnings.warn("this form of MoEExperts has no gradient: forward_train has", stacklevel=3)
-
     def forward(self, bs: int, hiddens: torch.Tensor, batch_sizes: torch.Tensor,
                 host_batch_sizes: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``gmm(silu(u[:, :I]) * u[:, I:], w2)`` with ``u = gmm(hiddens, w13)``
@@ -113,7 +114,7 @@ class MoEExperts(_GemmState, torch.nn.Module):
         off its CUTLASS path) or ``host_batch_sizes`` beside a device tensor let the
         library count the launch's tiles instead of estimating them.  The result has no
         gradient (a warning says so where something requires one): :meth:`forward_train`."""
-        self._warn_without_gradient(hiddens)
+        _warn_without_gradient("this form of MoEExperts has no gradient: forward_train has", hiddens, self.w13_weight, self.w2_weight)
         ws = dict(self._gemm_state(), host_batch_sizes=host_batch_sizes)
         if self.enable_cache and bs <= self.gmm_cache_max_batch_size and hiddens.shape[0] <= self.cache_up.shape[0]:
             h = gg.gmm_swiglu(hiddens, self.w13_weight, batch_sizes, c=self.cache_up, **ws)[:hiddens.shape[0]]
@@ -127,7 +128,7 @@ class MoEExperts(_GemmState, torch.nn.Module):
         and ``row_token [R]`` (``ops.memory.route_tokens_with_sources``) instead of the
         expert-sorted copy ``hiddens [R, d]``: the gate-up kernel reads row ``row_token[r]`` of
         ``x``, and the permute in front of the FFN (engine.py:671-680) is never launched."""
-        self._warn_without_gradient(x)
+        _warn_without_gradient("this form of MoEExperts has no gradient: forward_train has", x, self.w13_weight, self.w2_weight)
         ws = dict(self._gemm_state(), host_batch_sizes=host_batch_sizes)
         h = gg.gmm_swiglu_rows(x, row_token, self.w13_weight, batch_sizes, **ws)
         return gg.gmm(h, self.w2_weight, batch_sizes, **ws)
@@ -204,6 +205,7 @@ class MoEExpertsFP8(_GemmState, torch.nn.Module):
 
     def forward(self, bs: int, hiddens: torch.Tensor, batch_sizes: torch.Tensor,
                 host_batch_sizes: Optional[torch.Tensor] = None) -> torch.Tensor:
+        _warn_without_gradient("MoEExpertsFP8 has no gradient", hiddens)
         xq, xs = gg.quantize_rows(hiddens)
         return self.forward_quantized(bs, xq, xs, batch_sizes, host_batch_sizes)
 
@@ -238,7 +240,9 @@ class MoEExpertsW4(_GemmState, torch.nn.Module):
 
     def forward(self, bs: int, hiddens: torch.Tensor, batch_sizes: torch.Tensor,
                 host_batch_sizes: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """``MoEExperts.forward`` on the 4-bit weights: expert-sorted rows ``[R, d]`` to ``[R, d]``."""
+        """``MoEExperts.forward`` on the 4-bit weights: expert-sorted rows ``[R, d]`` to ``[R, d]``, without
+        a gradient like there."""
+        _warn_without_gradient("MoEExpertsW4 has no gradient", hiddens)
         ws = dict(self._gemm_state(), host_batch_sizes=host_batch_sizes)
         d, inter = self.hidden_size, self.intermediate_size
         w13 = gg.W4Weight(self.w13_codes, self.w13_scales, self.w13_zeros, d, 2 * inter, self._group13)

@@ -52,3 +52,28 @@ def test_forms_without_a_gradient_say_so(layer):
     layer.w2_weight.requires_grad_(False)
     layer.w13_weight.requires_grad_()
     both(x, True)
+
+
+@pytest.mark.parametrize("kind", ["MoEExpertsW4", "MoEExpertsFP8"])
+def test_quantised_experts_say_so_too(monkeypatch, kind):
+    """Frozen experts of few bits in the middle of something that is trained: the rows' gradient ends there."""
+    monkeypatch.setattr(experts._GemmState, "_gemm_state", lambda self: {})
+    monkeypatch.setattr(experts._GemmState, "__del__", lambda self: None)
+    for name in ("gmm_w4", "gmm_w4_swiglu"):
+        monkeypatch.setattr(gg, name, lambda a, w, n, **kw: a.detach())
+    monkeypatch.setattr(gg, "quantize_rows", lambda x: (x.detach(), torch.ones(4)))
+    for name in ("gmm_fp8", "gmm_fp8_swiglu"):
+        monkeypatch.setattr(gg, name, lambda a, s, b, t, n, **kw: a)
+    m = getattr(experts, kind).__new__(getattr(experts, kind))
+    torch.nn.Module.__init__(m)
+    m.hidden_size = m.intermediate_size = 8
+    m._group13 = m._group2 = 32
+    for w in ("w13", "w2"):
+        for t in ("codes", "scales", "zeros", "q", "scale"):
+            m.register_buffer(f"{w}_{t}", torch.zeros(1))
+    x, n = torch.zeros(4, 8), torch.tensor([1, 3])
+    for v, expect in ((x, 0), (x.clone().requires_grad_(), 1)):
+        with warnings.catch_warnings(record=True) as said:
+            warnings.simplefilter("always")
+            m.forward(4, v, n)
+        assert len(said) == expect and all(w.filename == __file__ and kind in str(w.message) for w in said)
